@@ -159,6 +159,8 @@ def _own(s):
         mb.gemm_grouped_(s["d_a"], s["d"], s["b"].transpose(1, 2), s["offsets"])
         mb.gemm_grouped_grad_(s["d_b"], s["d"], s["a"], s["offsets"])
         return {"d_a": s["d_a"], "d_b": s["d_b"]}
+    if s["c"].dtype == torch.float32:  # a Float32 sum is added to in place, as the plain form does
+        return {"d": mb.gemm_lora_(s["c"], s["x"], s["a"], s["b"], s["which"], s["offsets"], scales=s["scales"])}
     return {"d": mb.gemm_lora_(s["d"], s["x"], s["a"], s["b"], s["which"], s["offsets"], scales=s["scales"], C=s["c"])}
 
 
