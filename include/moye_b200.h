@@ -281,6 +281,65 @@ int moye_b200_gemm_skinny_static_status(void* stream, int32_t* site);
  * rounding to the element type.  X may be Y. */
 int moye_b200_axpby(moye_handle_t h, const moye_tensor_t* Y, const moye_tensor_t* X, float a, float b, void* stream);
 
+/* ---- rows that choose their own weights: rows sorted by group, products of row groups, low-rank adapters --------
+ * None of these has a counterpart in the reference.  Whole numbers are int32 device arrays, contiguous.  Numbers read
+ * on the device (choices, borders, adapter numbers) may hold anything: what is out of range is skipped as described,
+ * never followed. */
+
+/* Sorts the choices of `tokens` rows by group, on the device, stably and without atomics between runs' results.
+ * ids (tokens) or (tokens, choices), 32- or 64-bit integers (MOYE_S32 / MOYE_U64 read as signed), any strides; the
+ * choice j of token t is entry t * choices + j.  An id outside 0..groups-1 is dropped.  groups <= 1024.
+ *   order[p]    the entry at sorted position p; -1 from offsets[groups] on           (tokens * choices)
+ *   offsets[g]  first position of group g; offsets[groups] = entries kept            (groups + 1)
+ *   inverse[e]  position of entry e, -1 if it was dropped                            (tokens * choices) */
+int moye_b200_group_rows(moye_handle_t h, const moye_tensor_t* ids, int32_t groups, int32_t* order, int32_t* offsets,
+                         int32_t* inverse, void* stream);
+
+/* dst[inverse[t*choices + j]] = src[t]: every token's row to the positions of its choices.  src (tokens, width), dst
+ * (tokens * choices, width), contiguous rows, any element type of 1, 2, 4 or 8 bytes.  Rows of dst at which nothing
+ * arrives are left as they were.  dst and src must not overlap. */
+int moye_b200_gather_rows(moye_handle_t h, const moye_tensor_t* dst, const moye_tensor_t* src, const int32_t* inverse,
+                          int32_t choices, void* stream);
+
+/* dst[t] = sum_j weights[t,j] * src[inverse[t*choices + j]], dropped choices left out (all dropped: a row of zeros);
+ * summed in fp32 in the order of j, one rounding.  weights (tokens, choices) f32, f16 or bf16, any strides, or NULL
+ * for 1: then this is the gradient of moye_b200_gather_rows.  f32, f16, bf16 rows. */
+int moye_b200_combine_rows(moye_handle_t h, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
+                           const int32_t* inverse, int32_t choices, void* stream);
+
+/* The gradient of moye_b200_combine_rows: dsrc[inverse[t*choices + j]] = weights[t,j] * ddst[t] (other rows of dsrc are
+ * left as they were) and dweights[t,j] = <ddst[t], src[inverse[t*choices + j]]> (0 for a dropped choice), in fp32. */
+int moye_b200_combine_rows_grad(moye_handle_t h, const moye_tensor_t* dsrc, const moye_tensor_t* dweights,
+                                const moye_tensor_t* ddst, const moye_tensor_t* src, const moye_tensor_t* weights,
+                                const int32_t* inverse, int32_t choices, void* stream);
+
+/* D[i] = alpha * A[i] . B[g]^T + beta * D[i] for the rows offsets[g] <= i < offsets[g+1]; other rows of D are left as
+ * they were, and D is not read when beta == 0.  A (rows, K), B (groups, N, K), D (rows, N); offsets: groups + 1 borders
+ * on the device, not decreasing (clamped to the rows; a border that runs backwards makes an empty group); groups <= 1024.
+ * f16 or bf16 operands, fp32 accumulation, D f32 or the operands' type.  A: contiguous rows; B: unit stride along K, or
+ * along N (the swapped view of a (groups, K, N) array: dA = dD . B, the gradient of A); base and pitches of A and B
+ * multiples of 16 bytes.  D: contiguous rows, any pitch. */
+int moye_b200_gemm_grouped(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* A, const moye_tensor_t* B,
+                           const int32_t* offsets, float alpha, float beta, void* stream);
+
+/* The gradient of the weights: dB[g] = alpha * sum over the rows i of group g of dD[i]^T A[i], + beta * dB[g].  Every
+ * dB[g] is written: an empty group's becomes beta * dB[g].  Rows behind offsets[groups] are not used, whatever they
+ * hold.  A (rows, K) and dD (rows, N) f16 or bf16, contiguous rows, base and pitch multiples of 16 bytes; dB
+ * (groups, N, K) f32 or the operands' type. */
+int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
+                                const int32_t* offsets, float alpha, float beta, void* stream);
+
+/* Low-rank adapters of many requests: D[i] = C[i] + scales[a] * (X[i] . A[a]^T) . B[a]^T, where a = adapters[q] and q
+ * is the request with offsets[q] <= i < offsets[q+1] (borders not decreasing), or q = i when offsets is NULL (then
+ * requests = rows).  X (rows, K), A (count, R, K), B (count, N, R), C and D (rows, N).  An adapter number outside
+ * 0..count-1 means none: D[i] = C[i].  Rows outside every request are left as they were.  C NULL or C = D: in place.
+ * scales: one float per adapter, or NULL for 1.  The product of rank R stays in fp32 or an equivalent split.  X, A, B
+ * all f16 or all bf16; C and D both f32 or both the operands' type; R a multiple of 8 from 8 to 128 (pad with zeros),
+ * K a multiple of 8; base and pitches of X, A, B multiples of 16 bytes. */
+int moye_b200_gemm_lora(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* X, const moye_tensor_t* A,
+                        const moye_tensor_t* B, const moye_tensor_t* C, const int32_t* adapters, const int32_t* offsets,
+                        int32_t requests, const float* scales, void* stream);
+
 /* ---- several GPUs: one process (or thread) per GPU, each with its own handle ------------------------------------
  * The reference has no multi-GPU code.  The hot path shards without any exchange: GEMM along M (rows of A and D, B
  * replicated), weight-bound products along N (rows of W, columns of Y), copies along row blocks; every rank calls

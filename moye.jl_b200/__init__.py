@@ -11,6 +11,7 @@ from .layout import *  # noqa: F401,F403
 from .array import *  # noqa: F401,F403
 from .atom import *  # noqa: F401,F403
 from .algorithm import *  # noqa: F401,F403
+from .grouped import *  # noqa: F401,F403
 from .sharding import *  # noqa: F401,F403
 from .host_pipeline import *  # noqa: F401,F403
 from .printing import *  # noqa: F401,F403

@@ -6,6 +6,7 @@ visible when a handle is requested, the call raises.
 """
 import ctypes
 import os
+import struct
 import threading
 
 MAX_RANK = 4
@@ -96,6 +97,14 @@ EXPORTS = {
     "moye_b200_ldsm_copy": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
                                            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                            ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), ctypes.c_void_p]),
+    # descriptors of the row-group calls are packed bytes (see pack_tensor), hence plain pointers
+    "moye_b200_group_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32] + [ctypes.c_void_p] * 4),
+    "moye_b200_gather_rows": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int32, ctypes.c_void_p]),
+    "moye_b200_combine_rows": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int32, ctypes.c_void_p]),
+    "moye_b200_combine_rows_grad": (ctypes.c_int, [ctypes.c_void_p] * 7 + [ctypes.c_int32, ctypes.c_void_p]),
+    "moye_b200_gemm_grouped": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_float, ctypes.c_float, ctypes.c_void_p]),
+    "moye_b200_gemm_grouped_grad": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_float, ctypes.c_float, ctypes.c_void_p]),
+    "moye_b200_gemm_lora": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
     "moye_b200_layout_eval": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlatLayout), ctypes.c_int64,
                                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
 }
@@ -156,6 +165,15 @@ def make_tensor(ptr, dtype, shape, stride):
         t.shape[i] = s
         t.stride[i] = d
     return t
+
+
+_PACKERS = [None] + [struct.Struct(f"<Qii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(1, MAX_RANK + 1)]
+
+
+def pack_tensor(ptr, dtype, shape, stride):
+    """`make_tensor` as the bytes of a moye_tensor_t, which a call takes by pointer: a third of the cost of filling the
+    ctypes structure, for entry points whose descriptors are made anew on every call."""
+    return _PACKERS[len(shape)].pack(ptr, dtype, len(shape), *shape, *stride)
 
 
 def make_flat_layout(shape, stride):

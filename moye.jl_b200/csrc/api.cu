@@ -155,6 +155,26 @@ int encode_tmap_2d_uncached(CUtensorMap* out, const void* ptr, int dtype, uint64
   return MOYE_OK;
 }
 
+// A rank-3 map of 16-bit elements with the 128-byte swizzle and a box one deep along the outermost mode (the group).
+int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1, uint64_t dim2,
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) MOYE_FAIL(MOYE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  CUtensorMapDataType tdt;
+  if (!tmap_dtype(dtype, &tdt)) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "dtype %d has no tensor-map type", dtype);
+  cuuint64_t dims[3] = {dim0, dim1, dim2};
+  cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
+  cuuint32_t box[3] = {box0, box1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(out, tdt, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    MOYE_FAIL(MOYE_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d (dims %llu x %llu x %llu, pitches %llu, %llu)", (int)r,
+              (unsigned long long)dim0, (unsigned long long)dim1, (unsigned long long)dim2, (unsigned long long)stride1_bytes,
+              (unsigned long long)stride2_bytes);
+  return MOYE_OK;
+}
+
 // The skinny kernel's scratch is allocated once, at the size its widest instantiation needs, so that no launch
 // ever has to synchronise the device to free and re-allocate it.
 int ensure_workspace(moye_b200_ctx* h, size_t bytes) {
@@ -324,6 +344,64 @@ int moye_b200_axpby(moye_handle_t h, const moye_tensor_t* Y, const moye_tensor_t
   if (int rc = check_handle(h)) return rc;
   if (!Y || !X) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "Y and X must be non-null");
   return launch_axpby(h, Y, X, a, b, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_group_rows(moye_handle_t h, const moye_tensor_t* ids, int32_t groups, int32_t* order, int32_t* offsets,
+                         int32_t* inverse, void* stream) {
+  NvtxRange range("moye_b200_group_rows");
+  if (int rc = check_handle(h)) return rc;
+  if (!ids) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "ids must be non-null");
+  return launch_group_rows(h, ids, groups, order, offsets, inverse, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_gather_rows(moye_handle_t h, const moye_tensor_t* dst, const moye_tensor_t* src, const int32_t* inverse,
+                          int32_t choices, void* stream) {
+  NvtxRange range("moye_b200_gather_rows");
+  if (int rc = check_handle(h)) return rc;
+  if (!dst || !src) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "dst and src must be non-null");
+  return launch_gather_rows(h, dst, src, inverse, choices, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_combine_rows(moye_handle_t h, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
+                           const int32_t* inverse, int32_t choices, void* stream) {
+  NvtxRange range("moye_b200_combine_rows");
+  if (int rc = check_handle(h)) return rc;
+  if (!dst || !src) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "dst and src must be non-null");
+  return launch_combine_rows(h, dst, src, weights, inverse, choices, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_combine_rows_grad(moye_handle_t h, const moye_tensor_t* dsrc, const moye_tensor_t* dweights,
+                                const moye_tensor_t* ddst, const moye_tensor_t* src, const moye_tensor_t* weights,
+                                const int32_t* inverse, int32_t choices, void* stream) {
+  NvtxRange range("moye_b200_combine_rows_grad");
+  if (int rc = check_handle(h)) return rc;
+  if (!dsrc || !dweights || !ddst || !src || !weights) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "every array must be non-null");
+  return launch_combine_rows_grad(h, dsrc, dweights, ddst, src, weights, inverse, choices, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_gemm_grouped(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* A, const moye_tensor_t* B,
+                           const int32_t* offsets, float alpha, float beta, void* stream) {
+  NvtxRange range("moye_b200_gemm_grouped");
+  if (int rc = check_handle(h)) return rc;
+  if (!D || !A || !B) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "D, A and B must be non-null");
+  return launch_gemm_grouped(h, D, A, B, offsets, alpha, beta, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
+                                const int32_t* offsets, float alpha, float beta, void* stream) {
+  NvtxRange range("moye_b200_gemm_grouped_grad");
+  if (int rc = check_handle(h)) return rc;
+  if (!dB || !dD || !A) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "dB, dD and A must be non-null");
+  return launch_gemm_grouped_grad(h, dB, dD, A, offsets, alpha, beta, static_cast<cudaStream_t>(stream));
+}
+
+int moye_b200_gemm_lora(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* X, const moye_tensor_t* A,
+                        const moye_tensor_t* B, const moye_tensor_t* C, const int32_t* adapters, const int32_t* offsets,
+                        int32_t requests, const float* scales, void* stream) {
+  NvtxRange range("moye_b200_gemm_lora");
+  if (int rc = check_handle(h)) return rc;
+  if (!D || !X || !A || !B) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "D, X, A and B must be non-null");
+  return launch_gemm_lora(h, D, X, A, B, C, adapters, offsets, requests, scales, static_cast<cudaStream_t>(stream));
 }
 
 int moye_b200_layout_copy(moye_handle_t h, void* dst, const moye_layout_t* dl, const void* src,

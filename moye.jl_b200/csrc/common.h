@@ -156,6 +156,9 @@ int make_tmap_2d(moye_b200_ctx* h, CUtensorMap* out, const void* ptr, int dtype,
 int encode_tmap_2d_uncached(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1,
                             uint64_t stride1_bytes, uint32_t box0, uint32_t box1, bool swizzle128);
 
+int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1, uint64_t dim2,
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1);
+
 // Raises a kernel's dynamic shared-memory limit the first time this handle launches it.
 template <typename K>
 inline int configure_once(moye_b200_ctx* h, K kernel, int smem_bytes) {
@@ -188,6 +191,22 @@ int launch_copy(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_tensor_t*
 int launch_transpose(moye_b200_ctx* h, void* dst, int64_t dst_pitch, const void* src, int64_t src_pitch, int dtype,
                      int64_t m, int64_t n, cudaStream_t stream);
 int launch_axpby(moye_b200_ctx* h, const moye_tensor_t* Y, const moye_tensor_t* X, float a, float b, cudaStream_t stream);
+int launch_group_rows(moye_b200_ctx* h, const moye_tensor_t* ids, int groups, int* order, int* offsets, int* inverse,
+                      cudaStream_t stream);
+int launch_gather_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_tensor_t* src, const int* inverse, int choices,
+                       cudaStream_t stream);
+int launch_combine_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
+                        const int* inverse, int choices, cudaStream_t stream);
+int launch_combine_rows_grad(moye_b200_ctx* h, const moye_tensor_t* dsrc, const moye_tensor_t* dweights, const moye_tensor_t* ddst,
+                             const moye_tensor_t* src, const moye_tensor_t* weights, const int* inverse, int choices,
+                             cudaStream_t stream);
+int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor_t* A, const moye_tensor_t* B, const int* offsets,
+                        float alpha, float beta, cudaStream_t stream);
+int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
+                             const int* offsets, float alpha, float beta, cudaStream_t stream);
+int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor_t* X, const moye_tensor_t* A,
+                     const moye_tensor_t* B, const moye_tensor_t* C, const int* adapters, const int* offsets, int requests,
+                     const float* scales, cudaStream_t stream);
 int launch_layout_copy(moye_b200_ctx* h, void* dst, const moye_layout_t* dl, const void* src,
                        const moye_layout_t* sl, int elem_bytes, cudaStream_t stream);
 int launch_layout_eval(moye_b200_ctx* h, const moye_layout_t* l, int64_t first, int64_t n, int64_t* out,

@@ -1,0 +1,476 @@
+// Products of row groups: rows [offsets[g], offsets[g+1]) of A meet the weight B[g] of their group.
+//
+//   forward   D[i]  = alpha * A[i] . B[g]^T + beta * D[i]         A (rows, K), B (G, N, K), D (rows, N)
+//             (B seen as (G, K, N) with its last two modes swapped gives dA = dD . B, the gradient of the rows)
+//   gradient  dB[g] = alpha * sum_{i in g} dD[i]^T A[i] + beta * dB[g]
+//
+// The group borders are read on the device: nothing waits for the host, and a captured launch follows new borders.
+// The reference has no counterpart; the arithmetic per group is its `gemm!` (src/algorithm/blas.jl:39-88).
+//
+// The accumulator is turned against the dense kernels': the tensor-memory lanes (the M of the instruction, always full)
+// run along the output's contiguous mode -- the weight's rows in the forward product, the features of A in the
+// gradient -- and the columns (its N, 16 to 256) along the rows of the group or of the weight.  A group of a few rows
+// then costs a narrow instruction instead of a 128-row tile that is mostly padding, the last tile of a group simply
+// stores fewer columns, and a warp's 32 lanes store 32 neighbouring elements.
+//
+// Persistent CTAs of 6 warps as in the dense kernels: warp 0 TMA producer, warp 1 tcgen05.mma issuer, warps 2-5
+// epilogue, accumulator double-buffered in tensor memory.
+#include <cstring>
+
+#include "gemm_common.cuh"
+
+namespace moye {
+
+constexpr int kMaxGemmGroups = 1024;
+enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164 };
+enum : int { GROUPED_K_MAJOR = 0, GROUPED_MN_MAJOR = 1, GROUPED_GRAD = 2 };
+
+struct GroupedArgs {
+  int rows, groups;
+  int lanes;            // extent of the output's contiguous mode (N forward, K gradient)
+  int cols;             // gradient: extent of the other mode (N)
+  int k_blocks;         // forward: blocks of 64 along K
+  int lane_tiles, col_tiles;
+  const int* offsets;
+  uint32_t idesc;
+  float alpha, beta;
+  void* D;
+  long long ld, group_stride;  // elements
+  int* status;
+};
+
+struct GroupedTile {
+  int g, row0, nrows;  // the group, its first row here and the rows of it this tile reads (gradient: all of them)
+  int lane0, col0;     // first output element along the two modes (forward: col0 = row0)
+};
+
+template <int MODE, int BT>
+struct GroupedSchedule {
+  const GroupedArgs& a;
+  const int* row_of;   // [groups + 1] first rows, clamped to the array and not decreasing
+  const int* before;   // [groups + 1] column tiles of the groups before (forward)
+  __device__ __forceinline__ int total() const {
+    return MODE == GROUPED_GRAD ? a.groups * a.lane_tiles * a.col_tiles : before[a.groups] * a.lane_tiles;
+  }
+  __device__ __forceinline__ GroupedTile at(int t) const {
+    GroupedTile r;
+    if (MODE == GROUPED_GRAD) {
+      const int per = a.lane_tiles * a.col_tiles;
+      r.g = t / per;
+      const int q = t - r.g * per;
+      r.lane0 = (q % a.lane_tiles) * 128;
+      r.col0 = (q / a.lane_tiles) * BT;
+      r.row0 = row_of[r.g];
+      r.nrows = row_of[r.g + 1] - r.row0;
+    } else {
+      int lo = 0, hi = a.groups;  // the group whose tiles hold t: before[lo] * lane_tiles <= t < before[lo + 1] * lane_tiles
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] * a.lane_tiles <= t) lo = mid;
+        else hi = mid;
+      }
+      r.g = lo;
+      const int q = t - before[lo] * a.lane_tiles, tiles = before[lo + 1] - before[lo];
+      r.lane0 = (q / tiles) * 128;
+      r.row0 = row_of[lo] + (q % tiles) * BT;
+      r.nrows = min(BT, row_of[lo + 1] - r.row0);
+      r.col0 = r.row0;
+    }
+    return r;
+  }
+  __device__ __forceinline__ int k_blocks(const GroupedTile& r) const {
+    return MODE == GROUPED_GRAD ? (r.nrows + 63) >> 6 : a.k_blocks;
+  }
+};
+
+// First rows and column-tile counts of all groups, by one warp.  Borders outside the arrays or running backwards are a
+// caller's mistake that must not become a bad address: they are clamped, such groups come out empty.
+template <int BT>
+__device__ __forceinline__ void grouped_borders(const GroupedArgs& a, int* row_of, int* before, int lane) {
+  int last = 0, tiles = 0;
+  for (int g0 = 0; g0 <= a.groups; g0 += 32) {
+    const int g = g0 + lane;
+    int v = g <= a.groups ? min(max(__ldg(a.offsets + g), 0), a.rows) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, v, d);
+      if (lane >= d) v = max(v, up);
+    }
+    v = max(v, last);
+    int prev = __shfl_up_sync(~0u, v, 1);
+    if (lane == 0) prev = g0 == 0 ? v : last;
+    // this lane's entry of `before` counts the tiles of the groups up to g - 1
+    int c = g == 0 || g > a.groups ? 0 : (v - prev + BT - 1) / BT;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, c, d);
+      if (lane >= d) c += up;
+    }
+    if (g <= a.groups) {
+      row_of[g] = v;
+      before[g] = tiles + c;
+    }
+    tiles += __shfl_sync(~0u, c, 31);
+    last = __shfl_sync(~0u, v, 31);
+  }
+}
+
+template <int MODE, typename OutT, int BT, int STAGES>
+__global__ void __launch_bounds__(192, 1)
+gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC, const GroupedArgs a) {
+  // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD)
+  constexpr int BK = 64, UMMA_K = 16;
+  constexpr int L_BYTES = 128 * 128;
+  constexpr int C_BYTES = BT * 128;
+  constexpr int STAGE_BYTES = L_BYTES + C_BYTES;
+  constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
+  constexpr bool L_MN = MODE != GROUPED_K_MAJOR, C_MN = MODE == GROUPED_GRAD;
+  constexpr int CHUNK = BT < 32 ? BT : 32;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* acc_full = bars + 2 * STAGES;
+  uint64_t* acc_empty = bars + 2 * STAGES + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  int* row_of = reinterpret_cast<int*>(tmem_holder + 2);
+  int* before = row_of + kMaxGemmGroups + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    fence_mbar_init();
+    if (a.rows > 0) {  // without rows the maps are not set up, and nothing is loaded
+      prefetch_tensormap(&tmL);
+      prefetch_tensormap(&tmC);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, TMEM_COLS);
+    tmem_relinquish();
+  }
+  griddep_launch();  // programmatic dependent launch: see launch_dependent(); nothing above touches global memory
+  griddep_wait();
+  if (warp == 2) grouped_borders<BT>(a, row_of, before, lane);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
+  const GroupedSchedule<MODE, BT> sched{a, row_of, before};
+  const int num_tiles = sched.total();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        const GroupedTile tile = sched.at(t);
+        const int kbs = sched.k_blocks(tile);
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, a.status, SITEG_PROD_EMPTY)) { ok = false; break; }
+          mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
+          uint8_t* sl = smem + stage * STAGE_BYTES;
+          uint8_t* sc = sl + L_BYTES;
+          if constexpr (MODE == GROUPED_K_MAJOR) {
+            tma_load_3d(sl, &tmL, &full[stage], kb * BK, tile.lane0, tile.g);
+          } else if constexpr (MODE == GROUPED_MN_MAJOR) {
+            for (int c = 0; c < 2; ++c) tma_load_3d(sl + c * (BK * 128), &tmL, &full[stage], tile.lane0 + c * 64, kb * BK, tile.g);
+          } else {
+            for (int c = 0; c < 2; ++c) tma_load_2d(sl + c * (BK * 128), &tmL, &full[stage], tile.lane0 + c * 64, tile.row0 + kb * BK);
+          }
+          if constexpr (C_MN) {
+            for (int c = 0; c < BT / 64; ++c) tma_load_2d(sc + c * (BK * 128), &tmC, &full[stage], tile.col0 + c * 64, tile.row0 + kb * BK);
+          } else {
+            tma_load_2d(sc, &tmC, &full[stage], kb * BK, tile.row0);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    int stage = 0;
+    uint32_t phase = 0;
+    int lt = 0;
+    bool ok = true;
+    const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
+    for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+      const GroupedTile tile = sched.at(t);
+      const int kbs = sched.k_blocks(tile);
+      if (kbs == 0) continue;
+      const int buf = lt & 1;
+      const uint32_t aphase = (lt >> 1) & 1;
+      ++lt;
+      if (lane == 0) ok = mbar_wait(&acc_empty[buf], aphase ^ 1, a.status, SITEG_MMA_ACC);
+      ok = __shfl_sync(~0u, ok, 0);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + buf * BT;
+      for (int kb = 0; kb < kbs; ++kb) {
+        if (lane == 0) ok = mbar_wait(&full[stage], phase, a.status, SITEG_MMA_FULL);
+        ok = __shfl_sync(~0u, ok, 0);
+        if (!ok) break;
+        uint8_t* sl = smem + stage * STAGE_BYTES;
+        if constexpr (MODE == GROUPED_GRAD) {
+          // The last block of a group reaches into the next group's rows (or past the last one, where anything may
+          // lie): their K rows are zeroed in both operands.  A K row is 128 bytes in every chunk, swizzled in itself.
+          const int valid = tile.nrows - kb * BK;
+          if (valid < BK) {
+            for (int c = 0; c < 2 + BT / 64; ++c)
+              for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
+                *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (lane == 0) {
+          tc_fence_after_sync();
+          const uint32_t s = smem_u32(sl);
+          const uint64_t ld = dl.base + (s >> 4), cd = dc.base + ((s + L_BYTES) >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            tc_mma_ss<KIND_F16>(d_tmem, ld + k * dl.kstep, cd + k * dc.kstep, a.idesc, (kb | k) != 0 ? 1u : 0u);
+          tc_commit(&empty[stage]);
+          if (kb == kbs - 1) tc_commit(&acc_full[buf]);
+        }
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..5)
+    const int q = warp & 3;
+    int lt = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+      const GroupedTile tile = sched.at(t);
+      const int kbs = sched.k_blocks(tile);
+      const int buf = lt & 1;
+      const uint32_t aphase = (lt >> 1) & 1;
+      if (kbs != 0) {
+        ++lt;
+        if (!mbar_wait(&acc_full[buf], aphase, a.status, SITEG_EPI_ACC)) break;
+        tc_fence_after_sync();
+      }
+      const int m = tile.lane0 + q * 32 + lane;
+      const int ncols = MODE == GROUPED_GRAD ? min(BT, a.cols - tile.col0) : tile.nrows;
+      OutT* out = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld + m;
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT;
+#pragma unroll 1
+      for (int c = 0; c < BT; c += CHUNK) {
+        uint32_t v[CHUNK];
+        if (kbs != 0) {
+          if constexpr (CHUNK == 32) tmem_ld_x32(t_addr + c, v);
+          else tmem_ld_x16(t_addr + c, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] = 0u;
+        }
+        if (kbs != 0 && c + CHUNK >= BT) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+        if (m < a.lanes) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            if (c + j < ncols) {
+              OutT* p = out + (c + j) * a.ld;
+              float x = __uint_as_float(v[j]) * a.alpha;
+              if (a.beta != 0.f) x += a.beta * load_c_as_float<OutT>(p, 0);
+              *p = cvt_out<OutT>(x);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  if (*reinterpret_cast<volatile int*>(a.status) != 0) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // a wait gave up: copies in flight get time to land
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+template <int MODE, typename OutT, int BT>
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a, long long tiles,
+                               cudaStream_t stream) {
+  constexpr int EXTRA = 1024 + 512 + 2 * (kMaxGemmGroups + 1) * 4;
+  constexpr int STAGE = 128 * 128 + BT * 128;
+  constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE < 12 ? (227 * 1024 - EXTRA) / STAGE : 12;
+  constexpr int SMEM = STAGES * STAGE + EXTRA;
+  auto kern = gemm_grouped_kernel<MODE, OutT, BT, STAGES>;
+  if (int rc = configure_once(h, kern, SMEM)) return rc;
+  const unsigned grid = (unsigned)(tiles < h->num_sms ? tiles : h->num_sms);
+  MOYE_CUDA(launch_dependent(kern, dim3(grid), dim3(192), SMEM, stream, tl, tc, a));
+  return MOYE_OK;
+}
+
+template <int MODE, typename OutT>
+static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a,
+                             long long tiles, cudaStream_t stream) {
+  if constexpr (MODE != GROUPED_GRAD) {
+    if (bt == 16) return launch_grouped_inst<MODE, OutT, 16>(h, tl, tc, a, tiles, stream);
+    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, a, tiles, stream);
+  }
+  if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, a, tiles, stream);
+  if (bt == 128) return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, a, tiles, stream);
+  return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, a, tiles, stream);
+}
+
+template <int MODE>
+static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a,
+                              long long tiles, cudaStream_t stream) {
+  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, a, tiles, stream);
+  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, a, tiles, stream);
+}
+
+static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
+  if ((x->dtype != MOYE_F16 && x->dtype != MOYE_BF16) || y->dtype != x->dtype)
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "%s: operands must both be f16 or both bf16 (got %d, %d)", who, x->dtype, y->dtype);
+  if (out->dtype != MOYE_F32 && out->dtype != x->dtype)
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "%s: the output must be f32 or the operands' type (got %d)", who, out->dtype);
+  return MOYE_OK;
+}
+
+// A matrix of rows read by TMA: contiguous rows, base and pitch on 16 bytes.
+static int check_row_operand(const char* who, const char* what, const moye_tensor_t* t) {
+  if (t->shape[1] > 1 && t->stride[1] != 1) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows of %s must be contiguous", who, what);
+  if (t->shape[0] > 1 && t->stride[0] < t->shape[1]) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows of %s overlap", who, what);
+  if ((reinterpret_cast<uintptr_t>(t->ptr) & 15) != 0 || (t->shape[0] > 1 && (t->stride[0] * 2) % 16 != 0))
+    MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: %s needs a base and a row pitch that are multiples of 16 bytes", who, what);
+  return MOYE_OK;
+}
+
+static int check_borders(const char* who, const int* offsets, int groups) {
+  if (groups < 1 || groups > kMaxGemmGroups)
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d groups (got %d)", who, kMaxGemmGroups, groups);
+  if (!offsets) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: null offsets", who);
+  return MOYE_OK;
+}
+
+int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor_t* A, const moye_tensor_t* B, const int* offsets,
+                        float alpha, float beta, cudaStream_t stream) {
+  const char* who = "gemm_grouped";
+  if (D->rank != 2 || A->rank != 2 || B->rank != 3) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: D and A must be rank 2, B rank 3", who);
+  const int64_t R = A->shape[0], K = A->shape[1], G = B->shape[0], N = B->shape[1];
+  if (B->shape[2] != K || D->shape[0] != R || D->shape[1] != N)
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: shape mismatch: A (%lld,%lld) B (%lld,%lld,%lld) D (%lld,%lld)", who, (long long)R,
+              (long long)K, (long long)G, (long long)N, (long long)B->shape[2], (long long)D->shape[0], (long long)D->shape[1]);
+  if (int rc = check_grouped_types(who, A, B, D)) return rc;
+  if (R < 0 || N <= 0 || K <= 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: empty product", who);
+  if (R > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
+  if (int rc = check_borders(who, offsets, (int)(G > INT32_MAX ? INT32_MAX : G))) return rc;
+  if (R == 0) return MOYE_OK;
+  if (!A->ptr || !B->ptr || !D->ptr) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: null data pointer", who);
+  if (int rc = check_row_operand(who, "A", A)) return rc;
+  if ((N > 1 && D->stride[1] != 1) || (R > 1 && D->stride[0] < N))
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows of D must be contiguous and must not overlap", who);
+  const bool mn = K > 1 ? B->stride[2] != 1 : (B->stride[1] == 1 && N > 1);
+  const int64_t inner = mn ? N : K, outer = mn ? K : N, pitch = mn ? B->stride[2] : B->stride[1];
+  if (mn && N > 1 && B->stride[1] != 1) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: B needs a unit stride along K or along N", who);
+  if ((outer > 1 && pitch < inner) || (G > 1 && B->stride[0] < (outer - 1) * pitch + inner))
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows or groups of B overlap", who);
+  if ((reinterpret_cast<uintptr_t>(B->ptr) & 15) != 0 || (outer > 1 && pitch % 8 != 0) || (G > 1 && B->stride[0] % 8 != 0))
+    MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: B needs a base, a row pitch and a group pitch that are multiples of 16 bytes", who);
+  // Columns of a tile: the instruction width that holds an average group, so that weights are streamed once and padding
+  // stays small.
+  const int64_t mean = (R + G - 1) / G;
+  const int bt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+  GroupedArgs a = {};
+  a.rows = (int)R;
+  a.groups = (int)G;
+  a.lanes = (int)N;
+  a.k_blocks = (int)((K + 63) / 64);
+  a.lane_tiles = (int)((N + 127) / 128);
+  a.offsets = offsets;
+  const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
+  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((mn ? 1u : 0u) << 15) | ((uint32_t)(bt / 8) << 17) | (8u << 24);
+  a.alpha = alpha;
+  a.beta = beta;
+  a.D = D->ptr;
+  a.ld = D->stride[0];
+  a.status = h->d_status;
+  const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
+  if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
+  CUtensorMap tl, tc;
+  if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
+                              (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128))
+    return rc;
+  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt, true)) return rc;
+  log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 128 x %d", (long long)R, (long long)G, (long long)N,
+           (long long)K, A->dtype, bt);
+  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, a, tiles, stream);
+  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, a, tiles, stream);
+}
+
+int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
+                             const int* offsets, float alpha, float beta, cudaStream_t stream) {
+  const char* who = "gemm_grouped_grad";
+  if (dB->rank != 3 || dD->rank != 2 || A->rank != 2) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: dD and A must be rank 2, dB rank 3", who);
+  const int64_t R = A->shape[0], K = A->shape[1], G = dB->shape[0], N = dB->shape[1];
+  if (dB->shape[2] != K || dD->shape[0] != R || dD->shape[1] != N)
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: shape mismatch: A (%lld,%lld) dD (%lld,%lld) dB (%lld,%lld,%lld)", who, (long long)R,
+              (long long)K, (long long)dD->shape[0], (long long)dD->shape[1], (long long)G, (long long)N, (long long)dB->shape[2]);
+  if (int rc = check_grouped_types(who, A, dD, dB)) return rc;
+  if (R < 0 || N <= 0 || K <= 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: empty product", who);
+  if (R > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
+  if (int rc = check_borders(who, offsets, (int)(G > INT32_MAX ? INT32_MAX : G))) return rc;
+  if (!dB->ptr || (R > 0 && (!A->ptr || !dD->ptr))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: null data pointer", who);
+  if (int rc = check_row_operand(who, "A", A)) return rc;
+  if (int rc = check_row_operand(who, "dD", dD)) return rc;
+  if ((K > 1 && dB->stride[2] != 1) || (N > 1 && dB->stride[1] < K) || (G > 1 && dB->stride[0] < (N - 1) * dB->stride[1] + K))
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: dB needs contiguous rows, and rows and groups that do not overlap", who);
+  const int bt = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+  GroupedArgs a = {};
+  a.rows = (int)R;
+  a.groups = (int)G;
+  a.lanes = (int)K;
+  a.cols = (int)N;
+  a.lane_tiles = (int)((K + 127) / 128);
+  a.col_tiles = (int)((N + bt - 1) / bt);
+  a.offsets = offsets;
+  const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
+  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (3u << 15) | ((uint32_t)(bt / 8) << 17) | (8u << 24);
+  a.alpha = alpha;
+  a.beta = beta;
+  a.D = dB->ptr;
+  a.ld = dB->stride[1];
+  a.group_stride = dB->stride[0];
+  a.status = h->d_status;
+  const long long tiles = (long long)G * a.lane_tiles * a.col_tiles;
+  if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
+  CUtensorMap tl, tc;
+  if (R > 0) {
+    if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
+  } else {  // no rows: the kernel loads nothing, every group's sum is empty
+    std::memset(&tl, 0, sizeof(tl));
+    std::memset(&tc, 0, sizeof(tc));
+  }
+  log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 128 x %d", (long long)R, (long long)G,
+           (long long)N, (long long)K, A->dtype, bt);
+  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, a, tiles, stream);
+}
+
+}  // namespace moye

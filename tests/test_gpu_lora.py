@@ -1,0 +1,176 @@
+"""Low-rank adapters of many requests on the GPU: `gemm_lora_` against 64-bit products of every request.  The value is
+C + s * sum over R of (sum over K): in fp32 off by at most (K + R + 4) * 2^-23 of the sum of magnitudes; the product of
+rank R may be carried as a high and a low 16-bit part, off by 2^-16 of itself, when the output has 16 bits; the
+output rounding adds eps / 2 of the value."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+# borders (None: a request per row), rows, adapters of the requests, N, K, R, count
+CASES = [
+    (None, 1, [0], 8, 8, 8, 1),
+    (None, 5, [2, -1, 0, 7, 2], 1001, 520, 24, 3),                           # none, and a number that does not exist
+    ([0, 3, 3, 40, 41], 41, [1, 0, 0, -1], 136, 4096, 16, 2),                # an empty request, one without an adapter
+    ([2, 130, 300], 310, [3, 1], 2056, 1000, 64, 4),                         # rows before and behind every request
+    ([0, 129, 257, 700], 700, [0, 0, 2], 264, 264, 128, 3),                  # the largest rank, long requests
+    (list(range(0, 65)), 64, [i % 7 for i in range(64)], 4096, 512, 8, 7),
+    ([0, 1000], 1000, [0], 1, 16, 40, 1),
+    ([0, 1, 2, 200, 201, 460, 461], 461, [0, 1, 2, 3, 4, 5], 512, 1024, 32, 6),
+]
+
+
+def make(case, kind, dev, seed=1):
+    offsets, rows, which, n, k, rank, count = case
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s, scale=1.0: (torch.randn(*s, generator=gen, device=dev) * scale).to(DT[kind])
+    x, a, b = r(rows, k), r(count, rank, k, scale=k ** -0.5), r(count, n, rank, scale=rank ** -0.5)
+    scales = torch.rand(count, generator=gen, device=dev) + 0.5
+    edge = None if offsets is None else torch.tensor(offsets, dtype=torch.int32, device=dev)
+    return x, a, b, scales, torch.tensor(which, dtype=torch.int32, device=dev), edge
+
+
+def check(got, c, x, a, b, scales, which, offsets, out, untouched):
+    rank, k = a.shape[1:]
+    offsets = list(range(len(which) + 1)) if offsets is None else offsets
+    inside = torch.zeros(len(c), dtype=torch.bool, device=c.device)
+    for q, w in enumerate(which):
+        s = slice(offsets[q], offsets[q + 1])
+        inside[s] = True
+        if not 0 <= w < len(a):
+            assert torch.equal(got[s], c[s])
+            continue
+        f = 1.0 if scales is None else float(scales[w])
+        want = c[s].double() + f * ((x[s].double() @ a[w].double().T) @ b[w].double().T)
+        mag = f * ((x[s].double().abs() @ a[w].double().abs().T) @ b[w].double().abs().T)
+        tol = (k + rank + 4) * 2.0 ** -23 * (mag + c[s].double().abs())
+        if out != torch.float32:
+            tol = tol + 2.0 ** -16 * mag + torch.finfo(out).eps / 2 * want.abs() + torch.finfo(out).tiny * torch.finfo(out).eps
+        assert bool(((got[s].double() - want).abs() <= tol).all())
+    assert torch.equal(got[~inside], untouched[~inside])
+
+
+@pytest.mark.parametrize("out", ["same", "f32"])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_lora(mb, dev, case, kind, out):
+    offsets, rows, which, n, k, rank, count = CASES[case]
+    ot = DT[kind] if out == "same" else torch.float32
+    x, a, b, scales, w, edge = make(CASES[case], kind, dev)
+    c = torch.randn(rows, n, device=dev).to(ot)
+    d0 = torch.full_like(c, -3.0)
+    d = d0.clone()
+    assert mb.gemm_lora_(d, x, a, b, w, edge, scales=scales, C=c) is d
+    check(d, c, x, a, b, scales, which, offsets, ot, d0)
+    inplace = c.clone()
+    mb.gemm_lora_(inplace, x, a, b, w, edge)
+    check(inplace, c, x, a, b, None, which, offsets, ot, c)
+    mb.synchronize_status(dev)
+
+
+def test_pitched_views_and_moye_arrays(mb, dev):
+    offsets, which, n, k, rank = [0, 5, 200], [1, 0], 100, 64, 16
+    gen = torch.Generator(device=dev).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device=dev).to(torch.bfloat16)
+    x, a, b = r(200, 2 * k)[:, 8:8 + k], r(2, rank + 3, k + 8)[:, 1:1 + rank, 8:8 + k], r(2, n + 1, rank + 8)[:, 1:, :rank]
+    base = r(200, n + 9)
+    big = base.clone()
+    d, c = big[:, 3:3 + n], r(200, n + 1)[:, 1:]
+    edge, w = torch.tensor(offsets, dtype=torch.int32, device=dev), torch.tensor(which, dtype=torch.int32, device=dev)
+    mb.gemm_lora_(mb.MoYeArray(d), mb.MoYeArray(x), a, b, w, edge, C=mb.MoYeArray(c))
+    check(d, c, x, a, b, None, which, offsets, torch.bfloat16, d)
+    assert torch.equal(big[:, :3], base[:, :3]) and torch.equal(big[:, 3 + n:], base[:, 3 + n:])
+
+
+def test_infinities_stay_in_their_rows(mb, dev):
+    x, a, b, scales, w, edge = make(CASES[3], "bf16", dev)
+    x[:2], x[300:], x[129] = float("nan"), float("inf"), float("inf")
+    d = torch.zeros(310, 2056, device=dev)
+    mb.gemm_lora_(d, x, a, b, w, edge)
+    bad = ~d.isfinite().all(1)
+    assert bad.nonzero().view(-1).tolist() == [129]
+
+
+def test_beside_a_projection_captured(mb, dev):
+    """A decoding step: the shared projection by `gemm_`, the adapters in place behind it, captured once and replayed
+    with other tokens and other adapters."""
+    rows, n, k, rank, count = 12, 512, 256, 16, 5
+    gen = torch.Generator(device=dev).manual_seed(5)
+    r = lambda *s, scale=1.0: (torch.randn(*s, generator=gen, device=dev) * scale).to(torch.bfloat16)
+    x, w, a, b = r(rows, k), r(n, k, scale=k ** -0.5), r(count, rank, k, scale=k ** -0.5), r(count, n, rank, scale=rank ** -0.5)
+    which = torch.arange(rows, dtype=torch.int32, device=dev) % (count + 1)
+    y = torch.empty(rows, n, dtype=torch.bfloat16, device=dev)
+
+    def step():
+        mb.matmul(x, w, y)
+        mb.gemm_lora_(y, x, a, b, which)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(2):
+        x.copy_(r(rows, k))
+        which.copy_((which + i) % (count + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        plain = torch.empty_like(y)
+        mb.matmul(x, w, plain)
+        check(got, plain, x, a, b, None, which.tolist(), None, torch.bfloat16, got)
+    mb.synchronize_status(dev)
+
+
+def test_same_bits_every_time(mb, dev):
+    for case in (1, 3, 7):
+        x, a, b, scales, w, edge = make(CASES[case], "bf16", dev)
+        rows, n = CASES[case][1], CASES[case][3]
+        outs = [mb.gemm_lora_(torch.zeros(rows, n, device=dev), x, a, b, w, edge, scales) for _ in range(3)]
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_no_rows_and_no_requests(mb, dev):
+    a, b = torch.ones(2, 8, 16, dtype=torch.bfloat16, device=dev), torch.ones(2, 24, 8, dtype=torch.bfloat16, device=dev)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    mb.gemm_lora_(torch.empty(0, 24, device=dev), torch.empty(0, 16, dtype=torch.bfloat16, device=dev), a, b, none)
+    d = torch.full((3, 24), 5.0, device=dev)
+    x = torch.ones(3, 16, dtype=torch.bfloat16, device=dev)
+    mb.gemm_lora_(d, x, a, b, none, torch.zeros(1, dtype=torch.int32, device=dev))
+    mb.gemm_lora_(d, x, a, b, torch.zeros(2, dtype=torch.int32, device=dev), torch.tensor([-5, 0, 0], dtype=torch.int32, device=dev))
+    assert bool((d == 5).all())
+    # borders behind the array's end stop at it, borders that run backwards make an empty request
+    mb.gemm_lora_(d, x, a, b, torch.zeros(3, dtype=torch.int32, device=dev), torch.tensor([-5, 2, 1, 99], dtype=torch.int32, device=dev))
+    mb.synchronize_status(dev)
+    assert bool((d == 5 + 16 * 8).all())
+
+
+def test_refusals(mb, dev):
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=dev)
+    which, edge = torch.zeros(2, dtype=torch.int32, device=dev), torch.tensor([0, 1, 4], dtype=torch.int32, device=dev)
+
+    def refused(code, *args, **kw):
+        with pytest.raises(mb.MoyeError) as e:
+            mb.gemm_lora_(*args, **kw)
+        assert e.value.code == code, str(e.value)
+
+    ok = (z(4, 32), z(4, 64), z(3, 16, 64), z(3, 32, 16), which, edge)
+    mb.gemm_lora_(*ok)
+    for code, i, bad in ((-4, 0, z(4, 40)), (-4, 1, z(5, 64)), (-4, 2, z(2, 16, 64)), (-4, 3, z(3, 32, 8)), (-4, 2, z(16, 64)),
+                         (-2, 0, z(4, 32, dtype=torch.float16)), (-2, 1, z(4, 64, dtype=torch.float16)), (-2, 3, z(3, 32, 16, dtype=torch.float32)),
+                         (-3, 0, z(32, 4).t()), (-3, 1, z(64, 4).t()), (-3, 2, z(3, 64, 16).transpose(1, 2)), (-3, 3, z(1, 32, 16).expand(3, 32, 16)),
+                         (-5, 1, z(4, 68)[:, :64]), (-5, 2, z(3, 16, 68)[:, :, :64]), (-5, 3, z(3, 32, 20)[:, :, :16]),
+                         (-1, 4, which.long()), (-4, 5, edge[:2]), (-1, 5, edge.long())):
+        args = list(ok)
+        args[i] = bad
+        refused(code, *args)
+    refused(-4, z(4, 32), z(4, 64), z(3, 12, 64), z(3, 32, 12), which, edge)        # rank 12
+    refused(-4, z(4, 32), z(4, 64), z(3, 136, 64), z(3, 32, 136), which, edge)      # rank 136
+    refused(-4, z(4, 32), z(4, 60), z(3, 16, 60), z(3, 32, 16), which, edge)        # K = 60
+    refused(-1, z(4, 32), z(4, 64), z(3, 16, 64), z(3, 32, 16), which)              # 2 requests, 4 rows, no borders
+    refused(-4, *ok, scales=torch.ones(2, device=dev))
+    refused(-1, *ok, scales=torch.ones(3, device=dev, dtype=torch.float64))
+    refused(-2, *ok, C=z(4, 32, dtype=torch.float32))
+    refused(-4, *ok, C=z(4, 40))
+    torch.cuda.synchronize()
