@@ -160,12 +160,13 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     tmem_alloc(tmem_holder, TMEM_COLS);
     tmem_relinquish();
   }
-  griddep_launch();  // programmatic dependent launch: see launch_dependent(); nothing above touches global memory
-  griddep_wait();
-  if (warp == 2) grouped_borders<BT>(a, row_of, before, lane);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  griddep_launch();  // programmatic dependent launch, after the tensor-memory allocation; nothing above touches global memory
+  griddep_wait();
+  if (warp == 2) grouped_borders<BT>(a, row_of, before, lane);
+  __syncthreads();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
   const GroupedSchedule<MODE, BT> sched{a, row_of, before};
   const int num_tiles = sched.total();
