@@ -116,6 +116,8 @@ _lock = threading.Lock()
 def load():
     """dlopen the in-tree library and type its exports.  Raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):
@@ -167,13 +169,14 @@ def make_tensor(ptr, dtype, shape, stride):
     return t
 
 
-_PACKERS = [None] + [struct.Struct(f"<Qii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(1, MAX_RANK + 1)]
+# one packer per rank: pointer, type, rank, shape and strides, the unused modes zero
+TENSOR_PACKERS = [None] + [struct.Struct(f"<Qii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(1, MAX_RANK + 1)]
 
 
 def pack_tensor(ptr, dtype, shape, stride):
     """`make_tensor` as the bytes of a moye_tensor_t, which a call takes by pointer: a third of the cost of filling the
     ctypes structure, for entry points whose descriptors are made anew on every call."""
-    return _PACKERS[len(shape)].pack(ptr, dtype, len(shape), *shape, *stride)
+    return TENSOR_PACKERS[len(shape)].pack(ptr, dtype, len(shape), *shape, *stride)
 
 
 def make_flat_layout(shape, stride):

@@ -137,11 +137,11 @@ lora_row_kernel(const LoraArgs g) {
 //
 // Warp 0 producer, warp 1 MMA issuer, warps 2-5 move the parts and run the epilogue.  The producer's ring carries first
 // the K blocks, then the chunks of B, which therefore arrive while the parts meet.  The output is bound by memory: the
-// accumulator crosses shared memory so that a warp reads C and writes D as rows of 128 bytes, and C of the next half
-// chunk is on its way while this one is added.
+// accumulator crosses shared memory so that a warp reads C and writes D in 16-byte accesses of whole sectors, and the
+// next 4 KB of C per warp are on their way while these are added.
 // Two CTAs fit on an SM (256 tensor-memory columns each, at most 113 KB); three never do, their shared memory is too large.
 constexpr int kLoraTileThreads = 192;
-enum : int { SITEL_PROD_EMPTY = 171, SITEL_MMA_FULL = 172, SITEL_MMA_V = 173, SITEL_MMA_ACC = 174, SITEL_EPI_V = 175, SITEL_EPI_PARTS = 176, SITEL_EPI_ACC = 177 };
+enum : int { SITEL_PROD_EMPTY = 171, SITEL_MMA_FULL = 172, SITEL_MMA_V = 173, SITEL_MMA_ACC = 174, SITEL_EPI_V = 175, SITEL_EPI_PARTS = 176, SITEL_EPI_ACC = 177, SITEL_SMEM_BASE = 178 };
 
 struct LoraTileArgs {
   LoraArgs g;
@@ -232,8 +232,13 @@ __global__ void __launch_bounds__(kLoraTileThreads, 2)
 lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
                  const __grid_constant__ CUtensorMap tmB, const LoraTileArgs p) {
   const LoraArgs& g = p.g;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // No slack for aligning the base by hand: two CTAs at rank 64 leave 700 bytes of an SM's shared memory.
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, SITEL_SMEM_BASE);
+    return;
+  }
   uint8_t* vparts = smem + p.v_off;                                // [part][64-wide block of R][128 rows][128 bytes], swizzled
   float* parts = reinterpret_cast<float*>(smem + p.stage_out_off);  // [128][R] fp32; later the epilogue's staging
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bar_off);
@@ -257,8 +262,25 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   if (a < 0 || a >= g.adapters) {
     if (g.C != g.D) {
       const int n0 = ch0 * 128, n1 = min(ch1 * 128, g.n);
-      for (int r = warp; r < nrows; r += kLoraTileThreads / 32)
-        for (int n = n0 + lane; n < n1; n += 32) d_base[r * g.d_pitch + n] = c_base[r * g.c_pitch + n];
+      if constexpr (VEC) {
+        constexpr int EPV = 16 / (int)sizeof(OutT);
+        for (int r = warp; r < nrows; r += kLoraTileThreads / 32) {
+          const OutT* from = c_base + r * g.c_pitch;
+          OutT* to = d_base + r * g.d_pitch;
+          for (int n = n0 + lane * EPV; n < n1; n += 8 * 32 * EPV) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i * 32 * EPV < n1) v[i] = *reinterpret_cast<const uint4*>(from + n + i * 32 * EPV);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i * 32 * EPV < n1) *reinterpret_cast<uint4*>(to + n + i * 32 * EPV) = v[i];
+          }
+        }
+      } else {
+        for (int r = warp; r < nrows; r += kLoraTileThreads / 32)
+          for (int n = n0 + lane; n < n1; n += 32) d_base[r * g.d_pitch + n] = c_base[r * g.c_pitch + n];
+      }
     }
     return;
   }
@@ -361,24 +383,27 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     __syncwarp();
   } else {
     // ------------------------------------------------------------ warps 2-5: the rank-R product, then the epilogue
-    constexpr int HW = 128 / (int)sizeof(OutT), EPV = 16 / (int)sizeof(OutT);  // columns of a half step, elements of 16 bytes
+    constexpr int EPV = 16 / (int)sizeof(OutT);  // elements of 16 bytes
+    constexpr int LPR = 32 / EPV;                // lanes side by side in one row of a step of 32 columns
+    constexpr int STEPS = 8 / LPR;               // steps whose C is on its way: 8 accesses of 16 bytes a lane
     const int qd = warp & 3, et = (warp - 2) * 32 + lane;  // tensor-memory quarter; thread among the 128
     const int my_row = qd * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(qd * 32) << 16;
     const float scale = g.scales ? __ldg(g.scales + a) : 1.f;
-    // row r of this warp's 32, 16-byte unit `lane % 8`, as read from C: unit columns n .. n + EPV - 1
-    uint4 cpre[8];
-    auto prefetch = [&](int n_first) {
-      if constexpr (VEC) {
-        const int n = n_first + (lane & 7) * EPV;
+    const int sub_row = lane / LPR, sub_col = (lane % LPR) * EPV;  // access i of a step: row i * EPV + sub_row
+    uint4 cpre[STEPS][LPR];
+    auto prefetch = [&](uint4 (&to)[LPR], int n) {
+      n += sub_col;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = qd * 32 + i * 4 + (lane >> 3);
-          if (r < nrows && n < g.n) cpre[i] = *reinterpret_cast<const uint4*>(c_base + r * g.c_pitch + n);
-        }
+      for (int i = 0; i < LPR; ++i) {
+        const int r = qd * 32 + i * EPV + sub_row;
+        if (r < nrows && n < g.n) to[i] = *reinterpret_cast<const uint4*>(c_base + r * g.c_pitch + n);
       }
     };
-    if (ch0 < ch1) prefetch(ch0 * 128);
+    if (VEC && ch0 < ch1) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) prefetch(cpre[s], ch0 * 128 + s * 32);
+    }
     // the value of `x` as PARTS 16-bit numbers, the largest first
     auto write_parts = [&](int row, int col, float4 x, auto&& store) {  // 4 columns at once
       float r[4] = {x.x, x.y, x.z, x.w};
@@ -442,61 +467,59 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         }
       }
     }
-    float* st = parts + (warp - 2) * 32 * HW;  // this warp's staging: [32 rows][HW columns], 16-byte units swizzled by the row
-    constexpr int UNITS = HW / 4;
+    float* st = parts + (warp - 2) * 32 * 32;  // this warp's staging: 32 rows of 32 columns, 16-byte units swizzled by the row
     for (int i = 0; i < ch1 - ch0 && ok; ++i) {
       const int buf = i & 1, n0 = (ch0 + i) * 128;
       ok = mbar_wait(&acc_full[buf], (i >> 1) & 1, p.status, SITEL_EPI_ACC);
       if (!ok) break;
       tc_fence_after_sync();
 #pragma unroll 1
-      for (int h = 0; h < 128; h += HW) {
+      for (int h = 0; h < 128; h += 32 * STEPS) {
 #pragma unroll
-        for (int c = 0; c < HW; c += 32) {
-          uint32_t v[32];
-          tmem_ld_x32(tmem_base + t_lane + buf * 128 + h + c, v);
-          tmem_ld_wait();
+        for (int s = 0; s < STEPS; ++s) {
+          const int col = h + s * 32;
+          {
+            uint32_t v[32];
+            tmem_ld_x32(tmem_base + t_lane + buf * 128 + col, v);
+            tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(st + lane * HW + ((((c >> 2) + j) ^ (lane & (UNITS - 1))) << 2)) =
-                make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
-        if (h + HW >= 128) {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        }
-        __syncwarp();
-        if constexpr (VEC) {
-          const int n = n0 + h + (lane & 7) * EPV;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = k * 4 + (lane >> 3);
-            const float* row = st + r * HW;
-            OutT o[EPV];
-            const OutT* cin = reinterpret_cast<const OutT*>(&cpre[k]);
-#pragma unroll
-            for (int e = 0; e < EPV; e += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(row + (((((lane & 7) * EPV + e) >> 2) ^ (r & (UNITS - 1))) << 2));
-              o[e] = cvt_out<OutT>(lora_load(cin + e) + x.x);
-              o[e + 1] = cvt_out<OutT>(lora_load(cin + e + 1) + x.y);
-              o[e + 2] = cvt_out<OutT>(lora_load(cin + e + 2) + x.z);
-              o[e + 3] = cvt_out<OutT>(lora_load(cin + e + 3) + x.w);
-            }
-            if (qd * 32 + r < nrows && n < g.n)
-              *reinterpret_cast<uint4*>(d_base + (qd * 32 + r) * g.d_pitch + n) = *reinterpret_cast<const uint4*>(o);
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(st + lane * 32 + ((j ^ (lane & 7)) << 2)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
-          const int next = h + HW < 128 ? n0 + h + HW : n0 + 128;
-          if (next < min(ch1 * 128, g.n)) prefetch(next);
-        } else {
-          for (int r = 0; r < 32 && qd * 32 + r < nrows; ++r)
-            for (int c = lane; c < HW && n0 + h + c < g.n; c += 32) {
-              const long long row = qd * 32 + r;
-              const float x = st[r * HW + (((c >> 2) ^ (r & (UNITS - 1))) << 2) + (c & 3)];
-              lora_store(d_base + row * g.d_pitch + n0 + h + c, lora_load(c_base + row * g.c_pitch + n0 + h + c) + x);
+          if (col + 32 >= 128) tc_fence_before_sync();
+          __syncwarp();
+          if (col + 32 >= 128 && lane == 0) mbar_arrive(&acc_empty[buf]);
+          if constexpr (VEC) {
+            const int n = n0 + col + sub_col;
+#pragma unroll
+            for (int k = 0; k < LPR; ++k) {
+              const int r = k * EPV + sub_row;
+              OutT o[EPV];
+              const OutT* cin = reinterpret_cast<const OutT*>(&cpre[s][k]);
+#pragma unroll
+              for (int e = 0; e < EPV; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(st + r * 32 + ((((sub_col + e) >> 2) ^ (r & 7)) << 2));
+                o[e] = cvt_out<OutT>(lora_load(cin + e) + x.x);
+                o[e + 1] = cvt_out<OutT>(lora_load(cin + e + 1) + x.y);
+                o[e + 2] = cvt_out<OutT>(lora_load(cin + e + 2) + x.z);
+                o[e + 3] = cvt_out<OutT>(lora_load(cin + e + 3) + x.w);
+              }
+              if (qd * 32 + r < nrows && n < g.n)
+                *reinterpret_cast<uint4*>(d_base + (qd * 32 + r) * g.d_pitch + n) = *reinterpret_cast<const uint4*>(o);
             }
+            const int next = n0 + col + 32 * STEPS;  // the same step of the next round, maybe in the next chunk
+            if (next < ch1 * 128) prefetch(cpre[s], next);
+          } else {
+            for (int r = 0; r < 32 && qd * 32 + r < nrows; ++r) {
+              const long long row = qd * 32 + r;
+              if (n0 + col + lane < g.n) {
+                const float x = st[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+                lora_store(d_base + row * g.d_pitch + n0 + col + lane, lora_load(c_base + row * g.c_pitch + n0 + col + lane) + x);
+              }
+            }
+          }
+          __syncwarp();  // the staging is read: the next step may overwrite it
         }
-        __syncwarp();  // the staging is read: the next half may overwrite it
       }
     }
   }
@@ -531,20 +554,20 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, cuda
   p.idesc1 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(rsteps * 2) << 17) | (8u << 24);
   p.idesc2 = (1u << 4) | (fmt << 7) | (fmt << 10) | (16u << 17) | (8u << 24);
   p.status = h->d_status;
-  const int block = 128 * 128, half = 128 / (int)sizeof(OutT);
+  const int block = 128 * 128;
   p.stage_bytes = block + rsteps * 16 * 128 > rblocks * block ? block + rsteps * 16 * 128 : rblocks * block;
   p.stage_bytes = (p.stage_bytes + 1023) & ~1023;
   const int v_bytes = PARTS * rblocks * block;
-  int out_bytes = 4 * 32 * half * 4;
+  int out_bytes = 4 * 32 * 32 * 4;
   if (ctas > 1 && 128 * rsteps * 16 * 4 > out_bytes) out_bytes = 128 * rsteps * 16 * 4;
-  const int rest = v_bytes + out_bytes + 512 + 1024, half_sm = 113 * 1024;
+  const int rest = v_bytes + out_bytes + 512, half_sm = 113 * 1024;
   // two CTAs per SM if three (two) stages fit into half of its shared memory, else one with as many as fit
   p.stages = rest + 3 * p.stage_bytes <= half_sm ? 3 : rest + 2 * p.stage_bytes <= half_sm ? 2 : 4;
   while (p.stages > 2 && rest + p.stages * p.stage_bytes > 227 * 1024) --p.stages;
   p.v_off = p.stages * p.stage_bytes;
   p.stage_out_off = p.v_off + v_bytes;
   p.bar_off = p.stage_out_off + out_bytes;
-  const int smem = p.bar_off + 512 + 1024;
+  const int smem = p.bar_off + 512;
   CUtensorMap tx, ta, tb;
   if (int rc = encode_tmap_2d_uncached(&tx, g.X, dtype, g.k, g.rows, (uint64_t)g.x_pitch * 2, 64, 128, true)) return rc;
   const uint64_t a_pitch = g.a_pitch * 2, a_stride = g.adapters > 1 ? g.a_stride * 2 : g.rank * a_pitch;

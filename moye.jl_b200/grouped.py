@@ -14,8 +14,6 @@ the operands' device or on `stream`, a violation raises `MoyeError`, nothing fal
 borders, choices and adapter numbers stay on the device: no call waits for the GPU, and a captured call follows new
 values in the same arrays.  The reference has no counterpart.
 """
-import ctypes
-
 import torch
 
 from . import _lib
@@ -26,6 +24,11 @@ __all__ = ["RowGroups", "group_rows", "group_rows_", "gather_rows_", "combine_ro
            "gemm_grouped_grad_", "gemm_lora_"]
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a torch Stream object costs 2 us a call
+_PACK = _lib.TENSOR_PACKERS
+_INT32, _FLOAT32 = torch.int32, torch.float32
+
+
 class RowGroups:
     """The result of sorting (tokens, choices) group numbers: int32 tensors on one device.
 
@@ -34,64 +37,66 @@ class RowGroups:
     position of a choice, -1 if it was dropped.  A plan made once can be filled again by `group_rows_` (a captured
     step needs that: the tensors keep their addresses)."""
 
-    __slots__ = ("order", "offsets", "inverse", "tokens", "choices", "groups")
+    __slots__ = ("order", "offsets", "inverse", "tokens", "choices", "groups", "_at")
 
     def __init__(self, tokens, choices, groups, device):
-        n = tokens * choices
-        buf = torch.empty(2 * n + groups + 1, dtype=torch.int32, device=device)
-        self.order, self.offsets = buf[:n], buf[2 * n:]
-        self.inverse = buf[n:2 * n].view(tokens, choices)
+        self.order = torch.empty(tokens * choices, dtype=_INT32, device=device)
+        self.offsets = torch.empty(groups + 1, dtype=_INT32, device=device)
+        self.inverse = torch.empty((tokens, choices), dtype=_INT32, device=device)
         self.tokens, self.choices, self.groups = tokens, choices, groups
+        self._at = self.order.get_device()
 
 
 def _arg(x, rank, what):
-    """(descriptor bytes, device) of a rank-`rank` device array."""
+    """(descriptor bytes, device index) of a rank-`rank` device array."""
     if isinstance(x, torch.Tensor):
-        shape, stride, dtype, ptr, dev = x.shape, x.stride(), TORCH_TO_MOYE.get(x.dtype), x.data_ptr(), x.device
+        dev, dtype = x.get_device(), TORCH_TO_MOYE.get(x.dtype)
+        if dev >= 0 and dtype is not None and x.dim() == rank:
+            return _PACK[rank].pack(x.data_ptr(), dtype, rank, *x.shape, *x.stride()), dev
+        shape, where = tuple(x.shape), x.device
     elif isinstance(x, MoYeArray):
         l = x.layout
         modes = [coalesce(l[i]) for i in range(len(l))] if len(l) > 1 else [coalesce(l)]
         if any(isinstance(m.shape, tuple) for m in modes):
             raise _lib.MoyeError(-3, f"{what} must have one stride per mode, got layout {l}")
-        shape, stride = [int(m.shape) for m in modes], [int(m.stride) for m in modes]
-        dtype, ptr, dev = x.dtype, x.ptr, x.device
+        shape, dtype, where = tuple(int(m.shape) for m in modes), x.dtype, x.device
+        if where.type == "cuda" and len(shape) == rank:
+            return _PACK[rank].pack(x.ptr, dtype, rank, *shape, *(int(m.stride) for m in modes)), where.index
     else:
         raise TypeError(f"{what} must be a torch.Tensor or a MoYeArray, got {type(x).__name__}")
-    if dev.type != "cuda":
-        raise RuntimeError(f"libmoye_b200 runs on device global memory only; {what} is on {dev} (there is no CPU fallback)")
+    if where.type != "cuda":
+        raise RuntimeError(f"libmoye_b200 runs on device global memory only; {what} is on {where} (there is no CPU fallback)")
     if dtype is None:
-        raise _lib.MoyeError(-2, f"{what}: unsupported element type")
-    if len(shape) != rank:
-        raise _lib.MoyeError(-4, f"{what} must be rank {rank}, got shape {tuple(shape)}")
-    return _lib.pack_tensor(ptr, dtype, shape, stride), dev
+        raise _lib.MoyeError(-2, f"{what}: unsupported element type {x.dtype}")
+    raise _lib.MoyeError(-4, f"{what} must be rank {rank}, got shape {shape}")
 
 
-def _ints(x, what, dev, numel=None, dtype=torch.int32):
-    """Address of a contiguous device vector of whole numbers (or scales) on `dev`."""
-    if not torch.is_tensor(x) or x.dtype != dtype or not x.is_contiguous():
+def _vector(x, what, dev, numel=None, dtype=_INT32):
+    """Address of a contiguous device vector of `dtype` on device `dev`."""
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or not x.is_contiguous():
         raise _lib.MoyeError(-1, f"{what} must be a contiguous {dtype} tensor")
-    if x.device != dev:
+    if x.get_device() != dev:
         raise RuntimeError("operands live on different devices")
     if numel is not None and x.numel() != numel:
         raise _lib.MoyeError(-4, f"{what} must hold {numel} values, got {x.numel()}")
     return x.data_ptr()
 
 
-def _same_device(dev, *others):
-    for d in others:
-        if d != dev:
-            raise RuntimeError("operands live on different devices")
+def _differ():
+    raise RuntimeError("operands live on different devices")
 
 
 def _call(fn, dev, stream, *args):
-    """fn(handle, *args, stream) with the operands' device current."""
+    """fn(handle, *args, stream) with device number `dev`, the operands', current."""
     if stream is None:
-        stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(_lib.handle(dev.index), *args, stream))
+        stream = _raw_stream(dev)
+    if torch.cuda.current_device() == dev:
+        rc = fn(_lib.handle(dev), *args, stream)
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(_lib.handle(dev.index), *args, stream))
+            rc = fn(_lib.handle(dev), *args, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def group_rows(ids, groups):
@@ -111,10 +116,12 @@ def group_rows(ids, groups):
 
 def group_rows_(plan, ids, stream=None):
     """`group_rows` into the tensors of an existing plan of the same tokens, choices and groups."""
-    t, dev = _arg(ids, 1 if len(ids.shape) == 1 else 2, "ids")
-    if ids.shape[0] != plan.tokens or (ids.shape[1] if len(ids.shape) == 2 else 1) != plan.choices:
+    rank = len(ids.shape)
+    t, dev = _arg(ids, 1 if rank == 1 else 2, "ids")
+    if ids.shape[0] != plan.tokens or (ids.shape[1] if rank == 2 else 1) != plan.choices:
         raise _lib.MoyeError(-4, f"the plan is for ({plan.tokens}, {plan.choices}) choices, ids are {tuple(ids.shape)}")
-    _same_device(dev, plan.order.device)
+    if dev != plan._at:
+        _differ()
     _call(_lib.load().moye_b200_group_rows, dev, stream, t, plan.groups, plan.order.data_ptr(), plan.offsets.data_ptr(),
           plan.inverse.data_ptr())
     return plan
@@ -124,8 +131,10 @@ def gather_rows_(dst, src, plan, stream=None):
     """dst[p] = src[plan.order[p] // choices] for the kept positions; rows of dst behind them are left as they were.
     src (tokens, width), dst (tokens * choices, width); any element type, contiguous rows.  Its gradient is
     `combine_rows_(dsrc, ddst, plan)`."""
-    (td, dev), (ts, d1) = _arg(dst, 2, "dst"), _arg(src, 2, "src")
-    _same_device(dev, d1, plan.inverse.device)
+    td, dev = _arg(dst, 2, "dst")
+    ts, d1 = _arg(src, 2, "src")
+    if not dev == d1 == plan._at:
+        _differ()
     _call(_lib.load().moye_b200_gather_rows, dev, stream, td, ts, plan.inverse.data_ptr(), plan.choices)
     return dst
 
@@ -133,12 +142,11 @@ def gather_rows_(dst, src, plan, stream=None):
 def combine_rows_(dst, src, plan, weights=None, stream=None):
     """dst[t] = sum_j weights[t, j] * src[plan.inverse[t, j]] over the choices that were kept (none: zeros), in fp32 in
     the order of j with one rounding.  `weights` (tokens, choices) in f32, f16 or bf16; None counts every choice once."""
-    (td, dev), (ts, d1) = _arg(dst, 2, "dst"), _arg(src, 2, "src")
-    _same_device(dev, d1, plan.inverse.device)
-    tw = None
-    if weights is not None:
-        tw, d2 = _arg(weights, 2, "weights")
-        _same_device(dev, d2)
+    td, dev = _arg(dst, 2, "dst")
+    ts, d1 = _arg(src, 2, "src")
+    tw, d2 = (None, dev) if weights is None else _arg(weights, 2, "weights")
+    if not dev == d1 == d2 == plan._at:
+        _differ()
     _call(_lib.load().moye_b200_combine_rows, dev, stream, td, ts, tw, plan.inverse.data_ptr(), plan.choices)
     return dst
 
@@ -147,17 +155,21 @@ def combine_rows_grad_(dsrc, dweights, ddst, src, plan, weights, stream=None):
     """The gradient of `combine_rows_(dst, src, plan, weights)`: dsrc[inverse[t, j]] = weights[t, j] * ddst[t] (rows
     behind the kept positions are left as they were), dweights[t, j] = <ddst[t], src[inverse[t, j]]>, 0 where the choice
     was dropped.  Returns (dsrc, dweights)."""
-    args = [_arg(x, 2, n) for x, n in ((dsrc, "dsrc"), (dweights, "dweights"), (ddst, "ddst"), (src, "src"), (weights, "weights"))]
-    dev = args[0][1]
-    _same_device(dev, plan.inverse.device, *(d for _, d in args[1:]))
-    _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, *(t for t, _ in args), plan.inverse.data_ptr(), plan.choices)
+    t0, dev = _arg(dsrc, 2, "dsrc")
+    t1, d1 = _arg(dweights, 2, "dweights")
+    t2, d2 = _arg(ddst, 2, "ddst")
+    t3, d3 = _arg(src, 2, "src")
+    t4, d4 = _arg(weights, 2, "weights")
+    if not dev == d1 == d2 == d3 == d4 == plan._at:
+        _differ()
+    _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, t0, t1, t2, t3, t4, plan.inverse.data_ptr(), plan.choices)
     return dsrc, dweights
 
 
 def _borders(offsets, groups, dev):
     if isinstance(offsets, RowGroups):
         offsets = offsets.offsets
-    return _ints(offsets, "offsets", dev, groups + 1)
+    return _vector(offsets, "offsets", dev, groups + 1)
 
 
 def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
@@ -167,8 +179,11 @@ def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
     groups + 1 borders or the RowGroups they come from.  B may be the swapped view of a (groups, K, N) array:
     `gemm_grouped_(dA, dD, B.transpose(1, 2), offsets)` is the gradient of A.  Rows outside the groups are left as they
     were; D is not read when beta == 0."""
-    (td, dev), (ta, d1), (tb, d2) = _arg(D, 2, "D"), _arg(A, 2, "A"), _arg(B, 3, "B")
-    _same_device(dev, d1, d2)
+    td, dev = _arg(D, 2, "D")
+    ta, d1 = _arg(A, 2, "A")
+    tb, d2 = _arg(B, 3, "B")
+    if not dev == d1 == d2:
+        _differ()
     _call(_lib.load().moye_b200_gemm_grouped, dev, stream, td, ta, tb, _borders(offsets, int(B.shape[0]), dev), alpha, beta)
     return D
 
@@ -176,8 +191,11 @@ def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
 def gemm_grouped_grad_(dB, dD, A, offsets, alpha=1.0, beta=0.0, stream=None):
     """dB[g] = alpha * sum of dD[i]^T A[i] over the rows of group g + beta * dB[g]: the gradient of `gemm_grouped_` with
     respect to B.  Every group is written (an empty one becomes beta * dB[g]); beta = 1 accumulates over micro-batches."""
-    (tb, dev), (td, d1), (ta, d2) = _arg(dB, 3, "dB"), _arg(dD, 2, "dD"), _arg(A, 2, "A")
-    _same_device(dev, d1, d2)
+    tb, dev = _arg(dB, 3, "dB")
+    td, d1 = _arg(dD, 2, "dD")
+    ta, d2 = _arg(A, 2, "A")
+    if not dev == d1 == d2:
+        _differ()
     _call(_lib.load().moye_b200_gemm_grouped_grad, dev, stream, tb, td, ta, _borders(offsets, int(dB.shape[0]), dev), alpha, beta)
     return dB
 
@@ -190,15 +208,15 @@ def gemm_lora_(D, X, A, B, adapters, offsets=None, scales=None, C=None, stream=N
     one int32 per request, a number outside 0..count-1 means none.  `offsets` (requests + 1 borders, int32) says which
     rows are a request's; without it every row is one.  Rows outside every request are left as they were.  R is a
     multiple of 8 up to 128: pad adapters of smaller rank with zeros."""
-    (td, dev), (tx, d1), (ta, d2), (tb, d3) = _arg(D, 2, "D"), _arg(X, 2, "X"), _arg(A, 3, "A"), _arg(B, 3, "B")
-    _same_device(dev, d1, d2, d3)
-    tc = None
-    if C is not None:
-        tc, d4 = _arg(C, 2, "C")
-        _same_device(dev, d4)
-    which = _ints(adapters, "adapters", dev)
-    requests = adapters.numel()
-    edges = None if offsets is None else _ints(offsets, "offsets", dev, requests + 1)
-    s = None if scales is None else _ints(scales, "scales", dev, int(A.shape[0]), torch.float32)
+    td, dev = _arg(D, 2, "D")
+    tx, d1 = _arg(X, 2, "X")
+    ta, d2 = _arg(A, 3, "A")
+    tb, d3 = _arg(B, 3, "B")
+    tc, d4 = (None, dev) if C is None else _arg(C, 2, "C")
+    if not dev == d1 == d2 == d3 == d4:
+        _differ()
+    which, requests = _vector(adapters, "adapters", dev), adapters.numel()
+    edges = None if offsets is None else _vector(offsets, "offsets", dev, requests + 1)
+    s = None if scales is None else _vector(scales, "scales", dev, int(A.shape[0]), _FLOAT32)
     _call(_lib.load().moye_b200_gemm_lora, dev, stream, td, tx, ta, tb, tc, which, edges, requests, s)
     return D
