@@ -33,13 +33,18 @@ constexpr int kMaxGroups = 1024;  // one thread per group in the scans; 32 count
 struct IdSource {
   const void* ptr;
   int is64;
+  int packed;  // entry i lies at i * s_choice
   long long s_token, s_choice;
   int choices;
 };
+constexpr int kIdBatch = 8;   // ids a lane requests at once: the walk is bound by the latency of these loads
 
 __device__ __forceinline__ int load_id(const IdSource& ids, int i, int groups) {
-  const int t = i / ids.choices, j = i - t * ids.choices;
-  const long long at = t * ids.s_token + j * ids.s_choice;
+  long long at = i * ids.s_choice;
+  if (!ids.packed) {
+    const int t = i / ids.choices, j = i - t * ids.choices;
+    at = t * ids.s_token + j * ids.s_choice;
+  }
   const long long v = ids.is64 ? static_cast<const long long*>(ids.ptr)[at] : static_cast<const int*>(ids.ptr)[at];
   return v >= 0 && v < groups ? static_cast<int>(v) : -1;
 }
@@ -48,6 +53,18 @@ __device__ __forceinline__ int ld_remote_i32(uint32_t cluster_addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
   return v;
+}
+
+// The lanes whose key equals this lane's, a ballot per bit of the key (11 at most).  `__match_any_sync` does the same in
+// one instruction whose time grows with the number of different keys: 131072 choices among 128 groups took 29 us with it.
+__device__ __forceinline__ unsigned same_key(int key, int bits) {
+  unsigned peers = ~0u;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (key >> b) & 1;
+    const unsigned set = __ballot_sync(~0u, one);
+    peers &= one ? set : ~set;
+  }
+  return peers;
 }
 
 __global__ void __launch_bounds__(kGroupThreads, 1)
@@ -68,10 +85,17 @@ group_rows_kernel(const IdSource ids, int n, int groups, int* order, int* offset
 
   for (int g = lane; g < groups; g += 32) mine[g] = 0;
   __syncwarp();
-  for (int b = b0; b < b1; ++b) {
-    const int i = b * 32 + lane;
-    const int id = i < n ? load_id(ids, i, groups) : -1;
-    if (id >= 0) atomicAdd(&mine[id], 1);
+  const int key_bits = 32 - __clz(groups);
+  int id[kIdBatch];
+  for (int b = b0; b < b1; b += kIdBatch) {
+#pragma unroll
+    for (int u = 0; u < kIdBatch; ++u) {
+      const int i = (b + u) * 32 + lane;
+      id[u] = b + u < b1 && i < n ? load_id(ids, i, groups) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kIdBatch; ++u)
+      if (id[u] >= 0) atomicAdd(&mine[id[u]], 1);
   }
   __syncthreads();
   for (int g = tid; g < groups; g += kGroupThreads) {
@@ -122,19 +146,29 @@ group_rows_kernel(const IdSource ids, int n, int groups, int* order, int* offset
   }
   if (rank == 0 && tid == 0) offsets[groups] = kept;
   __syncthreads();
-  for (int b = b0; b < b1; ++b) {
-    const int i = b * 32 + lane;
-    const int id = i < n ? load_id(ids, i, groups) : -1;
-    const unsigned peers = __match_any_sync(~0u, id);
-    const int ahead = __popc(peers & ((1u << lane) - 1));
-    int pos = -1;
-    if (id >= 0) pos = base[id] + mine[id] + ahead;
-    __syncwarp();
-    if (id >= 0 && ahead == 0) mine[id] += __popc(peers);
-    __syncwarp();
-    if (i < n) {
-      inverse[i] = pos;
-      if (pos >= 0) order[pos] = i;
+  for (int b = b0; b < b1; b += kIdBatch) {
+    if (b1 - b0 > kIdBatch) {  // else the counting walk has left them in place
+#pragma unroll
+      for (int u = 0; u < kIdBatch; ++u) {
+        const int i = (b + u) * 32 + lane;
+        id[u] = b + u < b1 && i < n ? load_id(ids, i, groups) : -1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kIdBatch; ++u) {
+      if (b + u >= b1) break;
+      const int i = (b + u) * 32 + lane;
+      const unsigned peers = same_key(id[u] < 0 ? groups : id[u], key_bits);
+      const int ahead = __popc(peers & ((1u << lane) - 1));
+      int pos = -1;
+      if (id[u] >= 0) pos = base[id[u]] + mine[id[u]] + ahead;
+      __syncwarp();
+      if (id[u] >= 0 && ahead == 0) mine[id[u]] += __popc(peers);
+      __syncwarp();
+      if (i < n) {
+        inverse[i] = pos;
+        if (pos >= 0) order[pos] = i;
+      }
     }
   }
   for (int p = kept + rank * kGroupThreads + tid; p < n; p += C * kGroupThreads) order[p] = -1;
@@ -153,7 +187,13 @@ int launch_group_rows(moye_b200_ctx* h, const moye_tensor_t* ids, int groups, in
   if (tokens > INT32_MAX / 2 / choices) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "group_rows: more than 2^30 choices");
   const int n = (int)(tokens * choices);
   if (!offsets || (n > 0 && (!ids->ptr || !order || !inverse))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "group_rows: null pointer");
-  const IdSource src{ids->ptr, ids->dtype == MOYE_U64, ids->stride[0], ids->rank == 2 ? ids->stride[1] : 0, (int)choices};
+  IdSource src;
+  src.ptr = ids->ptr;
+  src.is64 = ids->dtype == MOYE_U64;
+  src.s_token = ids->stride[0];
+  src.s_choice = choices > 1 ? ids->stride[1] : ids->stride[0];
+  src.packed = choices == 1 || src.s_token == choices * src.s_choice;
+  src.choices = (int)choices;
   const int smem = (kGroupWarps + 2) * groups * 4;
   if (int rc = configure_once(h, group_rows_kernel, (kGroupWarps + 2) * kMaxGroups * 4)) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -195,8 +235,17 @@ __device__ __forceinline__ __nv_bfloat16 float_to_row_elem<__nv_bfloat16>(float 
 
 // `V` elements moved as one access: 16 bytes where every row starts on a 16-byte boundary, single elements otherwise.
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Pack {
-  T e[V];
+struct Pack {
+  using Raw = typename std::conditional<V != 1, uint4,
+              typename std::conditional<sizeof(T) == 8, uint2,
+              typename std::conditional<sizeof(T) == 4, uint32_t,
+              typename std::conditional<sizeof(T) == 2, uint16_t, uint8_t>::type>::type>::type>::type;
+  static_assert(V == 1 || V * sizeof(T) == 16, "an access is one element or 16 bytes");
+  Raw raw;
+  __device__ __forceinline__ void load(const T* row, long long i) { raw = reinterpret_cast<const Raw*>(row)[i]; }
+  __device__ __forceinline__ void store(T* row, long long i) const { reinterpret_cast<Raw*>(row)[i] = raw; }
+  __device__ __forceinline__ float at(int e) const { return row_elem_to_float<T>(reinterpret_cast<const T*>(&raw)[e]); }
+  __device__ __forceinline__ void set(int e, float f) { reinterpret_cast<T*>(&raw)[e] = float_to_row_elem<T>(f); }
 };
 
 __device__ __forceinline__ float load_weight(const void* w, int dtype, long long i) {
@@ -222,124 +271,177 @@ struct RowArgs {
   long long dws_token, dws_choice;
 };
 
-constexpr int kRowPacks = 4;  // packs a lane holds at once
+// Accesses a lane has under way: kept near 8 of 16 bytes, which at the resident warps covers the latency of memory.
+template <int V>
+__host__ __device__ constexpr int gather_packs() { return V == 1 ? 8 : 4; }  // packs of a token's row a lane holds
+// combine and its gradient request the rows of U choices at once, 2 for one or two choices and 4 for more, N accesses of
+// each per thread.  Requests of missing choices are wasted (2 choices, 8192 rows of 4096 bf16: combine 58 us with U = 4);
+// more accesses in flight than this cost more in resident CTAs than they hide (the same with U = 2: 39 us with N = 2, 52
+// with 4, 59 with 8; 8 choices, 16384 rows of 2048: 103 us with U x N = 8, 105 with 4, 130 with 16).  The gradient reads
+// one row more and takes N = 4 (58 us, 59 with 2, 74 with 8).
+template <int V>
+__host__ __device__ constexpr int combine_packs() { return V == 1 ? 4 : 2; }
+template <int V, int U>
+__host__ __device__ constexpr int grad_packs() { return (V == 1 ? 16 : 8) / U; }
 
-// One warp takes kRowPacks * 32 packs of one token's row.
+// Position and weight of up to 32 choices of a token, one per lane; a dropped choice has position -1.
+struct Choices {
+  int pos;
+  float w;
+  __device__ __forceinline__ Choices(const RowArgs& g, long long t, int j0, int lane) : pos(-1), w(1.f) {
+    const int j = j0 + lane;
+    if (j < g.choices && t < g.tokens) {
+      pos = __ldg(g.inverse + t * g.choices + j);
+      if (g.weights) w = load_weight(g.weights, g.w_dtype, t * g.ws_token + j * g.ws_choice);
+    }
+    if (static_cast<unsigned>(pos) >= static_cast<unsigned>(g.positions)) pos = -1;
+  }
+};
+
+// One warp takes N * 32 packs of one token's row.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 gather_rows_kernel(T* dst, const T* src, const RowArgs g) {
   using P = Pack<T, V>;
+  constexpr int N = gather_packs<V>();
   griddep_launch();
   griddep_wait();
   const int lane = threadIdx.x & 31;
-  const long long parts = (g.packs + 32 * kRowPacks - 1) / (32 * kRowPacks);
-  const long long items = parts * g.tokens, step = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long it = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items; it += step) {
-    const long long t = it / parts, p0 = (it - t * parts) * (32 * kRowPacks) + lane;
-    const P* row = reinterpret_cast<const P*>(src + t * g.pitch_token);
-    P v[kRowPacks];
+  const int parts = (int)((g.packs + 32 * N - 1) / (32 * N));
+  const int it = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long long t = it / parts, p0 = (long long)(it - (int)t * parts) * (32 * N) + lane;
+  if (t >= g.tokens) return;
+  P v[N];
 #pragma unroll
-    for (int i = 0; i < kRowPacks; ++i)
-      if (p0 + i * 32 < g.packs) v[i] = row[p0 + i * 32];
-    for (int j = 0; j < g.choices; ++j) {
-      const int pos = __ldg(g.inverse + t * g.choices + j);
-      if (static_cast<unsigned>(pos) >= static_cast<unsigned>(g.positions)) continue;
-      P* out = reinterpret_cast<P*>(dst + pos * g.pitch_sorted);
+  for (int i = 0; i < N; ++i) v[i].load(src + t * g.pitch_token, min(p0 + i * 32, g.packs - 1));
+  for (int j0 = 0; j0 < g.choices; j0 += 32) {
+    const Choices c(g, t, j0, lane);
+    for (int j = 0; j < 32 && j0 + j < g.choices; ++j) {
+      const int pos = __shfl_sync(~0u, c.pos, j);
+      if (pos < 0) continue;
 #pragma unroll
-      for (int i = 0; i < kRowPacks; ++i)
-        if (p0 + i * 32 < g.packs) out[p0 + i * 32] = v[i];
+      for (int i = 0; i < N; ++i)
+        if (p0 + i * 32 < g.packs) v[i].store(dst + pos * g.pitch_sorted, p0 + i * 32);
     }
   }
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
+// One CTA of 128 threads per token, a thread N packs of its row at a time.
+template <typename T, int V, int U>
+__global__ void __launch_bounds__(128)
 combine_rows_kernel(T* dst, const T* src, const RowArgs g) {
   using P = Pack<T, V>;
+  constexpr int N = combine_packs<V>();
   griddep_launch();
   griddep_wait();
   const int lane = threadIdx.x & 31;
-  const long long parts = (g.packs + 32 * kRowPacks - 1) / (32 * kRowPacks);
-  const long long items = parts * g.tokens, step = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long it = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items; it += step) {
-    const long long t = it / parts, p0 = (it - t * parts) * (32 * kRowPacks) + lane;
-    float acc[kRowPacks][V];
+  const long long t = blockIdx.x;
+  const Choices first(g, t, 0, lane);
+  for (long long base = 0; base < g.packs; base += 128 * N) {
+    const long long p0 = base + threadIdx.x;
+    float acc[N][V];
 #pragma unroll
-    for (int i = 0; i < kRowPacks; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[i][e] = 0.f;
-    for (int j = 0; j < g.choices; ++j) {
-      const int pos = __ldg(g.inverse + t * g.choices + j);
-      if (static_cast<unsigned>(pos) >= static_cast<unsigned>(g.positions)) continue;
-      const float w = g.weights ? load_weight(g.weights, g.w_dtype, t * g.ws_token + j * g.ws_choice) : 1.f;
-      const P* in = reinterpret_cast<const P*>(src + pos * g.pitch_sorted);
-      P v[kRowPacks];
+    for (int j0 = 0; j0 < g.choices; j0 += 32) {
+      Choices c = first;
+      if (j0) c = Choices(g, t, j0, lane);
+      const int here = min(32, g.choices - j0);
+      for (int j = 0; j < here; j += U) {
+        P v[U][N];
+        int pos[U];
 #pragma unroll
-      for (int i = 0; i < kRowPacks; ++i)
-        if (p0 + i * 32 < g.packs) v[i] = in[p0 + i * 32];
+        for (int u = 0; u < U; ++u) {
+          pos[u] = __shfl_sync(~0u, c.pos, (j + u) & 31);
+          if (j + u >= here) pos[u] = -1;
+          // no branch around a load: a dropped choice reads row 0 and a lane behind the row its last pack, for nothing
+          const T* in = src + max(pos[u], 0) * g.pitch_sorted;
 #pragma unroll
-      for (int i = 0; i < kRowPacks; ++i)
-        if (p0 + i * 32 < g.packs)
+          for (int i = 0; i < N; ++i) v[u][i].load(in, min(p0 + i * 128, g.packs - 1));
+        }
 #pragma unroll
-          for (int e = 0; e < V; ++e) acc[i][e] += w * row_elem_to_float<T>(v[i].e[e]);
+        for (int u = 0; u < U; ++u) {
+          const float w = __shfl_sync(~0u, c.w, (j + u) & 31);
+          if (pos[u] < 0) continue;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[i][e] += w * v[u][i].at(e);
+        }
+      }
     }
-    P* out = reinterpret_cast<P*>(dst + t * g.pitch_token);
 #pragma unroll
-    for (int i = 0; i < kRowPacks; ++i)
-      if (p0 + i * 32 < g.packs) {
+    for (int i = 0; i < N; ++i)
+      if (p0 + i * 128 < g.packs) {
         P v;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v.e[e] = float_to_row_elem<T>(acc[i][e]);
-        out[p0 + i * 32] = v;
+        for (int e = 0; e < V; ++e) v.set(e, acc[i][e]);
+        v.store(dst + t * g.pitch_token, p0 + i * 128);
       }
   }
 }
 
 // One CTA of 128 threads per token: the dot products run over the whole row.
-template <typename T, int V>
+template <typename T, int V, int U>
 __global__ void __launch_bounds__(128)
 combine_rows_grad_kernel(T* dsrc, const T* ddst, const T* src, const RowArgs g) {
   using P = Pack<T, V>;
-  constexpr int NW = 4, CH = 8;  // choices taken at once
-  __shared__ float part[NW][CH];
+  constexpr int N = grad_packs<V, U>(), NW = 4;
+  __shared__ float part[NW][U];
   griddep_launch();
   griddep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int t = blockIdx.x; t < g.tokens; t += gridDim.x) {
-    const P* dy = reinterpret_cast<const P*>(ddst + t * g.pitch_token);
-    for (int j0 = 0; j0 < g.choices; j0 += CH) {
-      float dot[CH];
+  const long long t = blockIdx.x;
+  const T* dy = ddst + t * g.pitch_token;
+  for (int j0 = 0; j0 < g.choices; j0 += 32) {
+    const Choices c(g, t, j0, lane);
+    const int here = min(32, g.choices - j0);
+    for (int j = 0; j < here; j += U) {
+      float dot[U], w[U];
+      int pos[U];
 #pragma unroll
-      for (int j = 0; j < CH; ++j) dot[j] = 0.f;
-      for (long long p0 = tid; p0 < g.packs; p0 += 128) {
-        const P d = dy[p0];
+      for (int u = 0; u < U; ++u) {
+        dot[u] = 0.f;
+        pos[u] = __shfl_sync(~0u, c.pos, (j + u) & 31);
+        w[u] = __shfl_sync(~0u, c.w, (j + u) & 31);
+        if (j + u >= here) pos[u] = -1;
+      }
+      for (long long p0 = tid; p0 < g.packs; p0 += 128 * N) {
+        P d[N], y[U][N];
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          if (j0 + j >= g.choices) break;
-          const int pos = __ldg(g.inverse + (long long)t * g.choices + j0 + j);
-          if (static_cast<unsigned>(pos) >= static_cast<unsigned>(g.positions)) continue;
-          const float w = g.weights ? load_weight(g.weights, g.w_dtype, t * g.ws_token + (j0 + j) * g.ws_choice) : 1.f;
-          const P y = reinterpret_cast<const P*>(src + pos * g.pitch_sorted)[p0];
-          P o;
+        for (int i = 0; i < N; ++i) d[i].load(dy, min(p0 + i * 128, g.packs - 1));
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float de = row_elem_to_float<T>(d.e[e]);
-            dot[j] += de * row_elem_to_float<T>(y.e[e]);
-            o.e[e] = float_to_row_elem<T>(w * de);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < N; ++i) y[u][i].load(src + max(pos[u], 0) * g.pitch_sorted, min(p0 + i * 128, g.packs - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (pos[u] < 0) continue;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (p0 + i * 128 >= g.packs) continue;
+            P o;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float de = d[i].at(e);
+              dot[u] += de * y[u][i].at(e);
+              o.set(e, w[u] * de);
+            }
+            o.store(dsrc + pos[u] * g.pitch_dsorted, p0 + i * 128);
           }
-          reinterpret_cast<P*>(dsrc + pos * g.pitch_dsorted)[p0] = o;
         }
       }
 #pragma unroll
-      for (int j = 0; j < CH; ++j) {
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(~0u, dot[j], d);
-        if (lane == 0) part[warp][j] = dot[j];
+        for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(~0u, dot[u], d);
+        if (lane == 0) part[warp][u] = dot[u];
       }
       __syncthreads();
-      if (tid < CH && j0 + tid < g.choices) {
+      if (tid < U && j + tid < here) {
         const float s = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        store_weight(g.dweights, g.w_dtype, t * g.dws_token + (j0 + tid) * g.dws_choice, s);
+        store_weight(g.dweights, g.w_dtype, t * g.dws_token + (j0 + j + tid) * g.dws_choice, s);
       }
       __syncthreads();
     }
@@ -375,13 +477,15 @@ static bool rows_on_16_bytes(const moye_tensor_t* t) {
          (t->shape[0] <= 1 || (t->stride[0] * eb) % 16 == 0);
 }
 
-static unsigned row_grid(moye_b200_ctx* h, const RowArgs& g) {
-  const long long items = (g.packs + 32 * kRowPacks - 1) / (32 * kRowPacks) * g.tokens;
-  const long long cap = (long long)h->num_sms * 8, blocks = (items + 7) / 8;
-  return (unsigned)(blocks < cap ? blocks : cap);
+// CTAs of 8 warps, a warp per `packs_per_lane * 32` packs of a row.  More tokens than a grid holds are refused.
+static int row_grid(const char* who, const RowArgs& g, int packs_per_lane, unsigned* grid) {
+  const long long warps = (g.packs + 32 * packs_per_lane - 1) / (32 * packs_per_lane) * g.tokens, blocks = (warps + 7) / 8;
+  if (warps > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many rows of this width", who);
+  *grid = (unsigned)blocks;
+  return MOYE_OK;
 }
 
-int launch_gather_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_tensor_t* src, const int* inverse, int choices,
+int launch_gather_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_tensor_t* src, const int* inverse, int choices,
                        cudaStream_t stream) {
   if (int rc = check_rows("gather_rows", src, dst, choices)) return rc;
   const int eb = dtype_bytes(src->dtype);
@@ -400,7 +504,9 @@ int launch_gather_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_te
     g.packs = src->shape[1] / V;
     g.pitch_token = src->stride[0];
     g.pitch_sorted = dst->stride[0];
-    MOYE_CUDA(launch_dependent(gather_rows_kernel<T, V>, dim3(row_grid(h, g)), dim3(256), 0, stream, static_cast<T*>(dst->ptr),
+    unsigned grid;
+    if (int rc = row_grid("gather_rows", g, gather_packs<V>(), &grid)) return rc;
+    MOYE_CUDA(launch_dependent(gather_rows_kernel<T, V>, dim3(grid), dim3(256), 0, stream, static_cast<T*>(dst->ptr),
                                static_cast<const T*>(src->ptr), g));
     return MOYE_OK;
   };
@@ -434,7 +540,7 @@ static int for_float_rows(const char* who, int dtype, bool wide, F f) {
   }
 }
 
-int launch_combine_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
+int launch_combine_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
                         const int* inverse, int choices, cudaStream_t stream) {
   if (int rc = check_rows("combine_rows", dst, src, choices)) return rc;
   if (weights)
@@ -459,13 +565,17 @@ int launch_combine_rows(moye_b200_ctx* h, const moye_tensor_t* dst, const moye_t
     using T = decltype(elem);
     constexpr int V = decltype(v)::value;
     g.packs = dst->shape[1] / V;
-    MOYE_CUDA(launch_dependent(combine_rows_kernel<T, V>, dim3(row_grid(h, g)), dim3(256), 0, stream, static_cast<T*>(dst->ptr),
-                               static_cast<const T*>(src->ptr), g));
-    return MOYE_OK;
+    auto run = [&](auto u) -> int {
+      constexpr int U = decltype(u)::value;
+      MOYE_CUDA(launch_dependent(combine_rows_kernel<T, V, U>, dim3((unsigned)g.tokens), dim3(128), 0, stream, static_cast<T*>(dst->ptr),
+                                 static_cast<const T*>(src->ptr), g));
+      return MOYE_OK;
+    };
+    return choices <= 2 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 4>());
   });
 }
 
-int launch_combine_rows_grad(moye_b200_ctx* h, const moye_tensor_t* dsrc, const moye_tensor_t* dweights, const moye_tensor_t* ddst,
+int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const moye_tensor_t* dweights, const moye_tensor_t* ddst,
                              const moye_tensor_t* src, const moye_tensor_t* weights, const int* inverse, int choices,
                              cudaStream_t stream) {
   if (int rc = check_rows("combine_rows_grad", ddst, src, choices)) return rc;
@@ -497,11 +607,12 @@ int launch_combine_rows_grad(moye_b200_ctx* h, const moye_tensor_t* dsrc, const 
     using T = decltype(elem);
     constexpr int V = decltype(v)::value;
     g.packs = ddst->shape[1] / V;
-    const long long cap = (long long)h->num_sms * 16;
-    const unsigned blocks = (unsigned)(g.tokens < cap ? g.tokens : cap);
-    MOYE_CUDA(launch_dependent(combine_rows_grad_kernel<T, V>, dim3(blocks), dim3(128), 0, stream, static_cast<T*>(dsrc->ptr),
-                               static_cast<const T*>(ddst->ptr), static_cast<const T*>(src->ptr), g));
-    return MOYE_OK;
+    auto run = [&](auto u) -> int {
+      MOYE_CUDA(launch_dependent(combine_rows_grad_kernel<T, V, decltype(u)::value>, dim3((unsigned)g.tokens), dim3(128), 0, stream,
+                                 static_cast<T*>(dsrc->ptr), static_cast<const T*>(ddst->ptr), static_cast<const T*>(src->ptr), g));
+      return MOYE_OK;
+    };
+    return choices <= 2 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 4>());
   });
 }
 

@@ -37,14 +37,30 @@ class RowGroups:
     position of a choice, -1 if it was dropped.  A plan made once can be filled again by `group_rows_` (a captured
     step needs that: the tensors keep their addresses)."""
 
-    __slots__ = ("order", "offsets", "inverse", "tokens", "choices", "groups", "_at")
+    __slots__ = ("tokens", "choices", "groups", "_buf", "_at")
 
     def __init__(self, tokens, choices, groups, device):
-        self.order = torch.empty(tokens * choices, dtype=_INT32, device=device)
-        self.offsets = torch.empty(groups + 1, dtype=_INT32, device=device)
-        self.inverse = torch.empty((tokens, choices), dtype=_INT32, device=device)
         self.tokens, self.choices, self.groups = tokens, choices, groups
-        self._at = self.order.get_device()
+        self._buf = torch.empty(2 * tokens * choices + groups + 1, dtype=_INT32, device=device)  # order, inverse, offsets
+        self._at = self._buf.get_device()
+
+    @property
+    def order(self):
+        return self._buf[:self.tokens * self.choices]
+
+    @property
+    def inverse(self):
+        n = self.tokens * self.choices
+        return self._buf[n:2 * n].view(self.tokens, self.choices)
+
+    @property
+    def offsets(self):
+        return self._buf[2 * self.tokens * self.choices:]
+
+    def _pointers(self):
+        """Addresses of order, inverse and offsets."""
+        p, n = self._buf.data_ptr(), 4 * self.tokens * self.choices
+        return p, p + n, p + 2 * n
 
 
 def _arg(x, rank, what):
@@ -122,8 +138,8 @@ def group_rows_(plan, ids, stream=None):
         raise _lib.MoyeError(-4, f"the plan is for ({plan.tokens}, {plan.choices}) choices, ids are {tuple(ids.shape)}")
     if dev != plan._at:
         _differ()
-    _call(_lib.load().moye_b200_group_rows, dev, stream, t, plan.groups, plan.order.data_ptr(), plan.offsets.data_ptr(),
-          plan.inverse.data_ptr())
+    order, inverse, offsets = plan._pointers()
+    _call(_lib.load().moye_b200_group_rows, dev, stream, t, plan.groups, order, offsets, inverse)
     return plan
 
 
@@ -135,7 +151,7 @@ def gather_rows_(dst, src, plan, stream=None):
     ts, d1 = _arg(src, 2, "src")
     if not dev == d1 == plan._at:
         _differ()
-    _call(_lib.load().moye_b200_gather_rows, dev, stream, td, ts, plan.inverse.data_ptr(), plan.choices)
+    _call(_lib.load().moye_b200_gather_rows, dev, stream, td, ts, plan._pointers()[1], plan.choices)
     return dst
 
 
@@ -147,7 +163,7 @@ def combine_rows_(dst, src, plan, weights=None, stream=None):
     tw, d2 = (None, dev) if weights is None else _arg(weights, 2, "weights")
     if not dev == d1 == d2 == plan._at:
         _differ()
-    _call(_lib.load().moye_b200_combine_rows, dev, stream, td, ts, tw, plan.inverse.data_ptr(), plan.choices)
+    _call(_lib.load().moye_b200_combine_rows, dev, stream, td, ts, tw, plan._pointers()[1], plan.choices)
     return dst
 
 
@@ -162,13 +178,17 @@ def combine_rows_grad_(dsrc, dweights, ddst, src, plan, weights, stream=None):
     t4, d4 = _arg(weights, 2, "weights")
     if not dev == d1 == d2 == d3 == d4 == plan._at:
         _differ()
-    _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, t0, t1, t2, t3, t4, plan.inverse.data_ptr(), plan.choices)
+    _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, t0, t1, t2, t3, t4, plan._pointers()[1], plan.choices)
     return dsrc, dweights
 
 
 def _borders(offsets, groups, dev):
     if isinstance(offsets, RowGroups):
-        offsets = offsets.offsets
+        if offsets._at != dev:
+            _differ()
+        if offsets.groups != groups:
+            raise _lib.MoyeError(-4, f"the plan has {offsets.groups} groups, the weights {groups}")
+        return offsets._pointers()[2]
     return _vector(offsets, "offsets", dev, groups + 1)
 
 
