@@ -155,9 +155,9 @@ int encode_tmap_2d_uncached(CUtensorMap* out, const void* ptr, int dtype, uint64
   return MOYE_OK;
 }
 
-// A rank-3 map of 16-bit elements with the 128-byte swizzle and a box one deep along the outermost mode (the group).
+// A rank-3 map with a box one deep along the outermost mode (the group).
 int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1, uint64_t dim2,
-                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1) {
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, bool swizzle128) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) MOYE_FAIL(MOYE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   CUtensorMapDataType tdt;
@@ -167,7 +167,8 @@ int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, 
   cuuint32_t box[3] = {box0, box1, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(out, tdt, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     MOYE_FAIL(MOYE_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d (dims %llu x %llu x %llu, pitches %llu, %llu)", (int)r,
               (unsigned long long)dim0, (unsigned long long)dim1, (unsigned long long)dim2, (unsigned long long)stride1_bytes,

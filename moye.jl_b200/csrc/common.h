@@ -157,7 +157,7 @@ int encode_tmap_2d_uncached(CUtensorMap* out, const void* ptr, int dtype, uint64
                             uint64_t stride1_bytes, uint32_t box0, uint32_t box1, bool swizzle128);
 
 int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1, uint64_t dim2,
-                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1);
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, bool swizzle128);
 
 // Raises a kernel's dynamic shared-memory limit the first time this handle launches it.
 template <typename K>

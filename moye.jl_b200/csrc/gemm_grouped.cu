@@ -9,12 +9,18 @@
 //
 // The accumulator is turned against the dense kernels': the tensor-memory lanes (the M of the instruction, always full)
 // run along the output's contiguous mode -- the weight's rows in the forward product, the features of A in the
-// gradient -- and the columns (its N, 16 to 256) along the rows of the group or of the weight.  A group of a few rows
-// then costs a narrow instruction instead of a 128-row tile that is mostly padding, the last tile of a group simply
-// stores fewer columns, and a warp's 32 lanes store 32 neighbouring elements.
+// gradient -- and the columns (its N, a multiple of 32 up to 256, chosen per tile) along the rows of the group or of the
+// weight.  A group of a few rows then costs a narrow instruction instead of a 128-row tile that is mostly padding, the
+// last tile of a group simply has fewer columns, and a warp's 32 lanes are 32 neighbouring elements of an output row.
 //
-// Persistent CTAs of 6 warps as in the dense kernels: warp 0 TMA producer, warp 1 tcgen05.mma issuer, warps 2-5
-// epilogue, accumulator double-buffered in tensor memory.
+// Persistent CTA pairs (tcgen05 cta_group::2, see gemm_pair.cu): 256 lanes x up to 256 columns, each CTA holds 128 lanes
+// and half of the column operand.  Per CTA: warp 0 TMA producer, warp 1 tcgen05.mma issuer (leader), warp 2 reads the
+// borders and, in the gradient, clears the rows behind a group's end, warps 4-7 epilogue; accumulators double-buffered.
+//
+// The tensor cores cut the sum after every instruction's 16 products instead of rounding it, always towards zero: for a
+// 16-bit output far below its step, but a Float32 output loses precision in proportion to the length of the sum (1.2e-6
+// at 1000, plain fp32 sums 6e-7).  Float32 outputs are therefore summed in runs of 512 that the epilogue adds up in
+// registers, rounding to nearest (`PROMOTE`).
 #include <cstring>
 
 #include "gemm_common.cuh"
@@ -22,8 +28,10 @@
 namespace moye {
 
 constexpr int kMaxGemmGroups = 1024;
-enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164 };
+enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164, SITEG_FIX_TAIL = 165 };
 enum : int { GROUPED_K_MAJOR = 0, GROUPED_MN_MAJOR = 1, GROUPED_GRAD = 2 };
+
+constexpr int kPromoteBlocks = 8;  // blocks of 64 summed in tensor memory before registers take over
 
 struct GroupedArgs {
   int rows, groups;
@@ -31,8 +39,9 @@ struct GroupedArgs {
   int cols;             // gradient: extent of the other mode (N)
   int k_blocks;         // forward: blocks of 64 along K
   int lane_tiles, col_tiles;
+  int tma_out;          // D may be written by TMA: 16-byte base and pitches, beta == 0
   const int* offsets;
-  uint32_t idesc;
+  uint32_t idesc;       // without N
   float alpha, beta;
   void* D;
   long long ld, group_stride;  // elements
@@ -42,6 +51,7 @@ struct GroupedArgs {
 struct GroupedTile {
   int g, row0, nrows;  // the group, its first row here and the rows of it this tile reads (gradient: all of them)
   int lane0, col0;     // first output element along the two modes (forward: col0 = row0)
+  int ncols, width;    // columns to store; the instruction's N, a multiple of 32
 };
 
 template <int MODE, int BT>
@@ -52,16 +62,24 @@ struct GroupedSchedule {
   __device__ __forceinline__ int total() const {
     return MODE == GROUPED_GRAD ? a.groups * a.lane_tiles * a.col_tiles : before[a.groups] * a.lane_tiles;
   }
+  // Tile q of a group's lane_tiles x col_tiles: bands of 8 column tiles, whose operand stays in L2 while the lane tiles pass.
+  __device__ __forceinline__ void place(int q, int col_tiles, int& lt, int& ct) const {
+    const int band = q / (a.lane_tiles * 8), first = band * 8, w = min(8, col_tiles - first);
+    const int r = q - band * a.lane_tiles * 8;
+    ct = first + r % w;
+    lt = r / w;
+  }
   __device__ __forceinline__ GroupedTile at(int t) const {
     GroupedTile r;
+    int lt, ct;
     if (MODE == GROUPED_GRAD) {
       const int per = a.lane_tiles * a.col_tiles;
       r.g = t / per;
-      const int q = t - r.g * per;
-      r.lane0 = (q % a.lane_tiles) * 128;
-      r.col0 = (q / a.lane_tiles) * BT;
+      place(t - r.g * per, a.col_tiles, lt, ct);
+      r.col0 = ct * BT;
       r.row0 = row_of[r.g];
       r.nrows = row_of[r.g + 1] - r.row0;
+      r.ncols = min(BT, a.cols - r.col0);
     } else {
       int lo = 0, hi = a.groups;  // the group whose tiles hold t: before[lo] * lane_tiles <= t < before[lo + 1] * lane_tiles
       while (hi - lo > 1) {
@@ -70,12 +88,17 @@ struct GroupedSchedule {
         else hi = mid;
       }
       r.g = lo;
-      const int q = t - before[lo] * a.lane_tiles, tiles = before[lo + 1] - before[lo];
-      r.lane0 = (q / tiles) * 128;
-      r.row0 = row_of[lo] + (q % tiles) * BT;
-      r.nrows = min(BT, row_of[lo + 1] - r.row0);
+      const int tiles = before[lo + 1] - before[lo], count = row_of[lo + 1] - row_of[lo];
+      place(t - before[lo] * a.lane_tiles, tiles, lt, ct);
+      // a few tiles share a group's rows evenly; of many only the last is narrow
+      const int step = tiles <= 4 ? ((count + tiles - 1) / tiles + 31) & ~31 : BT;
+      r.row0 = row_of[lo] + ct * step;
+      r.nrows = min(step, row_of[lo + 1] - r.row0);
       r.col0 = r.row0;
+      r.ncols = r.nrows;
     }
+    r.lane0 = lt * 256;
+    r.width = (r.ncols + 31) & ~31;
     return r;
   }
   __device__ __forceinline__ int k_blocks(const GroupedTile& r) const {
@@ -116,52 +139,63 @@ __device__ __forceinline__ void grouped_borders(const GroupedArgs& a, int* row_o
 }
 
 template <int MODE, typename OutT, int BT, int STAGES>
-__global__ void __launch_bounds__(192, 1)
-gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC, const GroupedArgs a) {
-  // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD)
+__global__ void __launch_bounds__(256, 1)
+gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
+                    const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
+  // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmD: the output
   constexpr int BK = 64, UMMA_K = 16;
   constexpr int L_BYTES = 128 * 128;
-  constexpr int C_BYTES = BT * 128;
+  constexpr int C_BYTES = BT / 2 * 128;  // this CTA's half of the columns
   constexpr int STAGE_BYTES = L_BYTES + C_BYTES;
-  constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
+  constexpr uint32_t TMEM_COLS = 2 * BT;
   constexpr bool L_MN = MODE != GROUPED_K_MAJOR, C_MN = MODE == GROUPED_GRAD;
-  constexpr int CHUNK = BT < 32 ? BT : 32;
+  constexpr bool PROMOTE = sizeof(OutT) == 4;
+  constexpr int EPI_BUF = 32 * 32 * (int)sizeof(OutT);  // [32 columns][32 lanes], a warp's staging tile
+  static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128) && (!PROMOTE || BT <= 128), "tile columns");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint8_t* epi = smem + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + 8 * EPI_BUF);
   uint64_t* full = bars;
   uint64_t* empty = bars + STAGES;
-  uint64_t* acc_full = bars + 2 * STAGES;
-  uint64_t* acc_empty = bars + 2 * STAGES + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  uint64_t* tail = bars + 2 * STAGES;  // gradient: a group's last block has landed, its rows are not cleared yet
+  uint64_t* acc_full = bars + 3 * STAGES;
+  uint64_t* acc_empty = bars + 3 * STAGES + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 4);
   int* row_of = reinterpret_cast<int*>(tmem_holder + 2);
   int* before = row_of + kMaxGemmGroups + 1;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();  // 0 = leader
+  const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
+      mbar_init(&tail[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], 8);
     }
     fence_mbar_init();
-    if (a.rows > 0) {  // without rows the maps are not set up, and nothing is loaded
+    if (a.rows > 0) {  // without rows the operands' maps are not set up, and nothing is loaded
       prefetch_tensormap(&tmL);
       prefetch_tensormap(&tmC);
     }
+    if (a.tma_out) prefetch_tensormap(&tmD);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, TMEM_COLS);
-    tmem_relinquish();
+    tmem_alloc2(tmem_holder, TMEM_COLS);
+    tmem_relinquish2();
   }
   tc_fence_before_sync();
   __syncthreads();
+  cluster_arrive();
+  cluster_wait();  // both CTAs' barriers are initialised and both halves of the TMEM pair are allocated
   tc_fence_after_sync();
   griddep_launch();  // programmatic dependent launch, after the tensor-memory allocation; nothing above touches global memory
   griddep_wait();
@@ -172,122 +206,153 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   const int num_tiles = sched.total();
 
   if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+    // ------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+      const uint32_t leader_full0 = mapa_shared(smem_u32(&full[0]), 0);
+      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
         const GroupedTile tile = sched.at(t);
         const int kbs = sched.k_blocks(tile);
+        const int l0 = tile.lane0 + rank * 128, c0 = tile.col0 + rank * (tile.width / 2);
         for (int kb = 0; kb < kbs; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, a.status, SITEG_PROD_EMPTY)) { ok = false; break; }
-          mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
           uint8_t* sl = smem + stage * STAGE_BYTES;
           uint8_t* sc = sl + L_BYTES;
-          if constexpr (MODE == GROUPED_K_MAJOR) {
-            tma_load_3d(sl, &tmL, &full[stage], kb * BK, tile.lane0, tile.g);
-          } else if constexpr (MODE == GROUPED_MN_MAJOR) {
-            for (int c = 0; c < 2; ++c) tma_load_3d(sl + c * (BK * 128), &tmL, &full[stage], tile.lane0 + c * 64, kb * BK, tile.g);
+          auto load = [&](auto&& load2, auto&& load3) {
+            if constexpr (MODE == GROUPED_K_MAJOR) {
+              load3(sl, &tmL, kb * BK, l0, tile.g);
+            } else if constexpr (MODE == GROUPED_MN_MAJOR) {
+              for (int c = 0; c < 2; ++c) load3(sl + c * (BK * 128), &tmL, l0 + c * 64, kb * BK, tile.g);
+            } else {
+              for (int c = 0; c < 2; ++c) load2(sl + c * (BK * 128), &tmL, l0 + c * 64, tile.row0 + kb * BK);
+            }
+            if constexpr (C_MN) {
+              for (int c = 0; c < BT / 128; ++c) load2(sc + c * (BK * 128), &tmC, c0 + c * 64, tile.row0 + kb * BK);
+            } else {
+              load2(sc, &tmC, kb * BK, c0);
+            }
+          };
+          const bool cleared = MODE == GROUPED_GRAD && tile.nrows - kb * BK < BK;  // warp 2 passes this block on
+          if (rank == 0 || cleared) {
+            uint64_t* bar = cleared ? &tail[stage] : &full[stage];
+            mbar_arrive_expect_tx(bar, STAGE_BYTES);
+            load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d(d, m, bar, x, y); },
+                 [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d(d, m, bar, x, y, z); });
           } else {
-            for (int c = 0; c < 2; ++c) tma_load_2d(sl + c * (BK * 128), &tmL, &full[stage], tile.lane0 + c * 64, tile.row0 + kb * BK);
-          }
-          if constexpr (C_MN) {
-            for (int c = 0; c < BT / 64; ++c) tma_load_2d(sc + c * (BK * 128), &tmC, &full[stage], tile.col0 + c * 64, tile.row0 + kb * BK);
-          } else {
-            tma_load_2d(sc, &tmC, &full[stage], kb * BK, tile.row0);
+            const uint32_t bar = leader_full0 + stage * 8;
+            mbar_arrive_expect_tx_remote(bar, STAGE_BYTES);
+            load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d_pair(d, m, bar, x, y); },
+                 [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d_pair(d, m, bar, x, y, z); });
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    int stage = 0;
-    uint32_t phase = 0;
-    int lt = 0;
-    bool ok = true;
-    const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
-    for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-      const GroupedTile tile = sched.at(t);
-      const int kbs = sched.k_blocks(tile);
-      if (kbs == 0) continue;
-      const int buf = lt & 1;
-      const uint32_t aphase = (lt >> 1) & 1;
-      ++lt;
-      if (lane == 0) ok = mbar_wait(&acc_empty[buf], aphase ^ 1, a.status, SITEG_MMA_ACC);
-      ok = __shfl_sync(~0u, ok, 0);
-      if (!ok) break;
-      tc_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + buf * BT;
-      for (int kb = 0; kb < kbs; ++kb) {
-        if (lane == 0) ok = mbar_wait(&full[stage], phase, a.status, SITEG_MMA_FULL);
-        ok = __shfl_sync(~0u, ok, 0);
-        if (!ok) break;
-        uint8_t* sl = smem + stage * STAGE_BYTES;
-        if constexpr (MODE == GROUPED_GRAD) {
-          // The last block of a group reaches into the next group's rows (or past the last one, where anything may
-          // lie): their K rows are zeroed in both operands.  A K row is 128 bytes in every chunk, swizzled in itself.
-          const int valid = tile.nrows - kb * BK;
-          if (valid < BK) {
-            for (int c = 0; c < 2 + BT / 64; ++c)
-              for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
-                *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async_smem();
-            __syncwarp();
+    // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int lt = 0;
+      bool ok = true;
+      const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
+      const uint32_t empty_local = smem_u32(&empty[0]), empty_peer = mapa_shared(empty_local, 1);
+      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+        const GroupedTile tile = sched.at(t);
+        const int kbs = sched.k_blocks(tile);
+        const uint32_t idesc = a.idesc | ((uint32_t)(tile.width >> 3) << 17);
+        for (int seg = 0; seg < kbs && ok; seg += PROMOTE ? kPromoteBlocks : kbs, ++lt) {
+          const int buf = lt & 1, end = PROMOTE ? min(seg + kPromoteBlocks, kbs) : kbs;
+          const uint32_t aphase = (lt >> 1) & 1;
+          ok = mbar_wait(&acc_empty[buf], aphase ^ 1, a.status, SITEG_MMA_ACC);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t d_tmem = tmem_base + buf * BT;
+          for (int kb = seg; kb < end; ++kb) {
+            // a cleared block was written by threads of both CTAs
+            ok = MODE == GROUPED_GRAD ? mbar_wait_cluster(&full[stage], phase, a.status, SITEG_MMA_FULL)
+                                      : mbar_wait(&full[stage], phase, a.status, SITEG_MMA_FULL);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t s = smem_u32(smem + stage * STAGE_BYTES);
+            const uint64_t ld = dl.base + (s >> 4), cd = dc.base + ((s + L_BYTES) >> 4);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k)
+              tc_mma_ss2<KIND_F16>(d_tmem, ld + k * dl.kstep, cd + k * dc.kstep, idesc, (kb > seg || k > 0) ? 1u : 0u);
+            tc_commit2(empty_local + stage * 8);
+            tc_commit2(empty_peer + stage * 8);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (ok) {
+            const uint32_t f_local = smem_u32(&acc_full[buf]);
+            tc_commit2(f_local);
+            tc_commit2(mapa_shared(f_local, 1));
           }
         }
-        if (lane == 0) {
-          tc_fence_after_sync();
-          const uint32_t s = smem_u32(sl);
-          const uint64_t ld = dl.base + (s >> 4), cd = dc.base + ((s + L_BYTES) >> 4);
-#pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)
-            tc_mma_ss<KIND_F16>(d_tmem, ld + k * dl.kstep, cd + k * dc.kstep, a.idesc, (kb | k) != 0 ? 1u : 0u);
-          tc_commit(&empty[stage]);
-          if (kb == kbs - 1) tc_commit(&acc_full[buf]);
-        }
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
-  } else {
-    // ------------------------------------------------------------ epilogue (warps 2..5)
+    __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ rows behind a group's end (gradient, both CTAs)
+    // The last block of a group reaches into the next group's rows, or past the last one, where anything may lie: those K
+    // rows are zeroed in both operands.  A K row is 128 bytes in every chunk, swizzled within itself.
+    if constexpr (MODE == GROUPED_GRAD) {
+      int pos = 0;            // stages used before this tile
+      uint32_t phases = 0;    // one bit per stage
+      for (int t = first_tile; t < num_tiles; t += tile_step) {
+        const GroupedTile tile = sched.at(t);
+        const int kbs = sched.k_blocks(tile), valid = tile.nrows - (kbs - 1) * BK;
+        if (kbs > 0 && valid < BK) {
+          const int stage = (pos + kbs - 1) % STAGES;
+          bool ok = true;
+          if (lane == 0) ok = mbar_wait(&tail[stage], (phases >> stage) & 1, a.status, SITEG_FIX_TAIL);
+          ok = __shfl_sync(~0u, ok, 0);
+          if (!ok) break;
+          phases ^= 1u << stage;
+          uint8_t* sl = smem + stage * STAGE_BYTES;
+          for (int c = 0; c < 2 + BT / 128; ++c)
+            for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
+              *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote_release(mapa_shared(smem_u32(&full[stage]), 0));
+        }
+        pos = (pos + kbs) % STAGES;
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue (warps 4..7, both CTAs)
     const int q = warp & 3;
-    int lt = 0;
-    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+    uint8_t* my_buf = epi + (warp - 4) * 2 * EPI_BUF;
+    int nstore = 0, lt = 0;
+    bool ok = true;
+    for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
       const GroupedTile tile = sched.at(t);
       const int kbs = sched.k_blocks(tile);
-      const int buf = lt & 1;
-      const uint32_t aphase = (lt >> 1) & 1;
-      if (kbs != 0) {
-        ++lt;
-        if (!mbar_wait(&acc_full[buf], aphase, a.status, SITEG_EPI_ACC)) break;
-        tc_fence_after_sync();
-      }
-      const int m = tile.lane0 + q * 32 + lane;
-      const int ncols = MODE == GROUPED_GRAD ? min(BT, a.cols - tile.col0) : tile.nrows;
+      const int m0 = tile.lane0 + rank * 128 + q * 32, m = m0 + lane;
       OutT* out = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld + m;
-      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BT;
-#pragma unroll 1
-      for (int c = 0; c < BT; c += CHUNK) {
-        uint32_t v[CHUNK];
-        if (kbs != 0) {
-          if constexpr (CHUNK == 32) tmem_ld_x32(t_addr + c, v);
-          else tmem_ld_x16(t_addr + c, v);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] = 0u;
-        }
-        if (kbs != 0 && c + CHUNK >= BT) {
-          tc_fence_before_sync();
+      // 32 columns from registers to D: by TMA where the whole block belongs to this tile, else element by element
+      auto store = [&](int c, const uint32_t (&v)[32]) {
+        if (a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols)) {
+          OutT* sb = reinterpret_cast<OutT*>(my_buf + (nstore & 1) * EPI_BUF);
+          if (lane == 0) tma_store_wait_read<1>();  // the store that last used `sb` has drained
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        }
-        if (m < a.lanes) {
 #pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
-            if (c + j < ncols) {
+          for (int j = 0; j < 32; ++j) sb[j * 32 + lane] = cvt_out<OutT>(__uint_as_float(v[j]) * a.alpha);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && m0 < a.lanes) {
+            if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, sb, m0, tile.col0 + c, tile.g);
+            else tma_store_2d(&tmD, sb, m0, tile.col0 + c);
+          }
+          if (lane == 0) tma_store_commit();
+          ++nstore;
+        } else if (m < a.lanes) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (c + j < tile.ncols) {
               OutT* p = out + (c + j) * a.ld;
               float x = __uint_as_float(v[j]) * a.alpha;
               if (a.beta != 0.f) x += a.beta * load_c_as_float<OutT>(p, 0);
@@ -295,8 +360,68 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
             }
           }
         }
+      };
+      auto arrived = [&]() {  // waits for the accumulator of the next run
+        ok = mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC);
+        tc_fence_after_sync();
+        return ok;
+      };
+      auto release = [&]() {  // hands the accumulator back after its last read
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive(&acc_empty[lt & 1]);
+          else mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[lt & 1]), 0));
+        }
+        ++lt;
+      };
+      const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+      if constexpr (PROMOTE) {
+        float acc[BT];
+#pragma unroll
+        for (int j = 0; j < BT; ++j) acc[j] = 0.f;
+        for (int seg = 0; seg < kbs; seg += kPromoteBlocks) {
+          if (!arrived()) break;
+#pragma unroll
+          for (int c = 0; c < BT; c += 32) {
+            if (c < tile.width) {
+              uint32_t v[32];
+              tmem_ld_x32(t_lane + (lt & 1) * BT + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(v[j]);
+            }
+          }
+          release();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < BT; c += 32) {
+          if (c < tile.width) {
+            uint32_t v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[c + j]);
+            store(c, v);
+          }
+        }
+      } else {
+        if (kbs > 0 && !arrived()) break;
+#pragma unroll 1
+        for (int c = 0; c < tile.width; c += 32) {
+          uint32_t v[32];
+          if (kbs > 0) {
+            tmem_ld_x32(t_lane + (lt & 1) * BT + c, v);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          }
+          if (kbs > 0 && c + 32 >= tile.width) release();
+          store(c, v);
+        }
       }
     }
+    if (lane == 0) tma_store_wait_all<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -305,45 +430,63 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   }
   tc_fence_before_sync();
   __syncthreads();
+  // neither CTA may leave while its partner can still signal its barriers or read its operands
+  cluster_arrive();
+  cluster_wait();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    tmem_dealloc2(tmem_base, TMEM_COLS);
   }
 }
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int MODE, typename OutT, int BT>
-static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a, long long tiles,
-                               cudaStream_t stream) {
-  constexpr int EXTRA = 1024 + 512 + 2 * (kMaxGemmGroups + 1) * 4;
-  constexpr int STAGE = 128 * 128 + BT * 128;
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td, const GroupedArgs& a,
+                               long long tiles, cudaStream_t stream) {
+  constexpr int EXTRA = 1024 + 512 + 2 * (kMaxGemmGroups + 1) * 4 + 8 * 32 * 32 * (int)sizeof(OutT);
+  constexpr int STAGE = 128 * 128 + BT / 2 * 128;
   constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE < 12 ? (227 * 1024 - EXTRA) / STAGE : 12;
   constexpr int SMEM = STAGES * STAGE + EXTRA;
   auto kern = gemm_grouped_kernel<MODE, OutT, BT, STAGES>;
   if (int rc = configure_once(h, kern, SMEM)) return rc;
-  const unsigned grid = (unsigned)(tiles < h->num_sms ? tiles : h->num_sms);
-  MOYE_CUDA(launch_dependent(kern, dim3(grid), dim3(192), SMEM, stream, tl, tc, a));
+  const long long pairs = tiles < h->num_sms / 2 ? tiles : h->num_sms / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = launch_without_pdl() ? 1 : 2;
+  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, td, a));
   return MOYE_OK;
 }
 
 template <int MODE, typename OutT>
-static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a,
-                             long long tiles, cudaStream_t stream) {
+static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td,
+                             const GroupedArgs& a, long long tiles, cudaStream_t stream) {
   if constexpr (MODE != GROUPED_GRAD) {
-    if (bt == 16) return launch_grouped_inst<MODE, OutT, 16>(h, tl, tc, a, tiles, stream);
-    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, a, tiles, stream);
+    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, td, a, tiles, stream);
+    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, td, a, tiles, stream);
   }
-  if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, a, tiles, stream);
-  if (bt == 128) return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, a, tiles, stream);
-  return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, a, tiles, stream);
+  if constexpr (sizeof(OutT) != 4) {
+    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, td, a, tiles, stream);
+  }
+  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, td, a, tiles, stream);
 }
 
 template <int MODE>
-static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const GroupedArgs& a,
-                              long long tiles, cudaStream_t stream) {
-  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, a, tiles, stream);
-  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, a, tiles, stream);
-  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, a, tiles, stream);
+static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td,
+                              const GroupedArgs& a, long long tiles, cudaStream_t stream) {
+  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, td, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, td, a, tiles, stream);
+  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, td, a, tiles, stream);
 }
 
 static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
@@ -394,19 +537,21 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows or groups of B overlap", who);
   if ((reinterpret_cast<uintptr_t>(B->ptr) & 15) != 0 || (outer > 1 && pitch % 8 != 0) || (G > 1 && B->stride[0] % 8 != 0))
     MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: B needs a base, a row pitch and a group pitch that are multiples of 16 bytes", who);
-  // Columns of a tile: the instruction width that holds an average group, so that weights are streamed once and padding
-  // stays small.
+  // Columns of a tile: what holds an average group, so that its weight is streamed once.
   const int64_t mean = (R + G - 1) / G;
-  const int bt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+  int bt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+  if (D->dtype == MOYE_F32 && bt > 128) bt = 128;  // the epilogue's registers hold 128 sums a thread
+  const int ob = dtype_bytes(D->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
   a.groups = (int)G;
   a.lanes = (int)N;
   a.k_blocks = (int)((K + 63) / 64);
-  a.lane_tiles = (int)((N + 127) / 128);
+  a.lane_tiles = (int)((N + 255) / 256);
+  a.tma_out = beta == 0.f && (reinterpret_cast<uintptr_t>(D->ptr) & 15) == 0 && (R == 1 || (D->stride[0] * ob) % 16 == 0);
   a.offsets = offsets;
   const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
-  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((mn ? 1u : 0u) << 15) | ((uint32_t)(bt / 8) << 17) | (8u << 24);
+  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((mn ? 1u : 0u) << 15) | (16u << 24);
   a.alpha = alpha;
   a.beta = beta;
   a.D = D->ptr;
@@ -414,15 +559,18 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.status = h->d_status;
   const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
   if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc;
+  CUtensorMap tl, tc, td;
+  std::memset(&td, 0, sizeof(td));
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
-                              (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128))
+                              (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
-  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt, true)) return rc;
-  log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 128 x %d", (long long)R, (long long)G, (long long)N,
+  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
+  if (a.tma_out)
+    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 32, 32, false)) return rc;
+  log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype, bt);
-  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, a, tiles, stream);
-  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, a, tiles, stream);
+  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, td, a, tiles, stream);
+  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, td, a, tiles, stream);
 }
 
 int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
@@ -442,17 +590,20 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   if (int rc = check_row_operand(who, "dD", dD)) return rc;
   if ((K > 1 && dB->stride[2] != 1) || (N > 1 && dB->stride[1] < K) || (G > 1 && dB->stride[0] < (N - 1) * dB->stride[1] + K))
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: dB needs contiguous rows, and rows and groups that do not overlap", who);
-  const int bt = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+  const int bt = N <= 128 || dB->dtype == MOYE_F32 ? 128 : 256;  // Float32: the epilogue's registers hold 128 sums a thread
+  const int ob = dtype_bytes(dB->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
   a.groups = (int)G;
   a.lanes = (int)K;
   a.cols = (int)N;
-  a.lane_tiles = (int)((K + 127) / 128);
+  a.lane_tiles = (int)((K + 255) / 256);
   a.col_tiles = (int)((N + bt - 1) / bt);
+  a.tma_out = beta == 0.f && (reinterpret_cast<uintptr_t>(dB->ptr) & 15) == 0 && (N == 1 || (dB->stride[1] * ob) % 16 == 0) &&
+              (G == 1 || (dB->stride[0] * ob) % 16 == 0);
   a.offsets = offsets;
   const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
-  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (3u << 15) | ((uint32_t)(bt / 8) << 17) | (8u << 24);
+  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (3u << 15) | (16u << 24);
   a.alpha = alpha;
   a.beta = beta;
   a.D = dB->ptr;
@@ -461,17 +612,22 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.status = h->d_status;
   const long long tiles = (long long)G * a.lane_tiles * a.col_tiles;
   if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc;
-  if (R > 0) {
+  CUtensorMap tl, tc, td;
+  std::memset(&tl, 0, sizeof(tl));
+  std::memset(&tc, 0, sizeof(tc));
+  std::memset(&td, 0, sizeof(td));
+  if (R > 0) {  // without rows the kernel loads nothing, every group's sum is empty
     if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
     if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
-  } else {  // no rows: the kernel loads nothing, every group's sum is empty
-    std::memset(&tl, 0, sizeof(tl));
-    std::memset(&tc, 0, sizeof(tc));
   }
-  log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 128 x %d", (long long)R, (long long)G,
+  if (a.tma_out) {
+    const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
+    const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
+    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 32, 32, false)) return rc;
+  }
+  log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
            (long long)N, (long long)K, A->dtype, bt);
-  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, a, tiles, stream);
+  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, td, a, tiles, stream);
 }
 
 }  // namespace moye

@@ -150,29 +150,6 @@ struct LoraTileArgs {
   int stages, stage_bytes, v_off, stage_out_off, bar_off;  // shared-memory plan, bytes
 };
 
-__device__ __forceinline__ void mbar_arrive_remote_release(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// A bounded wait that also acquires what other CTAs of the cluster released on this barrier.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* status, int site) {
-#pragma unroll 1
-  for (uint32_t it = 0; it < kSpinLimit; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (it > kSpinFast) __nanosleep(64);
-  }
-  atomicCAS(status, 0, site);
-  return false;
-}
 __device__ __forceinline__ float4 ld_remote_f32x4(uint32_t cluster_addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
@@ -572,8 +549,8 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, cuda
   if (int rc = encode_tmap_2d_uncached(&tx, g.X, dtype, g.k, g.rows, (uint64_t)g.x_pitch * 2, 64, 128, true)) return rc;
   const uint64_t a_pitch = g.a_pitch * 2, a_stride = g.adapters > 1 ? g.a_stride * 2 : g.rank * a_pitch;
   const uint64_t b_pitch = g.n > 1 ? g.b_pitch * 2 : g.rank * 2, b_stride = g.adapters > 1 ? g.b_stride * 2 : g.n * b_pitch;
-  if (int rc = encode_tmap_3d(&ta, g.A, dtype, g.k, g.rank, g.adapters, a_pitch, a_stride, 64, rsteps * 16)) return rc;
-  if (int rc = encode_tmap_3d(&tb, g.B, dtype, g.rank, g.n, g.adapters, b_pitch, b_stride, 64, 128)) return rc;
+  if (int rc = encode_tmap_3d(&ta, g.A, dtype, g.k, g.rank, g.adapters, a_pitch, a_stride, 64, rsteps * 16, true)) return rc;
+  if (int rc = encode_tmap_3d(&tb, g.B, dtype, g.rank, g.n, g.adapters, b_pitch, b_stride, 64, 128, true)) return rc;
   auto kern = lora_tile_kernel<T, OutT, VEC, PARTS>;
   if (int rc = configure_once(h, kern, 227 * 1024)) return rc;
   cudaLaunchConfig_t cfg = {};
