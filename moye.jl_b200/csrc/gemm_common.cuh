@@ -67,6 +67,17 @@ __device__ __forceinline__ void tile_coord(int t, int m_tiles, int n_tiles, int 
   if (grp & 1) ni = n_tiles - 1 - ni;  // serpentine: a new group starts on the B tiles the last one ended on
 }
 
+// Barrier `id` over 128 threads that also ands a flag of each.
+__device__ __forceinline__ bool all_of_128(int id, bool mine) {
+  int r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.s32 q, %2, 0;\nbar.red.and.pred p, %1, 128, q;\nselp.s32 %0, 1, 0, p;\n}\n"
+      : "=r"(r)
+      : "r"(id), "r"((int)mine)
+      : "memory");
+  return r != 0;
+}
+
 template <typename OutT>
 __device__ __forceinline__ OutT cvt_out(float f);
 template <>

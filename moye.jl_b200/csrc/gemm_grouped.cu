@@ -15,7 +15,8 @@
 //
 // Persistent CTA pairs (tcgen05 cta_group::2, see gemm_pair.cu): 256 lanes x up to 256 columns, each CTA holds 128 lanes
 // and half of the column operand.  Per CTA: warp 0 TMA producer, warp 1 tcgen05.mma issuer (leader), warp 2 reads the
-// borders and, in the gradient, clears the rows behind a group's end, warps 4-7 epilogue; accumulators double-buffered.
+// borders and, in the gradient, clears the rows behind a group's end, warp 3 deals the tiles, warps 4-7 epilogue;
+// accumulators double-buffered.
 //
 // The tensor cores cut the sum after every instruction's 16 products instead of rounding it, always towards zero: for a
 // 16-bit output far below its step, but a Float32 output loses precision in proportion to the length of the sum (1.2e-6
@@ -28,7 +29,7 @@
 namespace moye {
 
 constexpr int kMaxGemmGroups = 1024;
-enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164, SITEG_FIX_TAIL = 165 };
+enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164, SITEG_FIX_TAIL = 165, SITEG_RING = 166 };
 enum : int { GROUPED_K_MAJOR = 0, GROUPED_MN_MAJOR = 1, GROUPED_GRAD = 2 };
 
 constexpr int kPromoteBlocks = 8;  // blocks of 64 summed in tensor memory before registers take over
@@ -48,10 +49,33 @@ struct GroupedArgs {
   int* status;
 };
 
-struct GroupedTile {
+struct alignas(16) GroupedTile {
   int g, row0, nrows;  // the group, its first row here and the rows of it this tile reads (gradient: all of them)
   int lane0, col0;     // first output element along the two modes (forward: col0 = row0)
   int ncols, width;    // columns to store; the instruction's N, a multiple of 32
+  int k_blocks;        // blocks of 64 summed; -1: no tile left
+};
+
+// Tiles are worked out by a warp of their own and handed to the others through a ring in shared memory: finding a tile's
+// group takes hundreds of cycles, which the producer and the MMA issuer spent between tiles (32768 rows, 32 groups,
+// 4096 x 2048: 411 us with the search in every role).
+constexpr int kTileRing = 4;
+struct TileRing {
+  GroupedTile* slots;
+  uint64_t *full, *empty;
+  int* status;
+  int n;
+  __device__ __forceinline__ bool take(GroupedTile& t) {  // one reader; `leave` gives the slot back
+    if (!mbar_wait(&full[n % kTileRing], (n / kTileRing) & 1, status, SITEG_RING)) return false;
+    const int4* p = reinterpret_cast<const int4*>(&slots[n % kTileRing]);
+    *reinterpret_cast<int4*>(&t) = p[0];
+    *(reinterpret_cast<int4*>(&t) + 1) = p[1];
+    return t.k_blocks >= 0;
+  }
+  __device__ __forceinline__ void leave() {
+    mbar_arrive(&empty[n % kTileRing]);
+    ++n;
+  }
 };
 
 template <int MODE, int BT>
@@ -99,10 +123,8 @@ struct GroupedSchedule {
     }
     r.lane0 = lt * 256;
     r.width = (r.ncols + 31) & ~31;
+    r.k_blocks = MODE == GROUPED_GRAD ? (r.nrows + 63) >> 6 : a.k_blocks;
     return r;
-  }
-  __device__ __forceinline__ int k_blocks(const GroupedTile& r) const {
-    return MODE == GROUPED_GRAD ? (r.nrows + 63) >> 6 : a.k_blocks;
   }
 };
 
@@ -138,11 +160,15 @@ __device__ __forceinline__ void grouped_borders(const GroupedArgs& a, int* row_o
   }
 }
 
+constexpr int kEpiBufs = 3;
+__host__ __device__ constexpr int grouped_box_rows(int bt) { return bt / 2 < 32 ? bt / 2 : 32; }
+
 template <int MODE, typename OutT, int BT, int STAGES>
 __global__ void __launch_bounds__(256, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
-                    const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
-  // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmD: the output
+                    const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
+  // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmN: the same in
+  // boxes of 32 rows for narrow tiles, tmD: the output
   constexpr int BK = 64, UMMA_K = 16;
   constexpr int L_BYTES = 128 * 128;
   constexpr int C_BYTES = BT / 2 * 128;  // this CTA's half of the columns
@@ -150,20 +176,24 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   constexpr uint32_t TMEM_COLS = 2 * BT;
   constexpr bool L_MN = MODE != GROUPED_K_MAJOR, C_MN = MODE == GROUPED_GRAD;
   constexpr bool PROMOTE = sizeof(OutT) == 4;
-  constexpr int EPI_BUF = 32 * 32 * (int)sizeof(OutT);  // [32 columns][32 lanes], a warp's staging tile
+  constexpr int EPI_BUF = 32 * 128 * (int)sizeof(OutT);  // [32 columns][128 lanes], a staging tile of the four epilogue warps
+  constexpr int C_BOX = grouped_box_rows(BT);            // rows of one load of a K-major column operand
   static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128) && (!PROMOTE || BT <= 128), "tile columns");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + STAGES * STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + 8 * EPI_BUF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + kEpiBufs * EPI_BUF);
   uint64_t* full = bars;
   uint64_t* empty = bars + STAGES;
   uint64_t* tail = bars + 2 * STAGES;  // gradient: a group's last block has landed, its rows are not cleared yet
   uint64_t* acc_full = bars + 3 * STAGES;
   uint64_t* acc_empty = bars + 3 * STAGES + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 4);
-  int* row_of = reinterpret_cast<int*>(tmem_holder + 2);
+  uint64_t* ring_full = bars + 3 * STAGES + 4;
+  uint64_t* ring_empty = ring_full + kTileRing;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ring_empty + kTileRing);
+  GroupedTile* ring_slots = reinterpret_cast<GroupedTile*>(ring_empty + kTileRing + 2 - (3 * STAGES & 1));
+  int* row_of = reinterpret_cast<int*>(ring_slots + kTileRing);
   int* before = row_of + kMaxGemmGroups + 1;
 
   const int warp = threadIdx.x >> 5;
@@ -181,10 +211,15 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 8);
     }
+    for (int i = 0; i < kTileRing; ++i) {
+      mbar_init(&ring_full[i], 1);
+      mbar_init(&ring_empty[i], 5 + (rank == 0 ? 1 : 0) + (MODE == GROUPED_GRAD ? 1 : 0));  // readers of this CTA
+    }
     fence_mbar_init();
     if (a.rows > 0) {  // without rows the operands' maps are not set up, and nothing is loaded
       prefetch_tensormap(&tmL);
       prefetch_tensormap(&tmC);
+      if (!C_MN) prefetch_tensormap(&tmN);
     }
     if (a.tma_out) prefetch_tensormap(&tmD);
   }
@@ -202,8 +237,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   if (warp == 2) grouped_borders<BT>(a, row_of, before, lane);
   __syncthreads();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
-  const GroupedSchedule<MODE, BT> sched{a, row_of, before};
-  const int num_tiles = sched.total();
+  TileRing ring{ring_slots, ring_full, ring_empty, a.status, 0};
+  GroupedTile tile;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -212,10 +247,14 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       const uint32_t leader_full0 = mapa_shared(smem_u32(&full[0]), 0);
-      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
-        const GroupedTile tile = sched.at(t);
-        const int kbs = sched.k_blocks(tile);
-        const int l0 = tile.lane0 + rank * 128, c0 = tile.col0 + rank * (tile.width / 2);
+      while (ok && ring.take(tile)) {
+        ring.leave();
+        const int kbs = tile.k_blocks;
+        const int l0 = tile.lane0 + rank * 128, half = tile.width / 2, c0 = tile.col0 + rank * half;
+        // only the columns that the instruction reads: narrow tiles are bound by these loads
+        const int loads = C_MN ? (half + 63) / 64 : (half + C_BOX - 1) / C_BOX;
+        const bool whole = !C_MN && loads * C_BOX == BT / 2;  // one large box is faster than four small ones
+        const uint32_t bytes = L_BYTES + loads * (C_MN ? BK * 128 : C_BOX * 128);
         for (int kb = 0; kb < kbs; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, a.status, SITEG_PROD_EMPTY)) { ok = false; break; }
           uint8_t* sl = smem + stage * STAGE_BYTES;
@@ -229,20 +268,22 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
               for (int c = 0; c < 2; ++c) load2(sl + c * (BK * 128), &tmL, l0 + c * 64, tile.row0 + kb * BK);
             }
             if constexpr (C_MN) {
-              for (int c = 0; c < BT / 128; ++c) load2(sc + c * (BK * 128), &tmC, c0 + c * 64, tile.row0 + kb * BK);
-            } else {
+              for (int c = 0; c < loads; ++c) load2(sc + c * (BK * 128), &tmC, c0 + c * 64, tile.row0 + kb * BK);
+            } else if (whole) {
               load2(sc, &tmC, kb * BK, c0);
+            } else {
+              for (int c = 0; c < loads; ++c) load2(sc + c * (C_BOX * 128), &tmN, kb * BK, c0 + c * C_BOX);
             }
           };
           const bool cleared = MODE == GROUPED_GRAD && tile.nrows - kb * BK < BK;  // warp 2 passes this block on
           if (rank == 0 || cleared) {
             uint64_t* bar = cleared ? &tail[stage] : &full[stage];
-            mbar_arrive_expect_tx(bar, STAGE_BYTES);
+            mbar_arrive_expect_tx(bar, bytes);
             load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d(d, m, bar, x, y); },
                  [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d(d, m, bar, x, y, z); });
           } else {
             const uint32_t bar = leader_full0 + stage * 8;
-            mbar_arrive_expect_tx_remote(bar, STAGE_BYTES);
+            mbar_arrive_expect_tx_remote(bar, bytes);
             load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d_pair(d, m, bar, x, y); },
                  [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d_pair(d, m, bar, x, y, z); });
           }
@@ -259,9 +300,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       bool ok = true;
       const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
       const uint32_t empty_local = smem_u32(&empty[0]), empty_peer = mapa_shared(empty_local, 1);
-      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
-        const GroupedTile tile = sched.at(t);
-        const int kbs = sched.k_blocks(tile);
+      while (ok && ring.take(tile)) {
+        ring.leave();
+        const int kbs = tile.k_blocks;
         const uint32_t idesc = a.idesc | ((uint32_t)(tile.width >> 3) << 17);
         for (int seg = 0; seg < kbs && ok; seg += PROMOTE ? kPromoteBlocks : kbs, ++lt) {
           const int buf = lt & 1, end = PROMOTE ? min(seg + kPromoteBlocks, kbs) : kbs;
@@ -301,9 +342,11 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     if constexpr (MODE == GROUPED_GRAD) {
       int pos = 0;            // stages used before this tile
       uint32_t phases = 0;    // one bit per stage
-      for (int t = first_tile; t < num_tiles; t += tile_step) {
-        const GroupedTile tile = sched.at(t);
-        const int kbs = sched.k_blocks(tile), valid = tile.nrows - (kbs - 1) * BK;
+      while (__all_sync(~0u, ring.take(tile))) {
+        __syncwarp();
+        if (lane == 0) ring.leave();
+        else ++ring.n;
+        const int kbs = tile.k_blocks, valid = tile.nrows - (kbs - 1) * BK;
         if (kbs > 0 && valid < BK) {
           const int stage = (pos + kbs - 1) % STAGES;
           bool ok = true;
@@ -312,7 +355,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
           if (!ok) break;
           phases ^= 1u << stage;
           uint8_t* sl = smem + stage * STAGE_BYTES;
-          for (int c = 0; c < 2 + BT / 128; ++c)
+          for (int c = 0; c < 2 + (tile.width / 2 + 63) / 64; ++c)
             for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
               *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async_smem();
@@ -322,33 +365,53 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
         pos = (pos + kbs) % STAGES;
       }
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ tile scheduler (each CTA for itself, the same tiles)
+    if (lane == 0) {
+      const GroupedSchedule<MODE, BT> sched{a, row_of, before};
+      const int num_tiles = sched.total();
+      int n = 0;
+      for (int t = first_tile;; t += tile_step, ++n) {
+        if (!mbar_wait(&ring_empty[n % kTileRing], ((n / kTileRing) & 1) ^ 1, a.status, SITEG_RING)) break;
+        GroupedTile r = {};
+        if (t < num_tiles) r = sched.at(t);
+        else r.k_blocks = -1;
+        ring_slots[n % kTileRing] = r;
+        mbar_arrive(&ring_full[n % kTileRing]);
+        if (t >= num_tiles) break;
+      }
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue (warps 4..7, both CTAs)
     const int q = warp & 3;
-    uint8_t* my_buf = epi + (warp - 4) * 2 * EPI_BUF;
-    int nstore = 0, lt = 0;
+    const bool storer = warp == 4 && lane == 0;  // issues the TMA stores of all four warps
+    int buf = 0, lt = 0;
     bool ok = true;
-    for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
-      const GroupedTile tile = sched.at(t);
-      const int kbs = sched.k_blocks(tile);
-      const int m0 = tile.lane0 + rank * 128 + q * 32, m = m0 + lane;
+    while (ok && all_of_128(1, ring.take(tile))) {
+      if (lane == 0) ring.leave();
+      else ++ring.n;
+      const int kbs = tile.k_blocks;
+      const int l0 = tile.lane0 + rank * 128, m = l0 + q * 32 + lane;
       OutT* out = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld + m;
-      // 32 columns from registers to D: by TMA where the whole block belongs to this tile, else element by element
+      // 32 columns from registers to D: by TMA where the whole block belongs to this tile, else element by element.  The
+      // four warps share a staging tile, whose rows are 128 lanes; with three of them one barrier a block is enough: the
+      // thread that issues the stores lets the one before the last drain before it arrives, and that was the next tile's.
       auto store = [&](int c, const uint32_t (&v)[32]) {
         if (a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols)) {
-          OutT* sb = reinterpret_cast<OutT*>(my_buf + (nstore & 1) * EPI_BUF);
-          if (lane == 0) tma_store_wait_read<1>();  // the store that last used `sb` has drained
-          __syncwarp();
+          OutT* sb = reinterpret_cast<OutT*>(epi + buf * EPI_BUF);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sb[j * 32 + lane] = cvt_out<OutT>(__uint_as_float(v[j]) * a.alpha);
+          for (int j = 0; j < 32; ++j) sb[j * 128 + q * 32 + lane] = cvt_out<OutT>(__uint_as_float(v[j]) * a.alpha);
           fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && m0 < a.lanes) {
-            if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, sb, m0, tile.col0 + c, tile.g);
-            else tma_store_2d(&tmD, sb, m0, tile.col0 + c);
+          if (storer) tma_store_wait_read<1>();
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (storer) {
+            if (l0 < a.lanes) {
+              if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, sb, l0, tile.col0 + c, tile.g);
+              else tma_store_2d(&tmD, sb, l0, tile.col0 + c);
+            }
+            tma_store_commit();
           }
-          if (lane == 0) tma_store_commit();
-          ++nstore;
+          buf = buf == kEpiBufs - 1 ? 0 : buf + 1;
         } else if (m < a.lanes) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -362,7 +425,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
         }
       };
       auto arrived = [&]() {  // waits for the accumulator of the next run
-        ok = mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC);
+        // the four warps go on or give up together: they meet again at the barriers of the stores
+        ok = all_of_128(1, mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC));
         tc_fence_after_sync();
         return ok;
       };
@@ -421,7 +485,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
         }
       }
     }
-    if (lane == 0) tma_store_wait_all<0>();
+    if (storer) tma_store_wait_all<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -441,9 +505,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int MODE, typename OutT, int BT>
-static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td, const GroupedArgs& a,
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td, const GroupedArgs& a,
                                long long tiles, cudaStream_t stream) {
-  constexpr int EXTRA = 1024 + 512 + 2 * (kMaxGemmGroups + 1) * 4 + 8 * 32 * 32 * (int)sizeof(OutT);
+  constexpr int EXTRA = 1024 + 1024 + 2 * (kMaxGemmGroups + 1) * 4 + kEpiBufs * 32 * 128 * (int)sizeof(OutT);
   constexpr int STAGE = 128 * 128 + BT / 2 * 128;
   constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE < 12 ? (227 * 1024 - EXTRA) / STAGE : 12;
   constexpr int SMEM = STAGES * STAGE + EXTRA;
@@ -464,29 +528,29 @@ static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CU
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_without_pdl() ? 1 : 2;
-  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, td, a));
+  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, tn, td, a));
   return MOYE_OK;
 }
 
 template <int MODE, typename OutT>
-static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td,
+static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
                              const GroupedArgs& a, long long tiles, cudaStream_t stream) {
   if constexpr (MODE != GROUPED_GRAD) {
-    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, td, a, tiles, stream);
-    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, td, a, tiles, stream);
+    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, td, a, tiles, stream);
+    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, td, a, tiles, stream);
   }
   if constexpr (sizeof(OutT) != 4) {
-    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, td, a, tiles, stream);
+    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
   }
-  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, td, a, tiles, stream);
+  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, td, a, tiles, stream);
 }
 
 template <int MODE>
-static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& td,
+static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
                               const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, td, a, tiles, stream);
-  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, td, a, tiles, stream);
-  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, td, a, tiles, stream);
+  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, td, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
@@ -558,19 +622,20 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.ld = D->stride[0];
   a.status = h->d_status;
   const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
-  if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, td;
+  if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
+  CUtensorMap tl, tc, tn, td;
   std::memset(&td, 0, sizeof(td));
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
                               (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
   if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
+  if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, grouped_box_rows(bt), true)) return rc;
   if (a.tma_out)
-    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 32, 32, false)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 128, 32, false)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype, bt);
-  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, td, a, tiles, stream);
-  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, td, a, tiles, stream);
+  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
@@ -611,8 +676,9 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.group_stride = dB->stride[0];
   a.status = h->d_status;
   const long long tiles = (long long)G * a.lane_tiles * a.col_tiles;
-  if (tiles > INT32_MAX) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, td;
+  if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
+  CUtensorMap tl, tc, tn, td;
+  std::memset(&tn, 0, sizeof(tn));
   std::memset(&tl, 0, sizeof(tl));
   std::memset(&tc, 0, sizeof(tc));
   std::memset(&td, 0, sizeof(td));
@@ -623,11 +689,11 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   if (a.tma_out) {
     const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
     const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
-    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 32, 32, false)) return rc;
+    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 128, 32, false)) return rc;
   }
   log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
            (long long)N, (long long)K, A->dtype, bt);
-  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, td, a, tiles, stream);
+  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 }  // namespace moye

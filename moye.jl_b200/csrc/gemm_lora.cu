@@ -392,7 +392,8 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         store((part * rblocks + (col >> 6)) * (128 * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 4) * 2, w0, w1);
       }
     };
-    bool ok = mbar_wait(v_acc, 0, p.status, SITEL_EPI_V);
+    // the four warps go on or give up together: they meet at barriers
+    bool ok = all_of_128(1, mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
     if (ok) {
       tc_fence_after_sync();
       for (int c = 0; c < rsteps * 16; c += 16) {  // columns behind R are products with zero rows: zero
@@ -421,7 +422,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         lora_epi_sync();
         if (et == 0)
           for (int c = 0; c < C; ++c) mbar_arrive_remote_release(mapa_shared(smem_u32(p_ready), c));
-        ok = mbar_wait_cluster(p_ready, 0, p.status, SITEL_EPI_PARTS);
+        ok = all_of_128(1, mbar_wait_cluster(p_ready, 0, p.status, SITEL_EPI_PARTS));
         if (ok) {
           const int units = rsteps * 4, r0 = 128 * rank / C, r1 = 128 * (rank + 1) / C;
           for (int i = et; i < (r1 - r0) * units; i += 128) {
