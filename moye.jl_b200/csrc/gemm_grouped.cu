@@ -14,9 +14,9 @@
 // last tile of a group simply has fewer columns, and a warp's 32 lanes are 32 neighbouring elements of an output row.
 //
 // Persistent CTA pairs (tcgen05 cta_group::2, see gemm_pair.cu): 256 lanes x up to 256 columns, each CTA holds 128 lanes
-// and half of the column operand.  Per CTA: warp 0 TMA producer, warp 1 tcgen05.mma issuer (leader), warp 2 reads the
-// borders and, in the gradient, clears the rows behind a group's end, warp 3 deals the tiles, warps 4-7 epilogue;
-// accumulators double-buffered.
+// and half of the column operand.  Per CTA: warp 0 TMA producer, warp 1 tcgen05.mma issuer (leader), warp 2
+// clears, in the gradient, the rows behind a group's end, warp 3 reads the borders and deals the tiles, warps 4-11
+// epilogue; accumulators double-buffered.
 //
 // The tensor cores cut the sum after every instruction's 16 products instead of rounding it, always towards zero: for a
 // 16-bit output far below its step, but a Float32 output loses precision in proportion to the length of the sum (1.2e-6
@@ -40,7 +40,7 @@ struct GroupedArgs {
   int cols;             // gradient: extent of the other mode (N)
   int k_blocks;         // forward: blocks of 64 along K
   int lane_tiles, col_tiles;
-  int tma_out;          // D may be written by TMA: 16-byte base and pitches, beta == 0
+  int vec_out;          // D has a 16-byte base and pitches (and, for 16-bit outputs, beta is 0: one rounding)
   const int* offsets;
   uint32_t idesc;       // without N
   float alpha, beta;
@@ -78,97 +78,115 @@ struct TileRing {
   }
 };
 
+// Deals this CTA's tiles to the ring; one warp.  The groups come 32 at a time, a lane each: clamped borders, tiles, and a
+// prefix over the lanes; the group of a tile is then found with one ballot.  Borders outside the arrays or running
+// backwards are a caller's mistake that must not become a bad address: they are clamped, such groups come out empty.
 template <int MODE, int BT>
-struct GroupedSchedule {
-  const GroupedArgs& a;
-  const int* row_of;   // [groups + 1] first rows, clamped to the array and not decreasing
-  const int* before;   // [groups + 1] column tiles of the groups before (forward)
-  __device__ __forceinline__ int total() const {
-    return MODE == GROUPED_GRAD ? a.groups * a.lane_tiles * a.col_tiles : before[a.groups] * a.lane_tiles;
-  }
-  // Tile q of a group's lane_tiles x col_tiles: bands of 8 column tiles, whose operand stays in L2 while the lane tiles pass.
-  __device__ __forceinline__ void place(int q, int col_tiles, int& lt, int& ct) const {
-    const int band = q / (a.lane_tiles * 8), first = band * 8, w = min(8, col_tiles - first);
-    const int r = q - band * a.lane_tiles * 8;
-    ct = first + r % w;
-    lt = r / w;
-  }
-  __device__ __forceinline__ GroupedTile at(int t) const {
-    GroupedTile r;
-    int lt, ct;
-    if (MODE == GROUPED_GRAD) {
-      const int per = a.lane_tiles * a.col_tiles;
-      r.g = t / per;
-      place(t - r.g * per, a.col_tiles, lt, ct);
-      r.col0 = ct * BT;
-      r.row0 = row_of[r.g];
-      r.nrows = row_of[r.g + 1] - r.row0;
-      r.ncols = min(BT, a.cols - r.col0);
-    } else {
-      int lo = 0, hi = a.groups;  // the group whose tiles hold t: before[lo] * lane_tiles <= t < before[lo + 1] * lane_tiles
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (before[mid] * a.lane_tiles <= t) lo = mid;
-        else hi = mid;
+__device__ __forceinline__ void deal_tiles(const GroupedArgs& a, TileRing& ring, int first_tile, int tile_step, int lane) {
+  int next = first_tile, before = 0, last = 0;
+  bool ok = true;
+  auto deal = [&](const GroupedTile& t) {
+    if (lane == 0) {
+      const int slot = ring.n % kTileRing;
+      ok = mbar_wait(&ring.empty[slot], ((ring.n / kTileRing) & 1) ^ 1, a.status, SITEG_RING);
+      if (ok) {
+        ring.slots[slot] = t;
+        mbar_arrive(&ring.full[slot]);
       }
-      r.g = lo;
-      const int tiles = before[lo + 1] - before[lo], count = row_of[lo + 1] - row_of[lo];
-      place(t - before[lo] * a.lane_tiles, tiles, lt, ct);
-      // a few tiles share a group's rows evenly; of many only the last is narrow
-      const int step = tiles <= 4 ? ((count + tiles - 1) / tiles + 31) & ~31 : BT;
-      r.row0 = row_of[lo] + ct * step;
-      r.nrows = min(step, row_of[lo + 1] - r.row0);
-      r.col0 = r.row0;
-      r.ncols = r.nrows;
     }
-    r.lane0 = lt * 256;
-    r.width = (r.ncols + 31) & ~31;
-    r.k_blocks = MODE == GROUPED_GRAD ? (r.nrows + 63) >> 6 : a.k_blocks;
-    return r;
-  }
-};
-
-// First rows and column-tile counts of all groups, by one warp.  Borders outside the arrays or running backwards are a
-// caller's mistake that must not become a bad address: they are clamped, such groups come out empty.
-template <int BT>
-__device__ __forceinline__ void grouped_borders(const GroupedArgs& a, int* row_of, int* before, int lane) {
-  int last = 0, tiles = 0;
-  for (int g0 = 0; g0 <= a.groups; g0 += 32) {
+    ++ring.n;
+    ok = __shfl_sync(~0u, ok, 0);
+  };
+  for (int g0 = 0; g0 < a.groups && ok; g0 += 32) {
     const int g = g0 + lane;
-    int v = g <= a.groups ? min(max(__ldg(a.offsets + g), 0), a.rows) : 0;
+    auto border = [&](int i) { return min(max(__ldg(a.offsets + i), 0), a.rows); };
+    int lo = g < a.groups ? border(g) : 0, hi = g < a.groups ? border(g + 1) : 0;
+    if (lane == 0 && g0 == 0) last = lo;
+    last = __shfl_sync(~0u, last, 0);
+    hi = max(hi, max(lo, last));  // not decreasing: the running maximum
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(~0u, v, d);
-      if (lane >= d) v = max(v, up);
+      const int up = __shfl_up_sync(~0u, hi, d);
+      if (lane >= d) hi = max(hi, up);
     }
-    v = max(v, last);
-    int prev = __shfl_up_sync(~0u, v, 1);
-    if (lane == 0) prev = g0 == 0 ? v : last;
-    // this lane's entry of `before` counts the tiles of the groups up to g - 1
-    int c = g == 0 || g > a.groups ? 0 : (v - prev + BT - 1) / BT;
+    lo = __shfl_up_sync(~0u, hi, 1);
+    if (lane == 0) lo = last;
+    last = __shfl_sync(~0u, hi, 31);
+    const int count = hi - lo;
+    const int col_tiles = MODE == GROUPED_GRAD ? a.col_tiles : (count + BT - 1) / BT;
+    const int mine = g < a.groups ? col_tiles * a.lane_tiles : 0;
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(~0u, c, d);
-      if (lane >= d) c += up;
+      const int up = __shfl_up_sync(~0u, incl, d);
+      if (lane >= d) incl += up;
     }
-    if (g <= a.groups) {
-      row_of[g] = v;
-      before[g] = tiles + c;
+    const int total = __shfl_sync(~0u, incl, 31);
+    while (next < before + total && ok) {
+      const int l = __ffs(__ballot_sync(~0u, before + incl > next)) - 1;
+      const int tiles = __shfl_sync(~0u, col_tiles, l), rows = __shfl_sync(~0u, count, l), start = __shfl_sync(~0u, lo, l);
+      const int q = next - before - __shfl_sync(~0u, incl - mine, l);
+      // bands of 8 column tiles, whose operand stays in L2 while the lane tiles pass
+      const int band = q / (a.lane_tiles * 8), w = min(8, tiles - band * 8), r = q - band * a.lane_tiles * 8;
+      const int ct = band * 8 + r % w;
+      GroupedTile t;
+      t.g = g0 + l;
+      t.lane0 = r / w * 256;
+      if (MODE == GROUPED_GRAD) {
+        t.col0 = ct * BT;
+        t.row0 = start;
+        t.nrows = rows;
+        t.ncols = min(BT, a.cols - t.col0);
+        t.k_blocks = (rows + 63) >> 6;
+      } else {
+        // a few tiles share a group's rows evenly; of many only the last is narrow
+        const int step = tiles <= 4 ? ((rows + tiles - 1) / tiles + 31) & ~31 : BT;
+        t.row0 = start + ct * step;
+        t.nrows = min(step, start + rows - t.row0);
+        t.col0 = t.row0;
+        t.ncols = t.nrows;
+        t.k_blocks = a.k_blocks;
+      }
+      t.width = (t.ncols + 31) & ~31;
+      deal(t);
+      next += tile_step;
     }
-    tiles += __shfl_sync(~0u, c, 31);
-    last = __shfl_sync(~0u, v, 31);
+    before += total;
   }
+  GroupedTile end = {};
+  end.k_blocks = -1;
+  if (ok) deal(end);
 }
 
-constexpr int kEpiBufs = 3;
+// Tensor memory -> registers in the order of matrix fragments: 16 lanes x 32 columns, of which thread T receives, for the
+// columns 8 b + 2 (T % 4) and the next one, lane T / 4 in v[4 b], v[4 b + 1] and lane T / 4 + 8 in v[4 b + 2], v[4 b + 3].
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Four transposed 8 x 8 fragments of 16-bit elements to shared memory; thread T gives the address of row T % 8 of fragment T / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  const T lo = cvt_out<T>(a), hi = cvt_out<T>(b);
+  return (uint32_t)(*reinterpret_cast<const uint16_t*>(&lo)) | ((uint32_t)(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
+}
 __host__ __device__ constexpr int grouped_box_rows(int bt) { return bt / 2 < 32 ? bt / 2 : 32; }
 
 template <int MODE, typename OutT, int BT, int STAGES>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(384, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
-                    const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
+                    const __grid_constant__ CUtensorMap tmN, const GroupedArgs a) {
   // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmN: the same in
-  // boxes of 32 rows for narrow tiles, tmD: the output
+  // boxes of 32 rows for narrow tiles
   constexpr int BK = 64, UMMA_K = 16;
   constexpr int L_BYTES = 128 * 128;
   constexpr int C_BYTES = BT / 2 * 128;  // this CTA's half of the columns
@@ -176,14 +194,15 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   constexpr uint32_t TMEM_COLS = 2 * BT;
   constexpr bool L_MN = MODE != GROUPED_K_MAJOR, C_MN = MODE == GROUPED_GRAD;
   constexpr bool PROMOTE = sizeof(OutT) == 4;
-  constexpr int EPI_BUF = 32 * 128 * (int)sizeof(OutT);  // [32 columns][128 lanes], a staging tile of the four epilogue warps
-  constexpr int C_BOX = grouped_box_rows(BT);            // rows of one load of a K-major column operand
+  constexpr int EPI_BUF = 32 * 128;            // a staging tile: 32 columns of 128 bytes
+  constexpr int EPI_BYTES = 8 * EPI_BUF;       // one per epilogue warp (Float32 outputs) or two per pair of them
+  constexpr int C_BOX = grouped_box_rows(BT);  // rows of one load of a K-major column operand
   static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128) && (!PROMOTE || BT <= 128), "tile columns");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + STAGES * STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + kEpiBufs * EPI_BUF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + EPI_BYTES);
   uint64_t* full = bars;
   uint64_t* empty = bars + STAGES;
   uint64_t* tail = bars + 2 * STAGES;  // gradient: a group's last block has landed, its rows are not cleared yet
@@ -193,8 +212,6 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   uint64_t* ring_empty = ring_full + kTileRing;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ring_empty + kTileRing);
   GroupedTile* ring_slots = reinterpret_cast<GroupedTile*>(ring_empty + kTileRing + 2 - (3 * STAGES & 1));
-  int* row_of = reinterpret_cast<int*>(ring_slots + kTileRing);
-  int* before = row_of + kMaxGemmGroups + 1;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -209,11 +226,11 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
+      mbar_init(&acc_empty[b], 16);
     }
     for (int i = 0; i < kTileRing; ++i) {
       mbar_init(&ring_full[i], 1);
-      mbar_init(&ring_empty[i], 5 + (rank == 0 ? 1 : 0) + (MODE == GROUPED_GRAD ? 1 : 0));  // readers of this CTA
+      mbar_init(&ring_empty[i], 9 + (rank == 0 ? 1 : 0) + (MODE == GROUPED_GRAD ? 1 : 0));  // readers of this CTA
     }
     fence_mbar_init();
     if (a.rows > 0) {  // without rows the operands' maps are not set up, and nothing is loaded
@@ -221,7 +238,6 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       prefetch_tensormap(&tmC);
       if (!C_MN) prefetch_tensormap(&tmN);
     }
-    if (a.tma_out) prefetch_tensormap(&tmD);
   }
   if (warp == 1) {
     tmem_alloc2(tmem_holder, TMEM_COLS);
@@ -234,8 +250,6 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   tc_fence_after_sync();
   griddep_launch();  // programmatic dependent launch, after the tensor-memory allocation; nothing above touches global memory
   griddep_wait();
-  if (warp == 2) grouped_borders<BT>(a, row_of, before, lane);
-  __syncthreads();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
   TileRing ring{ring_slots, ring_full, ring_empty, a.status, 0};
   GroupedTile tile;
@@ -367,56 +381,27 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------ tile scheduler (each CTA for itself, the same tiles)
-    if (lane == 0) {
-      const GroupedSchedule<MODE, BT> sched{a, row_of, before};
-      const int num_tiles = sched.total();
-      int n = 0;
-      for (int t = first_tile;; t += tile_step, ++n) {
-        if (!mbar_wait(&ring_empty[n % kTileRing], ((n / kTileRing) & 1) ^ 1, a.status, SITEG_RING)) break;
-        GroupedTile r = {};
-        if (t < num_tiles) r = sched.at(t);
-        else r.k_blocks = -1;
-        ring_slots[n % kTileRing] = r;
-        mbar_arrive(&ring_full[n % kTileRing]);
-        if (t >= num_tiles) break;
-      }
-    }
+    deal_tiles<MODE, BT>(a, ring, first_tile, tile_step, lane);
   } else if (warp >= 4) {
-    // ------------------------------------------------------------ epilogue (warps 4..7, both CTAs)
+    // ------------------------------------------------------------ epilogue (warps 4..11, both CTAs)
+    // Four warps read the tensor memory's four quarters of 32 lanes; two such sets share the blocks of 32 columns.
     const int q = warp & 3;
-    const bool storer = warp == 4 && lane == 0;  // issues the TMA stores of all four warps
+    const int set = (warp - 4) >> 2;
+    uint8_t* my_epi = epi + (PROMOTE ? warp - 4 : (warp - 4) >> 1 << 1) * EPI_BUF;
     int buf = 0, lt = 0;
     bool ok = true;
-    while (ok && all_of_128(1, ring.take(tile))) {
+    while (ok && all_of_128(1 + set, ring.take(tile))) {
       if (lane == 0) ring.leave();
       else ++ring.n;
       const int kbs = tile.k_blocks;
       const int l0 = tile.lane0 + rank * 128, m = l0 + q * 32 + lane;
-      OutT* out = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld + m;
-      // 32 columns from registers to D: by TMA where the whole block belongs to this tile, else element by element.  The
-      // four warps share a staging tile, whose rows are 128 lanes; with three of them one barrier a block is enough: the
-      // thread that issues the stores lets the one before the last drain before it arrives, and that was the next tile's.
-      auto store = [&](int c, const uint32_t (&v)[32]) {
-        if (a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols)) {
-          OutT* sb = reinterpret_cast<OutT*>(epi + buf * EPI_BUF);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sb[j * 128 + q * 32 + lane] = cvt_out<OutT>(__uint_as_float(v[j]) * a.alpha);
-          fence_proxy_async_smem();
-          if (storer) tma_store_wait_read<1>();
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (storer) {
-            if (l0 < a.lanes) {
-              if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, sb, l0, tile.col0 + c, tile.g);
-              else tma_store_2d(&tmD, sb, l0, tile.col0 + c);
-            }
-            tma_store_commit();
-          }
-          buf = buf == kEpiBufs - 1 ? 0 : buf + 1;
-        } else if (m < a.lanes) {
+      OutT* row0 = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld;
+      auto store_elements = [&](int c, const uint32_t (&v)[32]) {
+        if (m < a.lanes) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             if (c + j < tile.ncols) {
-              OutT* p = out + (c + j) * a.ld;
+              OutT* p = row0 + (c + j) * a.ld + m;
               float x = __uint_as_float(v[j]) * a.alpha;
               if (a.beta != 0.f) x += a.beta * load_c_as_float<OutT>(p, 0);
               *p = cvt_out<OutT>(x);
@@ -425,8 +410,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
         }
       };
       auto arrived = [&]() {  // waits for the accumulator of the next run
-        // the four warps go on or give up together: they meet again at the barriers of the stores
-        ok = all_of_128(1, mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC));
+        // the four warps of a set go on or give up together: they meet again at the barriers of the stores
+        ok = all_of_128(1 + set, mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC));
         tc_fence_after_sync();
         return ok;
       };
@@ -441,51 +426,147 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       };
       const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
       if constexpr (PROMOTE) {
-        float acc[BT];
+        constexpr int MINE = (BT + 63) / 64;  // this set's blocks of 32 columns, from 64 i + 32 set on
+        float acc[MINE * 32];
 #pragma unroll
-        for (int j = 0; j < BT; ++j) acc[j] = 0.f;
+        for (int j = 0; j < MINE * 32; ++j) acc[j] = 0.f;
         for (int seg = 0; seg < kbs; seg += kPromoteBlocks) {
           if (!arrived()) break;
 #pragma unroll
-          for (int c = 0; c < BT; c += 32) {
+          for (int i = 0; i < MINE; ++i) {
+            const int c = i * 64 + set * 32;
             if (c < tile.width) {
               uint32_t v[32];
               tmem_ld_x32(t_lane + (lt & 1) * BT + c, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(v[j]);
+              for (int j = 0; j < 32; ++j) acc[i * 32 + j] += __uint_as_float(v[j]);
             }
           }
           release();
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < BT; c += 32) {
+        for (int i = 0; i < MINE; ++i) {
+          const int c = i * 64 + set * 32;
           if (c < tile.width) {
             uint32_t v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[c + j]);
-            store(c, v);
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[i * 32 + j]);
+            if (a.vec_out) {
+              // [32 columns][32 lanes] per warp, stored as rows of 128 bytes
+              float* sb = reinterpret_cast<float*>(my_epi);
+              __syncwarp();  // the last block's rows have been read
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sb[j * 32 + lane] = __uint_as_float(v[j]) * a.alpha;
+              __syncwarp();
+              const int x = l0 + q * 32 + (lane & 7) * 4;
+              float4 w[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const float4*>(sb + (k * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
+              float* p = reinterpret_cast<float*>(row0) + (c + (lane >> 3)) * a.ld + x;
+              const int live = x < a.lanes ? tile.ncols - c - (lane >> 3) : 0;  // rows k * 4 < live are stored
+              if (x + 4 <= a.lanes) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  if (k * 4 < live) {
+                    float4* to = reinterpret_cast<float4*>(p + k * 4 * a.ld);
+                    if (a.beta != 0.f) {
+                      const float4 old = *to;
+                      w[k] = make_float4(w[k].x + a.beta * old.x, w[k].y + a.beta * old.y, w[k].z + a.beta * old.z, w[k].w + a.beta * old.w);
+                    }
+                    *to = w[k];
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  if (k * 4 < live) {
+                    const float e[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                    float* to = p + k * 4 * a.ld;
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                      if (x + i < a.lanes) to[i] = a.beta != 0.f ? e[i] + a.beta * to[i] : e[i];
+                  }
+                }
+              }
+            } else {
+              store_elements(c, v);
+            }
           }
         }
       } else {
         if (kbs > 0 && !arrived()) break;
+        const int t_buf = (lt & 1) * BT;
+        const int blocks = tile.width / 32, last = (blocks - 1 - set) / 2 * 2 + set;  // this set's last block (below 0: none)
+        if (kbs > 0 && blocks <= set) release();
 #pragma unroll 1
-        for (int c = 0; c < tile.width; c += 32) {
-          uint32_t v[32];
-          if (kbs > 0) {
-            tmem_ld_x32(t_lane + (lt & 1) * BT + c, v);
-            tmem_ld_wait();
-          } else {
+        for (int blk = set; blk < blocks; blk += 2) {
+          const int c = blk * 32;
+          const uint32_t at = t_lane + t_buf + c;
+          if (a.vec_out) {
+            // Two warps share a staging tile [32 columns][128 bytes of 64 lanes], its 16-byte units swizzled by the column, and
+            // store it as rows of 128 bytes; of two tiles one is free again when its readers have come to the next barrier.
+            // Whole 8 x 8 fragments are staged transposed: single 16-bit elements would take twice the shared-memory cycles,
+            // which the tensor cores need for their operands.  Stores by TMA from such tiles took 14 cycles per 128 bytes
+            // (64 gradients of 2048 x 2048 of empty groups: 212 us).
+            const uint32_t sb = smem_u32(my_epi + buf * EPI_BUF);
+            {
+              uint32_t v[2][16];
+              if (kbs > 0) {
+                tmem_ld_16x32(at, v[0]);
+                tmem_ld_16x32(at + (16u << 16), v[1]);
+                tmem_ld_wait();
+                if (blk == last) release();
+              } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0u;
+                for (int j = 0; j < 16; ++j) v[0][j] = v[1][j] = 0u;
+              }
+              const int row = lane & 7, unit = (q & 1) * 4 + (lane >> 3);  // this thread's row and fragment of every group of four
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                uint32_t f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  f[i] = pack_pair<OutT>(__uint_as_float(v[i >> 1][4 * b + 2 * (i & 1)]) * a.alpha,
+                                         __uint_as_float(v[i >> 1][4 * b + 2 * (i & 1) + 1]) * a.alpha);
+                stmatrix_x4_trans(sb + (b * 8 + row) * 128 + ((unit ^ row) << 4), f[0], f[1], f[2], f[3]);
+              }
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(3 + ((warp - 4) >> 1)) : "memory");  // barriers 3..6
+            const int x = l0 + (q >> 1) * 64 + (lane & 7) * 8, j0 = (q & 1) * 16 + (lane >> 3);
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = *reinterpret_cast<const uint4*>(my_epi + buf * EPI_BUF + (j0 + i * 4) * 128 + (((lane & 7) ^ ((j0 + i * 4) & 7)) << 4));
+            OutT* p = row0 + (c + j0) * a.ld + x;
+            const int live = x < a.lanes ? tile.ncols - c - j0 : 0;  // rows i * 4 < live are stored
+            if (x + 8 <= a.lanes) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (i * 4 < live) *reinterpret_cast<uint4*>(p + i * 4 * a.ld) = w[i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (i * 4 < live)
+                  for (int k = 0; x + k < a.lanes; ++k) p[i * 4 * a.ld + k] = reinterpret_cast<const OutT*>(&w[i])[k];
+            }
+            buf ^= 1;
+          } else {
+            uint32_t v[32];
+            if (kbs > 0) {
+              tmem_ld_x32(at, v);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0u;
+            }
+            if (kbs > 0 && blk == last) release();
+            store_elements(c, v);
           }
-          if (kbs > 0 && c + 32 >= tile.width) release();
-          store(c, v);
         }
       }
     }
-    if (storer) tma_store_wait_all<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -505,9 +586,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int MODE, typename OutT, int BT>
-static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td, const GroupedArgs& a,
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const GroupedArgs& a,
                                long long tiles, cudaStream_t stream) {
-  constexpr int EXTRA = 1024 + 1024 + 2 * (kMaxGemmGroups + 1) * 4 + kEpiBufs * 32 * 128 * (int)sizeof(OutT);
+  constexpr int EXTRA = 1024 + 1024 + 8 * 32 * 128;
   constexpr int STAGE = 128 * 128 + BT / 2 * 128;
   constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE < 12 ? (227 * 1024 - EXTRA) / STAGE : 12;
   constexpr int SMEM = STAGES * STAGE + EXTRA;
@@ -516,7 +597,7 @@ static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CU
   const long long pairs = tiles < h->num_sms / 2 ? tiles : h->num_sms / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -528,29 +609,29 @@ static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CU
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_without_pdl() ? 1 : 2;
-  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, tn, td, a));
+  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, tn, a));
   return MOYE_OK;
 }
 
 template <int MODE, typename OutT>
-static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
+static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn,
                              const GroupedArgs& a, long long tiles, cudaStream_t stream) {
   if constexpr (MODE != GROUPED_GRAD) {
-    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, td, a, tiles, stream);
-    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, td, a, tiles, stream);
+    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, a, tiles, stream);
+    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, a, tiles, stream);
   }
   if constexpr (sizeof(OutT) != 4) {
-    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
+    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, a, tiles, stream);
   }
-  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, a, tiles, stream);
 }
 
 template <int MODE>
-static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
+static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn,
                               const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, td, a, tiles, stream);
-  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, td, a, tiles, stream);
-  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, td, a, tiles, stream);
+  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, a, tiles, stream);
+  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, a, tiles, stream);
 }
 
 static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
@@ -612,7 +693,7 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.lanes = (int)N;
   a.k_blocks = (int)((K + 63) / 64);
   a.lane_tiles = (int)((N + 255) / 256);
-  a.tma_out = beta == 0.f && (reinterpret_cast<uintptr_t>(D->ptr) & 15) == 0 && (R == 1 || (D->stride[0] * ob) % 16 == 0);
+  a.vec_out = (beta == 0.f || ob == 4) && (reinterpret_cast<uintptr_t>(D->ptr) & 15) == 0 && (R == 1 || (D->stride[0] * ob) % 16 == 0);
   a.offsets = offsets;
   const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
   a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((mn ? 1u : 0u) << 15) | (16u << 24);
@@ -623,19 +704,16 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.status = h->d_status;
   const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, tn, td;
-  std::memset(&td, 0, sizeof(td));
+  CUtensorMap tl, tc, tn;
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
                               (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
   if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
   if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, grouped_box_rows(bt), true)) return rc;
-  if (a.tma_out)
-    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 128, 32, false)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype, bt);
-  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
-  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, a, tiles, stream);
+  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, a, tiles, stream);
 }
 
 int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
@@ -664,7 +742,7 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.cols = (int)N;
   a.lane_tiles = (int)((K + 255) / 256);
   a.col_tiles = (int)((N + bt - 1) / bt);
-  a.tma_out = beta == 0.f && (reinterpret_cast<uintptr_t>(dB->ptr) & 15) == 0 && (N == 1 || (dB->stride[1] * ob) % 16 == 0) &&
+  a.vec_out = (beta == 0.f || ob == 4) && (reinterpret_cast<uintptr_t>(dB->ptr) & 15) == 0 && (N == 1 || (dB->stride[1] * ob) % 16 == 0) &&
               (G == 1 || (dB->stride[0] * ob) % 16 == 0);
   a.offsets = offsets;
   const uint32_t fmt = A->dtype == MOYE_BF16 ? 1u : 0u;
@@ -677,23 +755,17 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.status = h->d_status;
   const long long tiles = (long long)G * a.lane_tiles * a.col_tiles;
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, tn, td;
+  CUtensorMap tl, tc, tn;
   std::memset(&tn, 0, sizeof(tn));
   std::memset(&tl, 0, sizeof(tl));
   std::memset(&tc, 0, sizeof(tc));
-  std::memset(&td, 0, sizeof(td));
   if (R > 0) {  // without rows the kernel loads nothing, every group's sum is empty
     if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
     if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
   }
-  if (a.tma_out) {
-    const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
-    const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
-    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 128, 32, false)) return rc;
-  }
   log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
            (long long)N, (long long)K, A->dtype, bt);
-  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, a, tiles, stream);
 }
 
 }  // namespace moye
