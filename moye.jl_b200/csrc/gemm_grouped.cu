@@ -40,6 +40,7 @@ struct GroupedArgs {
   int cols;             // gradient: extent of the other mode (N)
   int k_blocks;         // forward: blocks of 64 along K
   int lane_tiles, col_tiles;
+  int tma_out;          // a 16-bit D that vectors and TMA may write
   int vec_out;          // D has a 16-byte base and pitches (and, for 16-bit outputs, beta is 0: one rounding)
   const int* offsets;
   uint32_t idesc;       // without N
@@ -184,9 +185,9 @@ __host__ __device__ constexpr int grouped_box_rows(int bt) { return bt / 2 < 32 
 template <int MODE, typename OutT, int BT, int STAGES>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
-                    const __grid_constant__ CUtensorMap tmN, const GroupedArgs a) {
+                    const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
   // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmN: the same in
-  // boxes of 32 rows for narrow tiles
+  // boxes of 32 rows for narrow tiles, tmD: a 16-bit output
   constexpr int BK = 64, UMMA_K = 16;
   constexpr int L_BYTES = 128 * 128;
   constexpr int C_BYTES = BT / 2 * 128;  // this CTA's half of the columns
@@ -238,6 +239,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       prefetch_tensormap(&tmC);
       if (!C_MN) prefetch_tensormap(&tmN);
     }
+    if (a.tma_out) prefetch_tensormap(&tmD);
   }
   if (warp == 1) {
     tmem_alloc2(tmem_holder, TMEM_COLS);
@@ -505,11 +507,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
           const int c = blk * 32;
           const uint32_t at = t_lane + t_buf + c;
           if (a.vec_out) {
-            // Two warps share a staging tile [32 columns][128 bytes of 64 lanes], its 16-byte units swizzled by the column, and
-            // store it as rows of 128 bytes; of two tiles one is free again when its readers have come to the next barrier.
-            // Whole 8 x 8 fragments are staged transposed: single 16-bit elements would take twice the shared-memory cycles,
-            // which the tensor cores need for their operands.  Stores by TMA from such tiles took 14 cycles per 128 bytes
-            // (64 gradients of 2048 x 2048 of empty groups: 212 us).
+            // Two warps share a staging tile [32 columns][128 bytes of 64 lanes] in the 128-byte swizzle; of two tiles one is
+            // free again when its readers have come to the next barrier.  Whole 8 x 8 fragments are staged transposed: single
+            // 16-bit elements would take twice the shared-memory cycles, which the tensor cores need for their operands.
             const uint32_t sb = smem_u32(my_epi + buf * EPI_BUF);
             {
               uint32_t v[2][16];
@@ -533,7 +533,23 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
                 stmatrix_x4_trans(sb + (b * 8 + row) * 128 + ((unit ^ row) << 4), f[0], f[1], f[2], f[3]);
               }
             }
+            // A block that belongs to this tile as a whole goes out by TMA, the last rows of a group by vector stores.  The
+            // thread that issues a pair's TMA stores lets the one before drain first: it read the tile that comes next.
+            const bool whole = a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols);
+            const bool storer = (q & 1) == 0 && lane == 0;
+            fence_proxy_async_smem();
+            if (storer) tma_store_wait_read<0>();
             asm volatile("bar.sync %0, 64;" ::"r"(3 + ((warp - 4) >> 1)) : "memory");  // barriers 3..6
+            if (whole) {
+              const int x = l0 + (q >> 1) * 64;
+              if (storer && x < a.lanes) {
+                if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, my_epi + buf * EPI_BUF, x, tile.col0 + c, tile.g);
+                else tma_store_2d(&tmD, my_epi + buf * EPI_BUF, x, tile.col0 + c);
+                tma_store_commit();
+              }
+              buf ^= 1;
+              continue;
+            }
             const int x = l0 + (q >> 1) * 64 + (lane & 7) * 8, j0 = (q & 1) * 16 + (lane >> 3);
             uint4 w[4];
 #pragma unroll
@@ -569,6 +585,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     }
   }
 
+  if (!PROMOTE && warp >= 4) tma_store_wait_all<0>();
+
   // ---------------------------------------------------------------- teardown
   if (*reinterpret_cast<volatile int*>(a.status) != 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);  // a wait gave up: copies in flight get time to land
@@ -586,7 +604,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int MODE, typename OutT, int BT>
-static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const GroupedArgs& a,
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td, const GroupedArgs& a,
                                long long tiles, cudaStream_t stream) {
   constexpr int EXTRA = 1024 + 1024 + 8 * 32 * 128;
   constexpr int STAGE = 128 * 128 + BT / 2 * 128;
@@ -609,29 +627,29 @@ static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CU
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_without_pdl() ? 1 : 2;
-  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, tn, a));
+  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tl, tc, tn, td, a));
   return MOYE_OK;
 }
 
 template <int MODE, typename OutT>
-static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn,
+static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
                              const GroupedArgs& a, long long tiles, cudaStream_t stream) {
   if constexpr (MODE != GROUPED_GRAD) {
-    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, a, tiles, stream);
-    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, a, tiles, stream);
+    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, td, a, tiles, stream);
+    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, td, a, tiles, stream);
   }
   if constexpr (sizeof(OutT) != 4) {
-    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, a, tiles, stream);
+    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
   }
-  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, a, tiles, stream);
+  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, td, a, tiles, stream);
 }
 
 template <int MODE>
-static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn,
+static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
                               const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, a, tiles, stream);
-  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, a, tiles, stream);
-  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, a, tiles, stream);
+  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, td, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
@@ -704,16 +722,20 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.status = h->d_status;
   const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, tn;
+  CUtensorMap tl, tc, tn, td;
+  std::memset(&td, 0, sizeof(td));
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
                               (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
   if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
   if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, grouped_box_rows(bt), true)) return rc;
+  a.tma_out = a.vec_out && ob == 2;
+  if (a.tma_out)
+    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 64, 32, true)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype, bt);
-  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, a, tiles, stream);
-  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, a, tiles, stream);
+  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
@@ -755,7 +777,8 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.status = h->d_status;
   const long long tiles = (long long)G * a.lane_tiles * a.col_tiles;
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
-  CUtensorMap tl, tc, tn;
+  CUtensorMap tl, tc, tn, td;
+  std::memset(&td, 0, sizeof(td));
   std::memset(&tn, 0, sizeof(tn));
   std::memset(&tl, 0, sizeof(tl));
   std::memset(&tc, 0, sizeof(tc));
@@ -763,9 +786,15 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
     if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
     if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
   }
+  a.tma_out = a.vec_out && ob == 2;
+  if (a.tma_out) {
+    const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
+    const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
+    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 64, 32, true)) return rc;
+  }
   log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
            (long long)N, (long long)K, A->dtype, bt);
-  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, a, tiles, stream);
+  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 }  // namespace moye
