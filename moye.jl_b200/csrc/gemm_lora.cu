@@ -128,26 +128,31 @@ lora_row_kernel(const LoraArgs g) {
   cluster_wait();
 }
 
-// ---------------------------------------------------------------------------------------------- long requests
+// ---------------------------------------------------------------------------------------------- requests of several rows
 // A cluster of C CTAs takes up to 128 rows of one request.  CTA c multiplies its K blocks of X (128 lanes of tensor
-// memory) with A[a] (R columns); with C > 1 the fp32 parts meet through distributed shared memory, CTA c summing 128 / C
-// rows in CTA order and handing the result to all; every CTA then multiplies it with its 128-column chunks of B[a] and
+// memory) with A[a] (R columns); with C > 1 the fp32 parts meet through distributed shared memory, CTA c summing 1 / C of
+// the rows in CTA order and handing the result to all; every CTA then multiplies it with its 128-column chunks of B[a] and
 // adds C.  The product of rank R enters the second multiplication as a sum of 16-bit parts: two parts carry 16 (bf16)
 // or 22 (f16) bits, a sixteenth of an output step or less; bf16 operands with a Float32 output take three (24 bits).
 //
-// Warp 0 producer, warp 1 MMA issuer, warps 2-5 move the parts and run the epilogue.  The producer's ring carries first
-// the K blocks, then the chunks of B, which therefore arrive while the parts meet.  The output is bound by memory: the
-// accumulator crosses shared memory so that a warp reads C and writes D in 16-byte accesses of whole sectors, and the
-// next 4 KB of C per warp are on their way while these are added.
-// Two CTAs fit on an SM (256 tensor-memory columns each, at most 113 KB); three never do, their shared memory is too large.
-constexpr int kLoraTileThreads = 192;
-enum : int { SITEL_PROD_EMPTY = 171, SITEL_MMA_FULL = 172, SITEL_MMA_V = 173, SITEL_MMA_ACC = 174, SITEL_EPI_V = 175, SITEL_EPI_PARTS = 176, SITEL_EPI_ACC = 177, SITEL_SMEM_BASE = 178 };
+// Warp 0 producer, warp 1 MMA issuer, warps 4-11 move the parts and run the epilogue.  The kernel is bound by memory (X and
+// C in, D out) and lives on bytes in flight.  The first product has all of shared memory for its ring of K blocks (9 at
+// rank 64; with 4 it took 34 us of 16384 rows x 4096); the second has it for chunks of B, the rank-R product and boxes of C:
+// the epilogue keeps one to five boxes of 4 KB ahead per warp, a thread holds one row of the accumulator and adds it to the same
+// row of the box, which goes out by TMA again.  (C through registers and D by vector stores, on two CTAs per SM: 16384 rows
+// of 24 requests, rank 64, 4096 x 4096: 115 us.)
+//
+// Tiles of at most 32 rows turn the second product round: the lanes are the columns of D and the rows its columns, so
+// that all warps have work and nothing crosses shared memory.
+constexpr int kLoraTileThreads = 384;
+enum : int { SITEL_PROD_EMPTY = 171, SITEL_MMA_FULL = 172, SITEL_MMA_V = 173, SITEL_MMA_ACC = 174, SITEL_EPI_V = 175, SITEL_EPI_PARTS = 176, SITEL_EPI_ACC = 177, SITEL_SMEM_BASE = 178, SITEL_EPI_C = 179 };
 
 struct LoraTileArgs {
   LoraArgs g;
   uint32_t idesc1, idesc2;
   int* status;
-  int stages, stage_bytes, v_off, stage_out_off, bar_off;  // shared-memory plan, bytes
+  int k_stages, k_bytes;                                    // first product: ring of K blocks from offset 0
+  int b_stages, b_bytes, v_off, c_off, c_bufs, bar_off;     // second: ring of chunks from 0, then the rest; bytes
 };
 
 __device__ __forceinline__ float4 ld_remote_f32x4(uint32_t cluster_addr) {
@@ -158,16 +163,38 @@ __device__ __forceinline__ float4 ld_remote_f32x4(uint32_t cluster_addr) {
 __device__ __forceinline__ void st_remote_u32x2(uint32_t cluster_addr, uint32_t x, uint32_t y) {
   asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(cluster_addr), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void lora_epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The epilogue's 256 threads meet, all going on or giving up together.
+__device__ __forceinline__ bool lora_epi_all(bool mine) {
+  int r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.s32 q, %1, 0;\nbar.red.and.pred p, 1, 256, q;\nselp.s32 %0, 1, 0, p;\n}\n"
+      : "=r"(r)
+      : "r"((int)mine)
+      : "memory");
+  return r != 0;
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t lora_pack2(float a, float b) {
   const T lo = cvt_out<T>(a), hi = cvt_out<T>(b);
   return (uint32_t)(*reinterpret_cast<const uint16_t*>(&lo)) | ((uint32_t)(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
 }
+// One 16-byte word of outputs: the input word plus EPV accumulators.
+__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float*) {
+  return make_uint4(__float_as_uint(__uint_as_float(c.x) + __uint_as_float(v[0])), __float_as_uint(__uint_as_float(c.y) + __uint_as_float(v[1])),
+                    __float_as_uint(__uint_as_float(c.z) + __uint_as_float(v[2])), __float_as_uint(__uint_as_float(c.w) + __uint_as_float(v[3])));
+}
+template <typename T>
+__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, T*) {
+  float f[8];
+  lora_unpack<T>(c, f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] += __uint_as_float(v[e]);
+  return make_uint4(lora_pack2<T>(f[0], f[1]), lora_pack2<T>(f[2], f[3]), lora_pack2<T>(f[4], f[5]), lora_pack2<T>(f[6], f[7]));
+}
 
 // The request and first row of tile `want`; q = -1 when there are fewer tiles.  All threads of the CTA; `sums` holds one
-// int per thread.
+// int per warp.
 __device__ __forceinline__ void lora_find_tile(const LoraArgs& g, int want, int* sums, int* result) {
   const int tid = threadIdx.x, per = (g.requests + kLoraTileThreads - 1) / kLoraTileThreads;
   const int q0 = min(tid * per, g.requests), q1 = min(q0 + per, g.requests);
@@ -205,32 +232,31 @@ __device__ __forceinline__ void lora_find_tile(const LoraArgs& g, int want, int*
 }
 
 template <typename T, typename OutT, bool VEC, int PARTS>
-__global__ void __launch_bounds__(kLoraTileThreads, 2)
-lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
-                 const __grid_constant__ CUtensorMap tmB, const LoraTileArgs p) {
+__global__ void __launch_bounds__(kLoraTileThreads, 1)
+lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD, const LoraTileArgs p) {
   const LoraArgs& g = p.g;
-  // No slack for aligning the base by hand: two CTAs at rank 64 leave 700 bytes of an SM's shared memory.
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = smem_raw;
-  if ((smem_u32(smem) & 1023u) != 0) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {  // the plan has no slack to align the base by hand
     if (threadIdx.x == 0) atomicCAS(p.status, 0, SITEL_SMEM_BASE);
     return;
   }
-  uint8_t* vparts = smem + p.v_off;                                // [part][64-wide block of R][128 rows][128 bytes], swizzled
-  float* parts = reinterpret_cast<float*>(smem + p.stage_out_off);  // [128][R] fp32; later the epilogue's staging
+  uint8_t* vparts = smem + p.v_off;                          // [part][64-wide block of R][128 rows][128 bytes], swizzled
+  uint8_t* cboxes = smem + p.c_off;                          // [8 warps][c_bufs][32 rows][128 bytes], swizzled
+  float* parts = reinterpret_cast<float*>(cboxes);           // before that (C > 1): [128][R] fp32
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bar_off);
-  uint64_t *full = bars, *empty = bars + 8, *acc_full = bars + 16, *acc_empty = bars + 18, *v_acc = bars + 20, *p_ready = bars + 21,
-           *v_ready = bars + 22;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 23);
-  int* scratch = reinterpret_cast<int*>(bars + 24);  // 8 warp sums, then the tile
+  uint64_t *k_full = bars, *k_empty = bars + 12, *b_full = bars + 24, *b_empty = bars + 28, *acc_full = bars + 32, *acc_empty = bars + 34,
+           *v_acc = bars + 36, *p_ready = bars + 37, *v_ready = bars + 38, *c_full = bars + 40;  // c_full[8 warps][c_bufs <= 6]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 39);
+  int* scratch = reinterpret_cast<int*>(bars + 88);          // 12 warp sums, then the tile
   constexpr uint32_t TMEM_COLS = 256;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
   griddep_wait();
-  lora_find_tile(g, blockIdx.x / C, scratch, scratch + 8);
-  const int q = scratch[8], row0 = scratch[9], nrows = scratch[10];
-  if (q < 0) return;  // fewer tiles than CTAs; the same in the whole cluster
+  lora_find_tile(g, blockIdx.x / C, scratch, scratch + 12);
+  const int q = scratch[12], row0 = scratch[13], nrows = scratch[14];
+  if (q < 0) return;  // fewer tiles than clusters; the same in the whole cluster
   const int a = g.which[q];
   const int chunks = (g.n + 127) / 128, kbs = (g.k + 63) / 64;
   const int ch0 = chunks * rank / C, ch1 = chunks * (rank + 1) / C;
@@ -264,19 +290,25 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   const int kb0 = kbs * rank / C, kb1 = kbs * (rank + 1) / C;  // at least one block: C <= kbs
   const int rblocks = (g.rank + 63) / 64, rsteps = (g.rank + 15) / 16;
   const int a_bytes = rsteps * 16 * 128;
+  const bool turned = nrows <= 32;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+    for (int s = 0; s < p.k_stages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < p.b_stages; ++s) {
+      mbar_init(&b_full[s], 1);
+      mbar_init(&b_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], turned ? 4 : 8);
     }
     mbar_init(v_acc, 1);
     mbar_init(p_ready, C);
     mbar_init(v_ready, C);
+    for (int i = 0; i < 8 * p.c_bufs; ++i) mbar_init(&c_full[i], 1);
     fence_mbar_init();
     prefetch_tensormap(&tmX);
     prefetch_tensormap(&tmA);
@@ -303,20 +335,27 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int i = 0; i < (kb1 - kb0) + (ch1 - ch0); ++i) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, p.status, SITEL_PROD_EMPTY)) break;
-        uint8_t* s = smem + stage * p.stage_bytes;
-        if (i < kb1 - kb0) {
-          const int k = (kb0 + i) * 64;
-          mbar_arrive_expect_tx(&full[stage], 128 * 128 + a_bytes);
-          tma_load_2d(s, &tmX, &full[stage], k, row0);
-          tma_load_3d(s + 128 * 128, &tmA, &full[stage], k, 0, a);
-        } else {
-          const int n = (ch0 + i - (kb1 - kb0)) * 128;
-          mbar_arrive_expect_tx(&full[stage], rblocks * 128 * 128);
-          for (int b = 0; b < rblocks; ++b) tma_load_3d(s + b * 128 * 128, &tmB, &full[stage], b * 64, n, a);
-        }
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      bool ok = true;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        ok = mbar_wait(&k_empty[stage], phase ^ 1, p.status, SITEL_PROD_EMPTY);
+        if (!ok) break;
+        uint8_t* s = smem + stage * p.k_bytes;
+        mbar_arrive_expect_tx(&k_full[stage], 128 * 128 + a_bytes);
+        tma_load_2d(s, &tmX, &k_full[stage], kb * 64, row0);
+        tma_load_3d(s + 128 * 128, &tmA, &k_full[stage], kb * 64, 0, a);
+        if (++stage == p.k_stages) { stage = 0; phase ^= 1; }
+      }
+      // the chunks lie where the K blocks did
+      ok = ok && mbar_wait(v_acc, 0, p.status, SITEL_PROD_EMPTY);
+      stage = 0;
+      phase = 0;
+      for (int ch = ch0; ch < ch1 && ok; ++ch) {
+        ok = mbar_wait(&b_empty[stage], phase ^ 1, p.status, SITEL_PROD_EMPTY);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&b_full[stage], p.b_bytes);
+        for (int b = 0; b < rblocks; ++b)
+          tma_load_3d(smem + stage * p.b_bytes + b * 128 * 128, &tmB, &b_full[stage], b * 64, ch * 128, a);
+        if (++stage == p.b_stages) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -326,61 +365,58 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       uint32_t phase = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(&full[stage], phase, p.status, SITEL_MMA_FULL);
+        ok = mbar_wait(&k_full[stage], phase, p.status, SITEL_MMA_FULL);
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t s = smem_u32(smem + stage * p.stage_bytes);
+        const uint32_t s = smem_u32(smem + stage * p.k_bytes);
         const uint64_t xd = umma_desc_k_sw128(s), ad = umma_desc_k_sw128(s + 128 * 128);
 #pragma unroll
         for (int k = 0; k < 4; ++k) tc_mma_ss<KIND_F16>(tmem_base, xd + 2 * k, ad + 2 * k, p.idesc1, (kb > kb0 || k > 0) ? 1u : 0u);
-        tc_commit(&empty[stage]);
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        tc_commit(&k_empty[stage]);
+        if (++stage == p.k_stages) { stage = 0; phase ^= 1; }
       }
       if (ok) tc_commit(v_acc);
+      stage = 0;
+      phase = 0;
       if (ok && ch1 > ch0) ok = mbar_wait_cluster(v_ready, 0, p.status, SITEL_MMA_V);
       fence_proxy_async_smem();
       const uint32_t vs = smem_u32(vparts);
+      const uint32_t idesc = p.idesc2 | ((uint32_t)(turned ? (nrows + 15) / 16 * 2 : 16) << 17);
       for (int i = 0; i < ch1 - ch0 && ok; ++i) {
         const int buf = i & 1;
-        ok = mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, p.status, SITEL_MMA_ACC) && mbar_wait(&full[stage], phase, p.status, SITEL_MMA_FULL);
+        ok = mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, p.status, SITEL_MMA_ACC) && mbar_wait(&b_full[stage], phase, p.status, SITEL_MMA_FULL);
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t s = smem_u32(smem + stage * p.stage_bytes);
+        const uint32_t s = smem_u32(smem + stage * p.b_bytes);
         for (int part = 0; part < PARTS; ++part)
           for (int k = 0; k < rsteps; ++k) {
             const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;  // block of 64, step of 16 inside it
-            tc_mma_ss<KIND_F16>(tmem_base + buf * 128, umma_desc_k_sw128(vs + part * rblocks * (128 * 128) + at), umma_desc_k_sw128(s + at),
-                                p.idesc2, (part | k) != 0 ? 1u : 0u);
+            const uint64_t vd = umma_desc_k_sw128(vs + part * rblocks * (128 * 128) + at), bd = umma_desc_k_sw128(s + at);
+            tc_mma_ss<KIND_F16>(tmem_base + buf * 128, turned ? bd : vd, turned ? vd : bd, idesc, (part | k) != 0 ? 1u : 0u);
           }
-        tc_commit(&empty[stage]);
+        tc_commit(&b_empty[stage]);
         tc_commit(&acc_full[buf]);
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        if (++stage == p.b_stages) { stage = 0; phase ^= 1; }
       }
     }
     __syncwarp();
-  } else {
-    // ------------------------------------------------------------ warps 2-5: the rank-R product, then the epilogue
-    constexpr int EPV = 16 / (int)sizeof(OutT);  // elements of 16 bytes
-    constexpr int LPR = 32 / EPV;                // lanes side by side in one row of a step of 32 columns
-    constexpr int STEPS = 8 / LPR;               // steps whose C is on its way: 8 accesses of 16 bytes a lane
-    const int qd = warp & 3, et = (warp - 2) * 32 + lane;  // tensor-memory quarter; thread among the 128
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ warps 4-11: the rank-R product, then the epilogue
+    constexpr int BW = 128 / (int)sizeof(OutT), EPV = 16 / (int)sizeof(OutT);  // columns of a box; elements of 16 bytes
+    constexpr int BPC = 64 / BW;                                                // boxes of a warp's 64 columns of a chunk
+    const int qd = warp & 3, set = (warp - 4) >> 2, et = (warp - 4) * 32 + lane;  // tensor-memory quarter; half of a chunk's columns
     const int my_row = qd * 32 + lane;
-    const uint32_t t_lane = static_cast<uint32_t>(qd * 32) << 16;
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(qd * 32) << 16);
     const float scale = g.scales ? __ldg(g.scales + a) : 1.f;
-    const int sub_row = lane / LPR, sub_col = (lane % LPR) * EPV;  // access i of a step: row i * EPV + sub_row
-    uint4 cpre[STEPS][LPR];
-    auto prefetch = [&](uint4 (&to)[LPR], int n) {
-      n += sub_col;
-#pragma unroll
-      for (int i = 0; i < LPR; ++i) {
-        const int r = qd * 32 + i * EPV + sub_row;
-        if (r < nrows && n < g.n) to[i] = *reinterpret_cast<const uint4*>(c_base + r * g.c_pitch + n);
-      }
+    uint8_t* my_boxes = cboxes + (warp - 4) * p.c_bufs * 4096;
+    uint64_t* my_full = c_full + (warp - 4) * p.c_bufs;
+    const int nboxes = VEC && !turned && qd * 32 < nrows ? (ch1 - ch0) * BPC : 0;
+    auto box_col = [&](int k) { return (ch0 + k / BPC) * 128 + set * 64 + (k % BPC) * BW; };
+    auto request = [&](int k) {  // one lane
+      const int slot = k % p.c_bufs;
+      mbar_arrive_expect_tx(&my_full[slot], 4096);
+      tma_load_2d(my_boxes + slot * 4096, &tmC, &my_full[slot], box_col(k), row0 + qd * 32);
     };
-    if (VEC && ch0 < ch1) {
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) prefetch(cpre[s], ch0 * 128 + s * 32);
-    }
     // the value of `x` as PARTS 16-bit numbers, the largest first
     auto write_parts = [&](int row, int col, float4 x, auto&& store) {  // 4 columns at once
       float r[4] = {x.x, x.y, x.z, x.w};
@@ -392,13 +428,14 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         store((part * rblocks + (col >> 6)) * (128 * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 4) * 2, w0, w1);
       }
     };
-    // the four warps go on or give up together: they meet at barriers
-    bool ok = all_of_128(1, mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
+    bool ok = lora_epi_all(mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
     if (ok) {
       tc_fence_after_sync();
-      for (int c = 0; c < rsteps * 16; c += 16) {  // columns behind R are products with zero rows: zero
+      if (C == 1 && lane == 0)
+        for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
+      for (int c = set * 16; c < rsteps * 16; c += 32) {  // columns behind R are products with zero rows: zero
         uint32_t v[16];
-        tmem_ld_x16(tmem_base + t_lane + c, v);
+        tmem_ld_x16(t_lane + c, v);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -416,16 +453,17 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       tc_fence_before_sync();
       if (C == 1) {
         fence_proxy_async_smem();
-        lora_epi_sync();
+        lora_epi_all(true);
         if (et == 0) mbar_arrive(v_ready);
       } else {
-        lora_epi_sync();
+        lora_epi_all(true);
         if (et == 0)
           for (int c = 0; c < C; ++c) mbar_arrive_remote_release(mapa_shared(smem_u32(p_ready), c));
-        ok = all_of_128(1, mbar_wait_cluster(p_ready, 0, p.status, SITEL_EPI_PARTS));
+        ok = lora_epi_all(mbar_wait_cluster(p_ready, 0, p.status, SITEL_EPI_PARTS));
         if (ok) {
-          const int units = rsteps * 4, r0 = 128 * rank / C, r1 = 128 * (rank + 1) / C;
-          for (int i = et; i < (r1 - r0) * units; i += 128) {
+          // rows of the instruction behind the tile's own stay whatever they are: nothing reads their products
+          const int units = rsteps * 4, r0 = nrows * rank / C, r1 = nrows * (rank + 1) / C;
+          for (int i = et; i < (r1 - r0) * units; i += 256) {
             const int row = r0 + i / units, u = i - (row - r0) * units;
             const uint32_t at = smem_u32(parts + row * units * 4 + ((u + row) % units) * 4);
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -439,67 +477,130 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             });
           }
           fence_proxy_async_all();
-          lora_epi_sync();
+          lora_epi_all(true);
           if (et == 0)
             for (int c = 0; c < C; ++c) mbar_arrive_remote_release(mapa_shared(smem_u32(v_ready), c));
+          // the boxes lie where the parts were: only when every CTA has read them
+          ok = lora_epi_all(mbar_wait_cluster(v_ready, 0, p.status, SITEL_EPI_PARTS));
+          fence_proxy_async_smem();
+          if (ok && lane == 0)
+            for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
         }
       }
     }
-    float* st = parts + (warp - 2) * 32 * 32;  // this warp's staging: 32 rows of 32 columns, 16-byte units swizzled by the row
-    for (int i = 0; i < ch1 - ch0 && ok; ++i) {
-      const int buf = i & 1, n0 = (ch0 + i) * 128;
-      ok = mbar_wait(&acc_full[buf], (i >> 1) & 1, p.status, SITEL_EPI_ACC);
-      if (!ok) break;
-      tc_fence_after_sync();
-#pragma unroll 1
-      for (int h = 0; h < 128; h += 32 * STEPS) {
+    if (turned) {
+      // lanes: 128 columns of D; columns: its rows.  The two sets of four warps take every other chunk; C of the next one
+      // is on its way.  No branch around a single load: rows behind the last read that one again.
+      using Raw = typename std::conditional<sizeof(OutT) == 4, float, uint16_t>::type;
+      auto fetch = [&](int i, Raw (&c)[32]) {
+        const Raw* from = reinterpret_cast<const Raw*>(c_base) + min((ch0 + i) * 128 + my_row, g.n - 1);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          const int col = h + s * 32;
-          {
-            uint32_t v[32];
-            tmem_ld_x32(tmem_base + t_lane + buf * 128 + col, v);
+        for (int j0 = 0; j0 < 32; j0 += 8)
+          if (j0 < nrows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j0 + j] = from[min(j0 + j, nrows - 1) * g.c_pitch];
+          }
+      };
+      Raw c[32], ahead[32];
+      if (set < ch1 - ch0) fetch(set, c);
+      for (int i = set; i < ch1 - ch0 && ok; i += 2) {
+        const int n = (ch0 + i) * 128 + my_row;
+        if (i + 2 < ch1 - ch0) fetch(i + 2, ahead);
+        ok = mbar_wait(&acc_full[set], (i >> 1) & 1, p.status, SITEL_EPI_ACC);
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t v[32];
+        tmem_ld_x32(t_lane + set * 128, v);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[set]);
+        if (n < g.n) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < nrows) lora_store(d_base + j * g.d_pitch + n, lora_load(reinterpret_cast<const OutT*>(&c[j])) + __uint_as_float(v[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) c[j] = ahead[j];
+      }
+    } else {
+      const bool live = qd * 32 < nrows, whole = qd * 32 + 32 <= nrows;  // this warp's 32 rows
+      for (int i = 0; i < ch1 - ch0 && ok; ++i) {
+        const int buf = i & 1;
+        ok = mbar_wait(&acc_full[buf], (i >> 1) & 1, p.status, SITEL_EPI_ACC);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t t_half = t_lane + buf * 128 + set * 64;
+        auto release = [&]() {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        };
+        if (!live) {
+          release();
+          continue;
+        }
+        if constexpr (VEC) {
+          for (int b = 0; b < BPC; ++b) {
+            const int k = i * BPC + b, slot = k % p.c_bufs, col = box_col(k);
+            uint32_t v[BW];
+#pragma unroll
+            for (int c = 0; c < BW; c += 32) tmem_ld_x32(t_half + b * BW + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+            ok = mbar_wait(&my_full[slot], (k / p.c_bufs) & 1, p.status, SITEL_EPI_C);
             tmem_ld_wait();
+            if (b == BPC - 1) release();
+            if (!ok) break;
+            uint8_t* row = my_boxes + slot * 4096 + lane * 128;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              uint4* w = reinterpret_cast<uint4*>(row + ((u ^ (lane & 7)) << 4));
+              *w = lora_add(*w, v + u * EPV, static_cast<OutT*>(nullptr));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (whole) {
+              if (lane == 0) {
+                if (col < g.n) tma_store_2d(&tmD, my_boxes + slot * 4096, col, row0 + qd * 32);
+                tma_store_commit();
+                tma_store_wait_read<1>();  // the box before this one is free again
+              }
+            } else {  // the last rows of a request: vector stores of whole 128-byte rows
+              const int n = col + (lane & 7) * EPV;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                if (qd * 32 + r < nrows && n < g.n)
+                  *reinterpret_cast<uint4*>(d_base + (qd * 32 + r) * g.d_pitch + n) =
+                      *reinterpret_cast<const uint4*>(my_boxes + slot * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              }
+            }
+            if (lane == 0 && k + p.c_bufs - 1 < nboxes) request(k + p.c_bufs - 1);
+          }
+        } else {
+          float* st = reinterpret_cast<float*>(my_boxes);  // 32 rows of 32 columns, 16-byte units swizzled by the row
+          for (int h = 0; h < 64; h += 32) {
+            uint32_t v[32];
+            tmem_ld_x32(t_half + h, v);
+            tmem_ld_wait();
+            if (h == 32) release();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<uint4*>(st + lane * 32 + ((j ^ (lane & 7)) << 2)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          }
-          if (col + 32 >= 128) tc_fence_before_sync();
-          __syncwarp();
-          if (col + 32 >= 128 && lane == 0) mbar_arrive(&acc_empty[buf]);
-          if constexpr (VEC) {
-            const int n = n0 + col + sub_col;
-#pragma unroll
-            for (int k = 0; k < LPR; ++k) {
-              const int r = k * EPV + sub_row;
-              OutT o[EPV];
-              const OutT* cin = reinterpret_cast<const OutT*>(&cpre[s][k]);
-#pragma unroll
-              for (int e = 0; e < EPV; e += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(st + r * 32 + ((((sub_col + e) >> 2) ^ (r & 7)) << 2));
-                o[e] = cvt_out<OutT>(lora_load(cin + e) + x.x);
-                o[e + 1] = cvt_out<OutT>(lora_load(cin + e + 1) + x.y);
-                o[e + 2] = cvt_out<OutT>(lora_load(cin + e + 2) + x.z);
-                o[e + 3] = cvt_out<OutT>(lora_load(cin + e + 3) + x.w);
-              }
-              if (qd * 32 + r < nrows && n < g.n)
-                *reinterpret_cast<uint4*>(d_base + (qd * 32 + r) * g.d_pitch + n) = *reinterpret_cast<const uint4*>(o);
-            }
-            const int next = n0 + col + 32 * STEPS;  // the same step of the next round, maybe in the next chunk
-            if (next < ch1 * 128) prefetch(cpre[s], next);
-          } else {
+            __syncwarp();
+            const int n = (ch0 + i) * 128 + set * 64 + h + lane;
             for (int r = 0; r < 32 && qd * 32 + r < nrows; ++r) {
-              const long long row = qd * 32 + r;
-              if (n0 + col + lane < g.n) {
+              const long long at = qd * 32 + r;
+              if (n < g.n) {
                 const float x = st[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-                lora_store(d_base + row * g.d_pitch + n0 + col + lane, lora_load(c_base + row * g.c_pitch + n0 + col + lane) + x);
+                lora_store(d_base + at * g.d_pitch + n, lora_load(c_base + at * g.c_pitch + n) + x);
               }
             }
+            __syncwarp();  // the staging is read: the next step may overwrite it
           }
-          __syncwarp();  // the staging is read: the next step may overwrite it
         }
       }
     }
+    if (lane == 0) tma_store_wait_all<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -519,39 +620,49 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 }
 
 template <typename T, typename OutT, bool VEC>
-static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, cudaStream_t stream) {
+static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int out, cudaStream_t stream) {
   constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value && sizeof(OutT) == 4 ? 3 : 2;
   const int rsteps = (g.rank + 15) / 16, rblocks = (g.rank + 63) / 64, kbs = (g.k + 63) / 64;
   const long long tiles = ((long long)g.rows + 127) / 128 + (g.requests < g.rows ? g.requests : g.rows);  // at most
-  // CTAs of a tile: as few as fill the GPU with two CTAs per SM; each needs a K block
-  int ctas = 1;
-  while (ctas < kLoraCtas && ctas * 2 <= kbs && tiles * ctas < 2 * h->num_sms) ctas *= 2;
+  // CTAs of a tile: as many as find room at once, one per SM; each needs a K block
+  int ctas = (int)(h->num_sms / tiles);
+  if (ctas > kLoraCtas) ctas = kLoraCtas;
+  if (ctas > kbs) ctas = kbs;
+  if (ctas < 1) ctas = 1;
+  if (tiles * ctas > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "gemm_lora: too many rows and requests");
   LoraTileArgs p = {};
   p.g = g;
   const uint32_t fmt = dtype == MOYE_BF16 ? 1u : 0u;
   p.idesc1 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(rsteps * 2) << 17) | (8u << 24);
-  p.idesc2 = (1u << 4) | (fmt << 7) | (fmt << 10) | (16u << 17) | (8u << 24);
+  p.idesc2 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
   p.status = h->d_status;
-  const int block = 128 * 128;
-  p.stage_bytes = block + rsteps * 16 * 128 > rblocks * block ? block + rsteps * 16 * 128 : rblocks * block;
-  p.stage_bytes = (p.stage_bytes + 1023) & ~1023;
+  const int block = 128 * 128, total = 227 * 1024 - 1024;
+  p.k_bytes = (block + rsteps * 16 * 128 + 1023) & ~1023;
+  p.k_stages = total / p.k_bytes < 12 ? total / p.k_bytes : 12;
+  p.b_bytes = rblocks * block;
   const int v_bytes = PARTS * rblocks * block;
-  int out_bytes = 4 * 32 * 32 * 4;
-  if (ctas > 1 && 128 * rsteps * 16 * 4 > out_bytes) out_bytes = 128 * rsteps * 16 * 4;
-  const int rest = v_bytes + out_bytes + 512, half_sm = 113 * 1024;
-  // two CTAs per SM if three (two) stages fit into half of its shared memory, else one with as many as fit
-  p.stages = rest + 3 * p.stage_bytes <= half_sm ? 3 : rest + 2 * p.stage_bytes <= half_sm ? 2 : 4;
-  while (p.stages > 2 && rest + p.stages * p.stage_bytes > 227 * 1024) --p.stages;
-  p.v_off = p.stages * p.stage_bytes;
-  p.stage_out_off = p.v_off + v_bytes;
-  p.bar_off = p.stage_out_off + out_bytes;
-  const int smem = p.bar_off + 512;
-  CUtensorMap tx, ta, tb;
+  // boxes of C per warp: what two chunks of B leave room for (2 at rank 128 in three parts, 5 at rank 64)
+  p.c_bufs = (total - v_bytes - 2 * p.b_bytes) / (8 * 4096);
+  if (p.c_bufs > 6) p.c_bufs = 6;
+  p.b_stages = (total - v_bytes - p.c_bufs * 8 * 4096) / p.b_bytes;
+  if (p.b_stages > 4) p.b_stages = 4;
+  p.v_off = p.b_stages * p.b_bytes;
+  p.c_off = p.v_off + v_bytes;
+  p.bar_off = total;
+  const int smem = p.bar_off + 1024;
+  CUtensorMap tx, ta, tb, tc, td;
   if (int rc = encode_tmap_2d_uncached(&tx, g.X, dtype, g.k, g.rows, (uint64_t)g.x_pitch * 2, 64, 128, true)) return rc;
   const uint64_t a_pitch = g.a_pitch * 2, a_stride = g.adapters > 1 ? g.a_stride * 2 : g.rank * a_pitch;
   const uint64_t b_pitch = g.n > 1 ? g.b_pitch * 2 : g.rank * 2, b_stride = g.adapters > 1 ? g.b_stride * 2 : g.n * b_pitch;
   if (int rc = encode_tmap_3d(&ta, g.A, dtype, g.k, g.rank, g.adapters, a_pitch, a_stride, 64, rsteps * 16, true)) return rc;
   if (int rc = encode_tmap_3d(&tb, g.B, dtype, g.rank, g.n, g.adapters, b_pitch, b_stride, 64, 128, true)) return rc;
+  if constexpr (VEC) {
+    if (int rc = encode_tmap_2d_uncached(&tc, g.C, out, g.n, g.rows, (uint64_t)g.c_pitch * sizeof(OutT), 128 / sizeof(OutT), 32, true)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&td, g.D, out, g.n, g.rows, (uint64_t)g.d_pitch * sizeof(OutT), 128 / sizeof(OutT), 32, true)) return rc;
+  } else {  // not used
+    tc = tx;
+    td = tx;
+  }
   auto kern = lora_tile_kernel<T, OutT, VEC, PARTS>;
   if (int rc = configure_once(h, kern, 227 * 1024)) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -568,9 +679,9 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, cuda
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_without_pdl() ? 1 : 2;
-  log_line("gemm_lora %d rows, %d requests, rank %d, %d x %d  in %d  -> tiles of 128 rows on %d CTAs, %d stages", g.rows, g.requests,
-           g.rank, g.n, g.k, dtype, ctas, p.stages);
-  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tx, ta, tb, p));
+  log_line("gemm_lora %d rows, %d requests, rank %d, %d x %d  in %d  -> tiles of 128 rows on %d CTAs", g.rows, g.requests, g.rank, g.n,
+           g.k, dtype, ctas);
+  MOYE_CUDA(cudaLaunchKernelEx(&cfg, kern, tx, ta, tb, tc, td, p));
   return MOYE_OK;
 }
 
@@ -644,13 +755,13 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
     };
     const bool vec = on16(C) && on16(D), wide = D->dtype == MOYE_F32;
     if (X->dtype == MOYE_F16) {
-      if (wide) return vec ? launch_lora_tile<__half, float, true>(h, g, X->dtype, stream) : launch_lora_tile<__half, float, false>(h, g, X->dtype, stream);
-      return vec ? launch_lora_tile<__half, __half, true>(h, g, X->dtype, stream) : launch_lora_tile<__half, __half, false>(h, g, X->dtype, stream);
+      if (wide) return vec ? launch_lora_tile<__half, float, true>(h, g, X->dtype, D->dtype, stream) : launch_lora_tile<__half, float, false>(h, g, X->dtype, D->dtype, stream);
+      return vec ? launch_lora_tile<__half, __half, true>(h, g, X->dtype, D->dtype, stream) : launch_lora_tile<__half, __half, false>(h, g, X->dtype, D->dtype, stream);
     }
     if (wide)
-      return vec ? launch_lora_tile<__nv_bfloat16, float, true>(h, g, X->dtype, stream) : launch_lora_tile<__nv_bfloat16, float, false>(h, g, X->dtype, stream);
-    return vec ? launch_lora_tile<__nv_bfloat16, __nv_bfloat16, true>(h, g, X->dtype, stream)
-               : launch_lora_tile<__nv_bfloat16, __nv_bfloat16, false>(h, g, X->dtype, stream);
+      return vec ? launch_lora_tile<__nv_bfloat16, float, true>(h, g, X->dtype, D->dtype, stream) : launch_lora_tile<__nv_bfloat16, float, false>(h, g, X->dtype, D->dtype, stream);
+    return vec ? launch_lora_tile<__nv_bfloat16, __nv_bfloat16, true>(h, g, X->dtype, D->dtype, stream)
+               : launch_lora_tile<__nv_bfloat16, __nv_bfloat16, false>(h, g, X->dtype, D->dtype, stream);
   }
   log_line("gemm_lora %lld rows, %d requests, rank %lld, %lld x %lld  in %d  -> a cluster per row", (long long)T, requests, (long long)R,
            (long long)N, (long long)K, X->dtype);
