@@ -175,9 +175,16 @@ __device__ __forceinline__ bool lora_epi_all(bool mine) {
 }
 
 template <typename T>
-__device__ __forceinline__ uint32_t lora_pack2(float a, float b) {
-  const T lo = cvt_out<T>(a), hi = cvt_out<T>(b);
-  return (uint32_t)(*reinterpret_cast<const uint16_t*>(&lo)) | ((uint32_t)(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
+__device__ __forceinline__ uint32_t lora_pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t lora_pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t lora_pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 // One 16-byte word of outputs: the input word plus EPV accumulators.
 __device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float*) {
@@ -551,11 +558,12 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             if (b == BPC - 1) release();
             if (!ok) break;
             uint8_t* row = my_boxes + slot * 4096 + lane * 128;
+            uint4 w[8];  // all reads before the first write: the compiler cannot know that they do not overlap
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              uint4* w = reinterpret_cast<uint4*>(row + ((u ^ (lane & 7)) << 4));
-              *w = lora_add(*w, v + u * EPV, static_cast<OutT*>(nullptr));
-            }
+            for (int u = 0; u < 8; ++u) w[u] = *reinterpret_cast<const uint4*>(row + ((u ^ (lane & 7)) << 4));
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(row + ((u ^ (lane & 7)) << 4)) = lora_add(w[u], v + u * EPV, static_cast<OutT*>(nullptr));
             fence_proxy_async_smem();
             __syncwarp();
             if (whole) {
