@@ -720,7 +720,7 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.D = D->ptr;
   a.ld = D->stride[0];
   a.status = h->d_status;
-  const long long tiles = ((R + bt - 1) / bt + (G < R ? G : R)) * a.lane_tiles;  // at most
+  const long long live = G < R ? G : R, tiles = (live + (R - live) / bt) * a.lane_tiles;  // at most
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
   CUtensorMap tl, tc, tn, td;
   std::memset(&td, 0, sizeof(td));

@@ -631,20 +631,51 @@ template <typename T, typename OutT, bool VEC>
 static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int out, cudaStream_t stream) {
   constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value && sizeof(OutT) == 4 ? 3 : 2;
   const int rsteps = (g.rank + 15) / 16, rblocks = (g.rank + 63) / 64, kbs = (g.k + 63) / 64;
-  const long long tiles = ((long long)g.rows + 127) / 128 + (g.requests < g.rows ? g.requests : g.rows);  // at most
-  // CTAs of a tile: as many as find room at once, one per SM; each needs a K block
-  int ctas = (int)(h->num_sms / tiles);
-  if (ctas > kLoraCtas) ctas = kLoraCtas;
-  if (ctas > kbs) ctas = kbs;
-  if (ctas < 1) ctas = 1;
-  if (tiles * ctas > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "gemm_lora: too many rows and requests");
+  const long long live = g.requests < g.rows ? g.requests : g.rows, tiles = live + (g.rows - live) / 128;  // at most
+  if (tiles > INT32_MAX / 16) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "gemm_lora: too many rows and requests");
+  auto kern = lora_tile_kernel<T, OutT, VEC, PARTS>;
+  if (int rc = configure_once(h, kern, 227 * 1024)) return rc;
+  const int total = 227 * 1024 - 1024, smem = total + 1024;
+  // CTAs of a tile: as many as let all tiles run at once, one CTA per SM (a cluster has to find its SMs in one part of the
+  // GPU: 16 clusters of 8 do not fit on 148 SMs); each needs a K block
+  int ctas = kLoraCtas < kbs ? kLoraCtas : kbs;
+  for (; ctas > 1; --ctas) {
+    if (tiles * ctas > h->num_sms) continue;
+    const uint64_t key = reinterpret_cast<uint64_t>(kern) * 16 + ctas;
+    int fit = -1;
+    {
+      std::lock_guard<std::mutex> lk(h->mu);
+      auto it = h->cluster_fit.find(key);
+      if (it != h->cluster_fit.end()) fit = it->second;
+    }
+    if (fit < 0) {
+      cudaLaunchConfig_t probe = {};
+      probe.gridDim = dim3((unsigned)ctas);
+      probe.blockDim = dim3(kLoraTileThreads);
+      probe.dynamicSmemBytes = smem;
+      cudaLaunchAttribute size[1];
+      size[0].id = cudaLaunchAttributeClusterDimension;
+      size[0].val.clusterDim.x = ctas;
+      size[0].val.clusterDim.y = 1;
+      size[0].val.clusterDim.z = 1;
+      probe.attrs = size;
+      probe.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fit, kern, &probe) != cudaSuccess) {
+        (void)cudaGetLastError();
+        fit = 0;
+      }
+      std::lock_guard<std::mutex> lk(h->mu);
+      h->cluster_fit[key] = fit;
+    }
+    if (fit >= tiles) break;
+  }
   LoraTileArgs p = {};
   p.g = g;
   const uint32_t fmt = dtype == MOYE_BF16 ? 1u : 0u;
   p.idesc1 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(rsteps * 2) << 17) | (8u << 24);
   p.idesc2 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
   p.status = h->d_status;
-  const int block = 128 * 128, total = 227 * 1024 - 1024;
+  const int block = 128 * 128;
   p.k_bytes = (block + rsteps * 16 * 128 + 1023) & ~1023;
   p.k_stages = total / p.k_bytes < 12 ? total / p.k_bytes : 12;
   p.b_bytes = rblocks * block;
@@ -657,7 +688,6 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int 
   p.v_off = p.b_stages * p.b_bytes;
   p.c_off = p.v_off + v_bytes;
   p.bar_off = total;
-  const int smem = p.bar_off + 1024;
   CUtensorMap tx, ta, tb, tc, td;
   if (int rc = encode_tmap_2d_uncached(&tx, g.X, dtype, g.k, g.rows, (uint64_t)g.x_pitch * 2, 64, 128, true)) return rc;
   const uint64_t a_pitch = g.a_pitch * 2, a_stride = g.adapters > 1 ? g.a_stride * 2 : g.rank * a_pitch;
@@ -671,8 +701,6 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int 
     tc = tx;
     td = tx;
   }
-  auto kern = lora_tile_kernel<T, OutT, VEC, PARTS>;
-  if (int rc = configure_once(h, kern, 227 * 1024)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ctas));
   cfg.blockDim = dim3(kLoraTileThreads);
@@ -754,8 +782,12 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
   g.which = which;
   g.offsets = offsets;
   g.scales = scales;
-  // Requests of several rows share their adapter's factors on the tensor cores; single rows do not.
-  if (offsets && T >= 4ll * requests) {
+  // Requests of several rows share their adapter's factors on the tensor cores.  A row by itself costs its factors' bytes
+  // from L2, about 4.3e-7 us x R (K + N) (2048 rows, R = 16, K = N = 4096: 117 us; R = 64: 416); the tile kernel starts 10 us
+  // later and takes about 3.6e-5 us x (K + N) per tile (256 tiles, R = 16: 93 us; R = 64: 109).  64 requests of 4 / 8 / 16
+  // rows, R = 16: rows 22 / 37 / 64 us, tiles 33 / 35 / 35.
+  const double tiles = (double)T / 128 + (requests < T ? requests : T);
+  if (offsets && (double)T * R > 84 * tiles + 2.3e7 / (double)(K + N)) {
     auto on16 = [](const moye_tensor_t* t) {
       const int eb = dtype_bytes(t->dtype);
       return (reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && (t->shape[1] * eb) % 16 == 0 &&
