@@ -29,6 +29,7 @@
 namespace moye {
 
 constexpr int kMaxGemmGroups = 1024;
+constexpr int kMaxGroupedExtent = 1 << 27;  // a sum this long ends well inside the limit of a bounded wait
 enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164, SITEG_FIX_TAIL = 165, SITEG_RING = 166 };
 enum : int { GROUPED_K_MAJOR = 0, GROUPED_MN_MAJOR = 1, GROUPED_GRAD = 2 };
 
@@ -686,7 +687,7 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
               (long long)K, (long long)G, (long long)N, (long long)B->shape[2], (long long)D->shape[0], (long long)D->shape[1]);
   if (int rc = check_grouped_types(who, A, B, D)) return rc;
   if (R < 0 || N <= 0 || K <= 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: empty product", who);
-  if (R > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
+  if (R > kMaxGroupedExtent || N > kMaxGroupedExtent || K > kMaxGroupedExtent) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
   if (int rc = check_borders(who, offsets, (int)(G > INT32_MAX ? INT32_MAX : G))) return rc;
   if (R == 0) return MOYE_OK;
   if (!A->ptr || !B->ptr || !D->ptr) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: null data pointer", who);
@@ -748,7 +749,7 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
               (long long)K, (long long)dD->shape[0], (long long)dD->shape[1], (long long)G, (long long)N, (long long)dB->shape[2]);
   if (int rc = check_grouped_types(who, A, dD, dB)) return rc;
   if (R < 0 || N <= 0 || K <= 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: empty product", who);
-  if (R > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
+  if (R > kMaxGroupedExtent || N > kMaxGroupedExtent || K > kMaxGroupedExtent) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: extent too large", who);
   if (int rc = check_borders(who, offsets, (int)(G > INT32_MAX ? INT32_MAX : G))) return rc;
   if (!dB->ptr || (R > 0 && (!A->ptr || !dD->ptr))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: null data pointer", who);
   if (int rc = check_row_operand(who, "A", A)) return rc;

@@ -134,6 +134,8 @@ lora_row_kernel(const LoraArgs g) {
 // the rows in CTA order and handing the result to all; every CTA then multiplies it with its 128-column chunks of B[a] and
 // adds C.  The product of rank R enters the second multiplication as a sum of 16-bit parts: two parts carry 16 (bf16)
 // or 22 (f16) bits, a sixteenth of an output step or less; bf16 operands with a Float32 output take three (24 bits).
+// f16 has not the range of the fp32 sums (65504, and steps of 2^-24 near zero): a row is brought to magnitude 1 by a power
+// of two first, which the epilogue takes back.
 //
 // Warp 0 producer, warp 1 MMA issuer, warps 4-11 move the parts and run the epilogue.  The kernel is bound by memory (X and
 // C in, D out) and lives on bytes in flight.  The first product has all of shared memory for its ring of K blocks (9 at
@@ -186,18 +188,27 @@ __device__ __forceinline__ uint32_t lora_pack2<__nv_bfloat16>(float a, float b) 
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// One 16-byte word of outputs: the input word plus EPV accumulators.
-__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float*) {
-  return make_uint4(__float_as_uint(__uint_as_float(c.x) + __uint_as_float(v[0])), __float_as_uint(__uint_as_float(c.y) + __uint_as_float(v[1])),
-                    __float_as_uint(__uint_as_float(c.z) + __uint_as_float(v[2])), __float_as_uint(__uint_as_float(c.w) + __uint_as_float(v[3])));
+// One 16-byte word of outputs: the input word plus `up` times EPV accumulators.
+__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float up, float*) {
+  return make_uint4(__float_as_uint(fmaf(__uint_as_float(v[0]), up, __uint_as_float(c.x))), __float_as_uint(fmaf(__uint_as_float(v[1]), up, __uint_as_float(c.y))),
+                    __float_as_uint(fmaf(__uint_as_float(v[2]), up, __uint_as_float(c.z))), __float_as_uint(fmaf(__uint_as_float(v[3]), up, __uint_as_float(c.w))));
 }
 template <typename T>
-__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, T*) {
+__device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float up, T*) {
   float f[8];
   lora_unpack<T>(c, f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] += __uint_as_float(v[e]);
+  for (int e = 0; e < 8; ++e) f[e] = fmaf(__uint_as_float(v[e]), up, f[e]);
   return make_uint4(lora_pack2<T>(f[0], f[1]), lora_pack2<T>(f[2], f[3]), lora_pack2<T>(f[4], f[5]), lora_pack2<T>(f[6], f[7]));
+}
+
+// The powers of two that bring a row whose magnitudes stay below `m` to magnitude 1 (`down`) and back (`up`); 1 where m
+// is no number.
+__device__ __forceinline__ void lora_range(float m, float& down, float& up) {
+  const int e = static_cast<int>(__float_as_uint(m) >> 23);  // m >= 0: the biased exponent
+  const int x = min(e, 252);
+  down = e == 255 ? 1.f : __uint_as_float(static_cast<uint32_t>(253 - x) << 23);  // 2^(126 - x): m * down is in [1/2, 1)
+  up = e == 255 ? 1.f : __uint_as_float(static_cast<uint32_t>(x + 1) << 23);
 }
 
 // The request and first row of tile `want`; q = -1 when there are fewer tiles.  All threads of the CTA; `sums` holds one
@@ -256,7 +267,10 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
            *v_acc = bars + 36, *p_ready = bars + 37, *v_ready = bars + 38, *c_full = bars + 40;  // c_full[8 warps][c_bufs <= 6]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 39);
   int* scratch = reinterpret_cast<int*>(bars + 88);          // 12 warp sums, then the tile
+  float* row_max = reinterpret_cast<float*>(bars + 128);     // [2 sets][128 rows]
+  float* row_up = row_max + 256;                             // [128 rows]
   constexpr uint32_t TMEM_COLS = 256;
+  constexpr bool RANGE = std::is_same<T, __half>::value;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
@@ -431,7 +445,9 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       for (int part = 0; part < PARTS; ++part) {
         const uint32_t w0 = lora_pack2<T>(r[0], r[1]), w1 = lora_pack2<T>(r[2], r[3]);
         const float2 f0 = lora_pair<T>(w0), f1 = lora_pair<T>(w1);
-        r[0] -= f0.x; r[1] -= f0.y; r[2] -= f1.x; r[3] -= f1.y;
+        const float f[4] = {f0.x, f0.y, f1.x, f1.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = isinf(f[i]) ? 0.f : r[i] - f[i];  // an infinity has no rest
         store((part * rblocks + (col >> 6)) * (128 * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 4) * 2, w0, w1);
       }
     };
@@ -440,23 +456,39 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       tc_fence_after_sync();
       if (C == 1 && lane == 0)
         for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
-      for (int c = set * 16; c < rsteps * 16; c += 32) {  // columns behind R are products with zero rows: zero
-        uint32_t v[16];
-        tmem_ld_x16(t_lane + c, v);
-        tmem_ld_wait();
+      auto each_16 = [&](auto&& f) {  // this set's columns; those behind R are products with zero rows: zero
+        for (int c = set * 16; c < rsteps * 16; c += 32) {
+          uint32_t v[16];
+          tmem_ld_x16(t_lane + c, v);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 x = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
-          if (C == 1) {
-            write_parts(my_row, c + j, make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale),
-                        [&](int at, uint32_t w0, uint32_t w1) { *reinterpret_cast<uint2*>(vparts + at) = make_uint2(w0, w1); });
-          } else {
-            // 16-byte units of a row rotated by the row: neighbouring rows fall on different banks
-            const int units = rsteps * 4, u = ((c + j) >> 2) + my_row;
-            *reinterpret_cast<float4*>(parts + my_row * units * 4 + (u % units) * 4) = x;
-          }
+          for (int j = 0; j < 16; j += 4)
+            f(c + j, make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
         }
+      };
+      float down = scale, most = 0.f;
+      auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))); };
+      if (RANGE && C == 1) {
+        each_16([&](int, const float4& x) { largest(x); });
+        row_max[set * 128 + my_row] = most;
+        lora_epi_all(true);
+        float up;
+        lora_range(fmaxf(row_max[my_row], row_max[128 + my_row]) * fabsf(scale), down, up);
+        down *= scale;
+        if (set == 0) row_up[my_row] = up;
       }
+      each_16([&](int c, const float4& x) {
+        if (C == 1) {
+          write_parts(my_row, c, make_float4(x.x * down, x.y * down, x.z * down, x.w * down),
+                      [&](int at, uint32_t w0, uint32_t w1) { *reinterpret_cast<uint2*>(vparts + at) = make_uint2(w0, w1); });
+        } else {
+          // 16-byte units of a row rotated by the row: neighbouring rows fall on different banks
+          const int units = rsteps * 4, u = (c >> 2) + my_row;
+          *reinterpret_cast<float4*>(parts + my_row * units * 4 + (u % units) * 4) = x;
+          if (RANGE) largest(x);
+        }
+      });
+      if (RANGE && C > 1) row_max[set * 128 + my_row] = most;
       tc_fence_before_sync();
       if (C == 1) {
         fence_proxy_async_smem();
@@ -470,6 +502,17 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         if (ok) {
           // rows of the instruction behind the tile's own stay whatever they are: nothing reads their products
           const int units = rsteps * 4, r0 = nrows * rank / C, r1 = nrows * (rank + 1) / C;
+          auto range_of = [&](int row, float& down, float& up) {  // by the sum of the CTAs' largest: cheaper than the sums' own
+            const uint32_t at = smem_u32(row_max + row);
+            float m = 0.f;
+            for (int c = 0; c < C; ++c) m += fmaxf(ld_remote_f32(mapa_shared(at, c)), ld_remote_f32(mapa_shared(at + 512, c)));
+            lora_range(m * fabsf(scale), down, up);
+          };
+          if (RANGE && et < nrows) {
+            float down, up;
+            range_of(et, down, up);
+            row_up[et] = up;
+          }
           for (int i = et; i < (r1 - r0) * units; i += 256) {
             const int row = r0 + i / units, u = i - (row - r0) * units;
             const uint32_t at = smem_u32(parts + row * units * 4 + ((u + row) % units) * 4);
@@ -478,7 +521,10 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
               const float4 x = ld_remote_f32x4(mapa_shared(at, c));
               s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
             }
-            write_parts(row, u * 4, make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale), [&](int off, uint32_t w0, uint32_t w1) {
+            float down = 1.f, up;
+            if (RANGE) range_of(row, down, up);
+            down *= scale;
+            write_parts(row, u * 4, make_float4(s.x * down, s.y * down, s.z * down, s.w * down), [&](int off, uint32_t w0, uint32_t w1) {
               const uint32_t to = smem_u32(vparts + off);
               for (int c = 0; c < C; ++c) st_remote_u32x2(mapa_shared(to, c), w0, w1);
             });
@@ -525,13 +571,14 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         if (n < g.n) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (j < nrows) lora_store(d_base + j * g.d_pitch + n, lora_load(reinterpret_cast<const OutT*>(&c[j])) + __uint_as_float(v[j]));
+            if (j < nrows) lora_store(d_base + j * g.d_pitch + n, fmaf(__uint_as_float(v[j]), RANGE ? row_up[j] : 1.f, lora_load(reinterpret_cast<const OutT*>(&c[j]))));
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) c[j] = ahead[j];
       }
     } else {
       const bool live = qd * 32 < nrows, whole = qd * 32 + 32 <= nrows;  // this warp's 32 rows
+      const float up = RANGE && my_row < nrows ? row_up[my_row] : 1.f;
       for (int i = 0; i < ch1 - ch0 && ok; ++i) {
         const int buf = i & 1;
         ok = mbar_wait(&acc_full[buf], (i >> 1) & 1, p.status, SITEL_EPI_ACC);
@@ -563,7 +610,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             for (int u = 0; u < 8; ++u) w[u] = *reinterpret_cast<const uint4*>(row + ((u ^ (lane & 7)) << 4));
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4*>(row + ((u ^ (lane & 7)) << 4)) = lora_add(w[u], v + u * EPV, static_cast<OutT*>(nullptr));
+              *reinterpret_cast<uint4*>(row + ((u ^ (lane & 7)) << 4)) = lora_add(w[u], v + u * EPV, up, static_cast<OutT*>(nullptr));
             fence_proxy_async_smem();
             __syncwarp();
             if (whole) {
@@ -600,7 +647,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
               const long long at = qd * 32 + r;
               if (n < g.n) {
                 const float x = st[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-                lora_store(d_base + at * g.d_pitch + n, lora_load(c_base + at * g.c_pitch + n) + x);
+                lora_store(d_base + at * g.d_pitch + n, fmaf(x, RANGE ? row_up[at] : 1.f, lora_load(c_base + at * g.c_pitch + n)));
               }
             }
             __syncwarp();  // the staging is read: the next step may overwrite it
@@ -635,7 +682,7 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int 
   if (tiles > INT32_MAX / 16) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "gemm_lora: too many rows and requests");
   auto kern = lora_tile_kernel<T, OutT, VEC, PARTS>;
   if (int rc = configure_once(h, kern, 227 * 1024)) return rc;
-  const int total = 227 * 1024 - 1024, smem = total + 1024;
+  const int total = 227 * 1024 - 3072, smem = total + 3072;  // the last 3 KB: barriers, row ranges
   // CTAs of a tile: as many as let all tiles run at once, one CTA per SM (a cluster has to find its SMs in one part of the
   // GPU: 16 clusters of 8 do not fit on 148 SMs); each needs a K block
   int ctas = kLoraCtas < kbs ? kLoraCtas : kbs;
@@ -765,8 +812,13 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
   for (const moye_tensor_t* t : {D, C})
     if ((N > 1 && t->stride[1] != 1) || (T > 1 && t->stride[0] < N))
       MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "gemm_lora: rows of C and D must be contiguous and must not overlap");
-  if (C->ptr == D->ptr && T > 1 && C->stride[0] != D->stride[0])
-    MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: C at D's address must be D");
+  auto overlap = [](const moye_tensor_t* a, const moye_tensor_t* b) {
+    auto end = [](const moye_tensor_t* t) { return static_cast<const char*>(t->ptr) + ((t->shape[0] - 1) * t->stride[0] + t->shape[1]) * dtype_bytes(t->dtype); };
+    return a->ptr < static_cast<const void*>(end(b)) && b->ptr < static_cast<const void*>(end(a));
+  };
+  if (overlap(C, D) && !(C->ptr == D->ptr && (T == 1 || C->stride[0] == D->stride[0])))
+    MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: C and D overlap without being the same");
+  if (overlap(X, D)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: X and D overlap");
   LoraArgs g = {};
   g.rows = (int)T;
   g.requests = requests;

@@ -449,7 +449,9 @@ combine_rows_grad_kernel(T* dsrc, const T* ddst, const T* src, const RowArgs g) 
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-static int check_rows(const char* who, const moye_tensor_t* token_side, const moye_tensor_t* sorted_side, int choices) {
+// Rows of an array that is only read may lie on one another (a broadcast gradient); `written` is the one that is not.
+static int check_rows(const char* who, const moye_tensor_t* token_side, const moye_tensor_t* sorted_side, const moye_tensor_t* written,
+                      int choices) {
   if (token_side->rank != 2 || sorted_side->rank != 2) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: arrays must be rank 2", who);
   if (token_side->dtype != sorted_side->dtype) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "%s: element types differ", who);
   const long long tokens = token_side->shape[0], width = token_side->shape[1];
@@ -460,7 +462,8 @@ static int check_rows(const char* who, const moye_tensor_t* token_side, const mo
               who, tokens, width, choices, tokens * choices, width, (long long)sorted_side->shape[0], (long long)sorted_side->shape[1]);
   for (const moye_tensor_t* t : {token_side, sorted_side}) {
     if (t->shape[1] > 1 && t->stride[1] != 1) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows must be contiguous", who);
-    if (t->shape[0] > 1 && t->stride[0] < t->shape[1]) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows overlap", who);
+    if (t->shape[0] > 1 && t->stride[0] < (t == written ? t->shape[1] : 0))
+      MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows %s", who, t == written ? "of an output overlap" : "with a negative pitch");
   }
   return MOYE_OK;
 }
@@ -487,7 +490,7 @@ static int row_grid(const char* who, const RowArgs& g, int packs_per_lane, unsig
 
 int launch_gather_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_tensor_t* src, const int* inverse, int choices,
                        cudaStream_t stream) {
-  if (int rc = check_rows("gather_rows", src, dst, choices)) return rc;
+  if (int rc = check_rows("gather_rows", src, dst, dst, choices)) return rc;
   const int eb = dtype_bytes(src->dtype);
   if (eb != 1 && eb != 2 && eb != 4 && eb != 8) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "gather_rows: elements of 1, 2, 4 or 8 bytes");
   if (src->shape[0] == 0 || src->shape[1] == 0) return MOYE_OK;
@@ -542,7 +545,7 @@ static int for_float_rows(const char* who, int dtype, bool wide, F f) {
 
 int launch_combine_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_tensor_t* src, const moye_tensor_t* weights,
                         const int* inverse, int choices, cudaStream_t stream) {
-  if (int rc = check_rows("combine_rows", dst, src, choices)) return rc;
+  if (int rc = check_rows("combine_rows", dst, src, dst, choices)) return rc;
   if (weights)
     if (int rc = check_weights("combine_rows", weights, dst->shape[0], choices)) return rc;
   if (dst->shape[0] == 0 || dst->shape[1] == 0) return MOYE_OK;
@@ -578,8 +581,8 @@ int launch_combine_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_ten
 int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const moye_tensor_t* dweights, const moye_tensor_t* ddst,
                              const moye_tensor_t* src, const moye_tensor_t* weights, const int* inverse, int choices,
                              cudaStream_t stream) {
-  if (int rc = check_rows("combine_rows_grad", ddst, src, choices)) return rc;
-  if (int rc = check_rows("combine_rows_grad", ddst, dsrc, choices)) return rc;
+  if (int rc = check_rows("combine_rows_grad", ddst, src, nullptr, choices)) return rc;
+  if (int rc = check_rows("combine_rows_grad", ddst, dsrc, dsrc, choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", weights, ddst->shape[0], choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", dweights, ddst->shape[0], choices)) return rc;
   if (weights->dtype != dweights->dtype) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "combine_rows_grad: weights and dweights differ in type");

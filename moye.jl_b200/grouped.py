@@ -24,7 +24,8 @@ __all__ = ["RowGroups", "group_rows", "group_rows_", "gather_rows_", "combine_ro
            "gemm_grouped_grad_", "gemm_lora_"]
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a torch Stream object costs 2 us a call
+# the stream's handle alone: a torch Stream object costs 2 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 _PACK = _lib.TENSOR_PACKERS
 _INT32, _FLOAT32 = torch.int32, torch.float32
 

@@ -92,6 +92,39 @@ def test_infinities_stay_in_their_rows(mb, dev):
     assert bad.nonzero().view(-1).tolist() == [129]
 
 
+@pytest.mark.parametrize("size", [1e-6, 3e5])
+@pytest.mark.parametrize("offsets", [[0, 300], [0, 20], [0, 1, 2], list(range(0, 40 * 200, 40))])
+def test_the_range_of_f16(mb, dev, offsets, size):
+    """The product of rank R may leave the range of f16 (65504; steps of 2^-24 near zero) where the operands and the result
+    do not: its 16-bit parts are taken relative to the row's largest."""
+    rows, n, k, rank, count = offsets[-1], 264, 512, 24, 3
+    gen = torch.Generator(device=dev).manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen, device=dev)
+    up, down = (size ** 0.5 * 0.2, 1.0) if size > 1 else (size ** 0.5, 1.0)
+    x, a = (r(rows, k) * up).half(), (r(count, rank, k) * up * k ** -0.5).half()
+    b = (r(count, n, rank) * min(down / size, 6e4 / 5)).half()
+    which = [i % count for i in range(len(offsets) - 1)]
+    edge, w = torch.tensor(offsets, dtype=torch.int32, device=dev), torch.tensor(which, dtype=torch.int32, device=dev)
+    c = r(rows, n)
+    d = mb.gemm_lora_(torch.empty_like(c), x, a, b, w, edge, C=c)
+    assert bool(d.isfinite().all())
+    check(d, c, x, a, b, None, which, offsets, torch.float32, d)
+
+
+def test_an_infinity_stays_one(mb, dev):
+    """One infinite product of rank R: the outputs it reaches are infinite, not undefined."""
+    for kind in ("f16", "bf16"):
+        for rows in (1, 20, 300):
+            x, a, b = torch.ones(rows, 64, device=dev).to(DT[kind]), torch.zeros(1, 8, 64, device=dev).to(DT[kind]), torch.ones(1, 40, 8, device=dev).to(DT[kind])
+            x[rows // 2, 0] = float("inf")
+            a[0, 3, 0] = 1.0
+            a[0, 3, 1] = 1.0
+            x[:, 2:] = 0
+            d = mb.gemm_lora_(torch.zeros(rows, 40, device=dev), x, a[:, 3:4].expand(1, 8, 64).contiguous(), b, torch.zeros(1, dtype=torch.int32, device=dev),
+                              torch.tensor([0, rows], dtype=torch.int32, device=dev))
+            assert bool((d[rows // 2] == float("inf")).all()) and int((~d.isfinite()).any(1).sum()) == 1
+
+
 def test_beside_a_projection_captured(mb, dev):
     """A decoding step: the shared projection by `gemm_`, the adapters in place behind it, captured once and replayed
     with other tokens and other adapters."""

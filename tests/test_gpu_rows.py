@@ -10,7 +10,7 @@ DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 # tokens, choices, groups, width, type: one row, odd and unaligned widths, more entries than one CTA sorts, the most groups
 CASES = [(1, 1, 1, 8, "bf16"), (1, 8, 8, 5000, "f16"), (5, 3, 4, 1, "f32"), (33, 2, 7, 130, "bf16"), (300, 1, 1, 64, "f32"),
          (2039, 3, 17, 101, "f32"), (513, 8, 128, 2048, "bf16"), (700, 9, 1024, 33, "f16"), (4100, 2, 1024, 16, "bf16"),
-         (97, 20, 31, 520, "f32")]
+         (97, 20, 31, 520, "f32"), (50, 40, 9, 264, "bf16"), (12, 67, 5, 33, "f16")]
 
 
 def ids_for(tokens, choices, groups, seed, dtype=torch.int64, dropped=0.2):
@@ -164,6 +164,19 @@ def test_pitched_and_unaligned_views(mb, dev):
         terms = xs.double()[plan.inverse.long()] * w.double()[:, :, None]
         assert close(out[:, shift:shift + width], terms.sum(1), terms.abs().sum(1), choices, torch.bfloat16)
         assert bool((out[:, :shift] == 7).all()) and bool((out[:, shift + width:] == 7).all())
+
+
+def test_broadcast_inputs(mb, dev):
+    """A gradient that is the same for all tokens (an expanded row) is read as it is."""
+    plan = mb.group_rows(ids_for(30, 2, 4, 29).to(dev), 4)
+    x, ys, w, dy = data(30, 2, 64, torch.float32, dev)
+    one = dy[:1].expand(30, 64)
+    got = mb.combine_rows_grad_(torch.zeros_like(ys), torch.empty_like(w), one, ys, plan, w)
+    want = mb.combine_rows_grad_(torch.zeros_like(ys), torch.empty_like(w), one.contiguous(), ys, plan, w)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(mb.gather_rows_(torch.zeros_like(ys), one, plan), mb.gather_rows_(torch.zeros_like(ys), one.contiguous(), plan))
+    with pytest.raises(mb.MoyeError):
+        mb.combine_rows_(torch.zeros(1, 64, device=dev).expand(30, 64), ys, plan)
 
 
 def test_infinities_stay_in_their_rows(mb, dev):
