@@ -41,8 +41,8 @@ struct GroupedArgs {
   int cols;             // gradient: extent of the other mode (N)
   int k_blocks;         // forward: blocks of 64 along K
   int lane_tiles, col_tiles;
-  int tma_out;          // a 16-bit D that vectors and TMA may write
   int vec_out;          // D has a 16-byte base and pitches (and, for 16-bit outputs, beta is 0: one rounding)
+  int tma_out;          // ... and TMA too: beta is 0 (or, for Float32 outputs, 1)
   const int* offsets;
   uint32_t idesc;       // without N
   float alpha, beta;
@@ -160,6 +160,13 @@ __device__ __forceinline__ void deal_tiles(const GroupedArgs& a, TileRing& ring,
   if (ok) deal(end);
 }
 
+__device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* m, const void* smem_src, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // Tensor memory -> registers in the order of matrix fragments: 16 lanes x 32 columns, of which thread T receives, for the
 // columns 8 b + 2 (T % 4) and the next one, lane T / 4 in v[4 b], v[4 b + 1] and lane T / 4 + 8 in v[4 b + 2], v[4 b + 3].
 __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(384, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
                     const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
   // tmL: the operand along the lanes (weights / A), tmC: the one along the columns (rows of A / dD), tmN: the same in
-  // boxes of 32 rows for narrow tiles, tmD: a 16-bit output
+  // boxes of 32 rows for narrow tiles, tmD: the output (swizzled boxes of 64 lanes, or plain ones of 32 for Float32)
   constexpr int BK = 64, UMMA_K = 16;
   constexpr int L_BYTES = 128 * 128;
   constexpr int C_BYTES = BT / 2 * 128;  // this CTA's half of the columns
@@ -199,7 +206,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   constexpr int EPI_BUF = 32 * 128;            // a staging tile: 32 columns of 128 bytes
   constexpr int EPI_BYTES = 8 * EPI_BUF;       // one per epilogue warp (Float32 outputs) or two per pair of them
   constexpr int C_BOX = grouped_box_rows(BT);  // rows of one load of a K-major column operand
-  static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128) && (!PROMOTE || BT <= 128), "tile columns");
+  static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128), "tile columns");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -257,6 +264,11 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   TileRing ring{ring_slots, ring_full, ring_empty, a.status, 0};
   GroupedTile tile;
 
+  // Float32 tiles of 256 columns keep 128 sums a thread: the eight epilogue warps take registers over from the other four
+  // (4 x 32 x 40 + 8 x 32 x 232 = 12 x 32 x 168).
+  constexpr bool SHIFT_REGS = PROMOTE && BT == 256;
+  if (warp < 4) {
+  if (SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
@@ -385,7 +397,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   } else if (warp == 3) {
     // ------------------------------------------------------------ tile scheduler (each CTA for itself, the same tiles)
     deal_tiles<MODE, BT>(a, ring, first_tile, tile_step, lane);
-  } else if (warp >= 4) {
+  }
+  } else {
+    if (SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ------------------------------------------------------------ epilogue (warps 4..11, both CTAs)
     // Four warps read the tensor memory's four quarters of 32 lanes; two such sets share the blocks of 32 columns.
     const int q = warp & 3;
@@ -401,14 +415,19 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       OutT* row0 = static_cast<OutT*>(a.D) + (MODE == GROUPED_GRAD ? tile.g * a.group_stride : 0ll) + tile.col0 * a.ld;
       auto store_elements = [&](int c, const uint32_t (&v)[32]) {
         if (m < a.lanes) {
+          OutT* p = row0 + c * a.ld + m;
+          const int live = tile.ncols - c;
+          float old[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) old[j] = 0.f;
+          if (a.beta != 0.f) {  // all requests under way at once: rows behind the last read that one again
+#pragma unroll
+            for (int j = 0; j < 32; ++j) old[j] = load_c_as_float<OutT>(p, min(j, live - 1) * a.ld);
+          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            if (c + j < tile.ncols) {
-              OutT* p = row0 + (c + j) * a.ld + m;
-              float x = __uint_as_float(v[j]) * a.alpha;
-              if (a.beta != 0.f) x += a.beta * load_c_as_float<OutT>(p, 0);
-              *p = cvt_out<OutT>(x);
-            }
+            const float x = __uint_as_float(v[j]) * a.alpha;
+            if (j < live) p[j * a.ld] = cvt_out<OutT>(a.beta != 0.f ? x + a.beta * old[j] : x);
           }
         }
       };
@@ -459,34 +478,53 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
             if (a.vec_out) {
               // [32 columns][32 lanes] per warp, stored as rows of 128 bytes
               float* sb = reinterpret_cast<float*>(my_epi);
-              __syncwarp();  // the last block's rows have been read
+              const bool add = a.beta == 1.f;  // the memory adds: nothing is read
+              const bool whole = a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols);
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();  // the last block has left
 #pragma unroll
               for (int j = 0; j < 32; ++j) sb[j * 32 + lane] = __uint_as_float(v[j]) * a.alpha;
+              if (whole) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                const int x = l0 + q * 32;
+                if (lane == 0 && x < a.lanes) {
+                  if constexpr (MODE == GROUPED_GRAD) {
+                    if (add) tma_reduce_add_3d(&tmD, sb, x, tile.col0 + c, tile.g);
+                    else tma_store_3d(&tmD, sb, x, tile.col0 + c, tile.g);
+                  } else {
+                    if (add) tma_reduce_add_2d(&tmD, sb, x, tile.col0 + c);
+                    else tma_store_2d(&tmD, sb, x, tile.col0 + c);
+                  }
+                  tma_store_commit();
+                }
+                continue;
+              }
               __syncwarp();
-              const int x = l0 + q * 32 + (lane & 7) * 4;
+              const int x = l0 + q * 32 + (lane & 7) * 4, j0 = lane >> 3;
               float4 w[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const float4*>(sb + (k * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
-              float* p = reinterpret_cast<float*>(row0) + (c + (lane >> 3)) * a.ld + x;
-              const int live = x < a.lanes ? tile.ncols - c - (lane >> 3) : 0;  // rows k * 4 < live are stored
+              for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const float4*>(sb + (k * 4 + j0) * 32 + (lane & 7) * 4);
+              float* p = reinterpret_cast<float*>(row0) + c * a.ld + x;
+              const int live = x < a.lanes ? tile.ncols - c : 0;  // rows k * 4 + j0 < live are stored
               if (x + 4 <= a.lanes) {
+                if (a.beta != 0.f) {
+                  float4 old[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  if (k * 4 < live) {
-                    float4* to = reinterpret_cast<float4*>(p + k * 4 * a.ld);
-                    if (a.beta != 0.f) {
-                      const float4 old = *to;
-                      w[k] = make_float4(w[k].x + a.beta * old.x, w[k].y + a.beta * old.y, w[k].z + a.beta * old.z, w[k].w + a.beta * old.w);
-                    }
-                    *to = w[k];
-                  }
+                  for (int k = 0; k < 8; ++k) old[k] = *reinterpret_cast<const float4*>(p + min(k * 4 + j0, live - 1) * a.ld);
+#pragma unroll
+                  for (int k = 0; k < 8; ++k)
+                    w[k] = make_float4(w[k].x + a.beta * old[k].x, w[k].y + a.beta * old[k].y, w[k].z + a.beta * old[k].z, w[k].w + a.beta * old[k].w);
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (k * 4 + j0 < live) *reinterpret_cast<float4*>(p + (k * 4 + j0) * a.ld) = w[k];
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                  if (k * 4 < live) {
+                  if (k * 4 + j0 < live) {
                     const float e[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-                    float* to = p + k * 4 * a.ld;
+                    float* to = p + (k * 4 + j0) * a.ld;
 #pragma unroll
                     for (int i = 0; i < 3; ++i)
                       if (x + i < a.lanes) to[i] = a.beta != 0.f ? e[i] + a.beta * to[i] : e[i];
@@ -586,7 +624,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     }
   }
 
-  if (!PROMOTE && warp >= 4) tma_store_wait_all<0>();
+  if (warp >= 4) tma_store_wait_all<0>();
 
   // ---------------------------------------------------------------- teardown
   if (*reinterpret_cast<volatile int*>(a.status) != 0) {
@@ -639,9 +677,7 @@ static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, co
     if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, td, a, tiles, stream);
     if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, td, a, tiles, stream);
   }
-  if constexpr (sizeof(OutT) != 4) {
-    if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
-  }
+  if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
   return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, td, a, tiles, stream);
 }
 
@@ -703,8 +739,7 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: B needs a base, a row pitch and a group pitch that are multiples of 16 bytes", who);
   // Columns of a tile: what holds an average group, so that its weight is streamed once.
   const int64_t mean = (R + G - 1) / G;
-  int bt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
-  if (D->dtype == MOYE_F32 && bt > 128) bt = 128;  // the epilogue's registers hold 128 sums a thread
+  const int bt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
   const int ob = dtype_bytes(D->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
@@ -730,9 +765,9 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     return rc;
   if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
   if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, grouped_box_rows(bt), true)) return rc;
-  a.tma_out = a.vec_out && ob == 2;
+  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f);
   if (a.tma_out)
-    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, 64, 32, true)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype, bt);
   if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
@@ -756,7 +791,7 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   if (int rc = check_row_operand(who, "dD", dD)) return rc;
   if ((K > 1 && dB->stride[2] != 1) || (N > 1 && dB->stride[1] < K) || (G > 1 && dB->stride[0] < (N - 1) * dB->stride[1] + K))
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: dB needs contiguous rows, and rows and groups that do not overlap", who);
-  const int bt = N <= 128 || dB->dtype == MOYE_F32 ? 128 : 256;  // Float32: the epilogue's registers hold 128 sums a thread
+  const int bt = N <= 128 ? 128 : 256;
   const int ob = dtype_bytes(dB->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
@@ -787,11 +822,11 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
     if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
     if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
   }
-  a.tma_out = a.vec_out && ob == 2;
+  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f);
   if (a.tma_out) {
     const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
     const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
-    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, 64, 32, true)) return rc;
+    if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
   }
   log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
            (long long)N, (long long)K, A->dtype, bt);
