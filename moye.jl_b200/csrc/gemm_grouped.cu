@@ -33,6 +33,11 @@ constexpr int kMaxGroupedExtent = 1 << 27;  // a sum this long ends well inside 
 enum : int { SITEG_PROD_EMPTY = 161, SITEG_MMA_ACC = 162, SITEG_MMA_FULL = 163, SITEG_EPI_ACC = 164, SITEG_FIX_TAIL = 165, SITEG_RING = 166 };
 enum : int { GROUPED_K_MAJOR = 0, GROUPED_MN_MAJOR = 1, GROUPED_GRAD = 2 };
 
+// Columns of a tile.  The instruction's N and the loads follow the tile's own width, so a group of a few rows pays nothing
+// for the size; narrower tiles for small groups gained at most 2 % (64 groups of 1 to 128 rows, 2048 x 2048) and lost 20 %
+// where groups are uneven and a weight is streamed for each of their tiles.
+constexpr int BT = 256;
+constexpr int kColBox = 32;  // rows of one load of a K-major column operand in a narrow tile
 constexpr int kPromoteBlocks = 8;  // blocks of 64 summed in tensor memory before registers take over
 
 struct GroupedArgs {
@@ -83,7 +88,7 @@ struct TileRing {
 // Deals this CTA's tiles to the ring; one warp.  The groups come 32 at a time, a lane each: clamped borders, tiles, and a
 // prefix over the lanes; the group of a tile is then found with one ballot.  Borders outside the arrays or running
 // backwards are a caller's mistake that must not become a bad address: they are clamped, such groups come out empty.
-template <int MODE, int BT>
+template <int MODE>
 __device__ __forceinline__ void deal_tiles(const GroupedArgs& a, TileRing& ring, int first_tile, int tile_step, int lane) {
   int next = first_tile, before = 0, last = 0;
   bool ok = true;
@@ -188,9 +193,8 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   const T lo = cvt_out<T>(a), hi = cvt_out<T>(b);
   return (uint32_t)(*reinterpret_cast<const uint16_t*>(&lo)) | ((uint32_t)(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
 }
-__host__ __device__ constexpr int grouped_box_rows(int bt) { return bt / 2 < 32 ? bt / 2 : 32; }
 
-template <int MODE, typename OutT, int BT, int STAGES>
+template <int MODE, typename OutT, int STAGES>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmC,
                     const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmD, const GroupedArgs a) {
@@ -205,8 +209,6 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   constexpr bool PROMOTE = sizeof(OutT) == 4;
   constexpr int EPI_BUF = 32 * 128;            // a staging tile: 32 columns of 128 bytes
   constexpr int EPI_BYTES = 8 * EPI_BUF;       // one per epilogue warp (Float32 outputs) or two per pair of them
-  constexpr int C_BOX = grouped_box_rows(BT);  // rows of one load of a K-major column operand
-  static_assert(BT % 32 == 0 && BT <= 256 && (!C_MN || BT >= 128), "tile columns");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -266,138 +268,138 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 
   // Float32 tiles of 256 columns keep 128 sums a thread: the eight epilogue warps take registers over from the other four
   // (4 x 32 x 40 + 8 x 32 x 232 = 12 x 32 x 168).
-  constexpr bool SHIFT_REGS = PROMOTE && BT == 256;
+  constexpr bool SHIFT_REGS = PROMOTE;
   if (warp < 4) {
-  if (SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer (both CTAs)
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t leader_full0 = mapa_shared(smem_u32(&full[0]), 0);
-      while (ok && ring.take(tile)) {
-        ring.leave();
-        const int kbs = tile.k_blocks;
-        const int l0 = tile.lane0 + rank * 128, half = tile.width / 2, c0 = tile.col0 + rank * half;
-        // only the columns that the instruction reads: narrow tiles are bound by these loads
-        const int loads = C_MN ? (half + 63) / 64 : (half + C_BOX - 1) / C_BOX;
-        const bool whole = !C_MN && loads * C_BOX == BT / 2;  // one large box is faster than four small ones
-        const uint32_t bytes = L_BYTES + loads * (C_MN ? BK * 128 : C_BOX * 128);
-        for (int kb = 0; kb < kbs; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, a.status, SITEG_PROD_EMPTY)) { ok = false; break; }
-          uint8_t* sl = smem + stage * STAGE_BYTES;
-          uint8_t* sc = sl + L_BYTES;
-          auto load = [&](auto&& load2, auto&& load3) {
-            if constexpr (MODE == GROUPED_K_MAJOR) {
-              load3(sl, &tmL, kb * BK, l0, tile.g);
-            } else if constexpr (MODE == GROUPED_MN_MAJOR) {
-              for (int c = 0; c < 2; ++c) load3(sl + c * (BK * 128), &tmL, l0 + c * 64, kb * BK, tile.g);
+    if (SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer (both CTAs)
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint32_t leader_full0 = mapa_shared(smem_u32(&full[0]), 0);
+        while (ok && ring.take(tile)) {
+          ring.leave();
+          const int kbs = tile.k_blocks;
+          const int l0 = tile.lane0 + rank * 128, half = tile.width / 2, c0 = tile.col0 + rank * half;
+          // only the columns that the instruction reads: narrow tiles are bound by these loads
+          const int loads = C_MN ? (half + 63) / 64 : (half + kColBox - 1) / kColBox;
+          const bool whole = !C_MN && loads * kColBox == BT / 2;  // one large box is faster than four small ones: 452 us against 479
+          const uint32_t bytes = L_BYTES + loads * (C_MN ? BK * 128 : kColBox * 128);
+          for (int kb = 0; kb < kbs; ++kb) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, a.status, SITEG_PROD_EMPTY)) { ok = false; break; }
+            uint8_t* sl = smem + stage * STAGE_BYTES;
+            uint8_t* sc = sl + L_BYTES;
+            auto load = [&](auto&& load2, auto&& load3) {
+              if constexpr (MODE == GROUPED_K_MAJOR) {
+                load3(sl, &tmL, kb * BK, l0, tile.g);
+              } else if constexpr (MODE == GROUPED_MN_MAJOR) {
+                for (int c = 0; c < 2; ++c) load3(sl + c * (BK * 128), &tmL, l0 + c * 64, kb * BK, tile.g);
+              } else {
+                for (int c = 0; c < 2; ++c) load2(sl + c * (BK * 128), &tmL, l0 + c * 64, tile.row0 + kb * BK);
+              }
+              if constexpr (C_MN) {
+                for (int c = 0; c < loads; ++c) load2(sc + c * (BK * 128), &tmC, c0 + c * 64, tile.row0 + kb * BK);
+              } else if (whole) {
+                load2(sc, &tmC, kb * BK, c0);
+              } else {
+                for (int c = 0; c < loads; ++c) load2(sc + c * (kColBox * 128), &tmN, kb * BK, c0 + c * kColBox);
+              }
+            };
+            const bool cleared = MODE == GROUPED_GRAD && tile.nrows - kb * BK < BK;  // warp 2 passes this block on
+            if (rank == 0 || cleared) {
+              uint64_t* bar = cleared ? &tail[stage] : &full[stage];
+              mbar_arrive_expect_tx(bar, bytes);
+              load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d(d, m, bar, x, y); },
+                   [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d(d, m, bar, x, y, z); });
             } else {
-              for (int c = 0; c < 2; ++c) load2(sl + c * (BK * 128), &tmL, l0 + c * 64, tile.row0 + kb * BK);
+              const uint32_t bar = leader_full0 + stage * 8;
+              mbar_arrive_expect_tx_remote(bar, bytes);
+              load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d_pair(d, m, bar, x, y); },
+                   [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d_pair(d, m, bar, x, y, z); });
             }
-            if constexpr (C_MN) {
-              for (int c = 0; c < loads; ++c) load2(sc + c * (BK * 128), &tmC, c0 + c * 64, tile.row0 + kb * BK);
-            } else if (whole) {
-              load2(sc, &tmC, kb * BK, c0);
-            } else {
-              for (int c = 0; c < loads; ++c) load2(sc + c * (C_BOX * 128), &tmN, kb * BK, c0 + c * C_BOX);
-            }
-          };
-          const bool cleared = MODE == GROUPED_GRAD && tile.nrows - kb * BK < BK;  // warp 2 passes this block on
-          if (rank == 0 || cleared) {
-            uint64_t* bar = cleared ? &tail[stage] : &full[stage];
-            mbar_arrive_expect_tx(bar, bytes);
-            load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d(d, m, bar, x, y); },
-                 [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d(d, m, bar, x, y, z); });
-          } else {
-            const uint32_t bar = leader_full0 + stage * 8;
-            mbar_arrive_expect_tx_remote(bar, bytes);
-            load([&](uint8_t* d, const CUtensorMap* m, int x, int y) { tma_load_2d_pair(d, m, bar, x, y); },
-                 [&](uint8_t* d, const CUtensorMap* m, int x, int y, int z) { tma_load_3d_pair(d, m, bar, x, y, z); });
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (leader CTA only)
-    if (lane == 0 && rank == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int lt = 0;
-      bool ok = true;
-      const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
-      const uint32_t empty_local = smem_u32(&empty[0]), empty_peer = mapa_shared(empty_local, 1);
-      while (ok && ring.take(tile)) {
-        ring.leave();
-        const int kbs = tile.k_blocks;
-        const uint32_t idesc = a.idesc | ((uint32_t)(tile.width >> 3) << 17);
-        for (int seg = 0; seg < kbs && ok; seg += PROMOTE ? kPromoteBlocks : kbs, ++lt) {
-          const int buf = lt & 1, end = PROMOTE ? min(seg + kPromoteBlocks, kbs) : kbs;
-          const uint32_t aphase = (lt >> 1) & 1;
-          ok = mbar_wait(&acc_empty[buf], aphase ^ 1, a.status, SITEG_MMA_ACC);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t d_tmem = tmem_base + buf * BT;
-          for (int kb = seg; kb < end; ++kb) {
-            // a cleared block was written by threads of both CTAs
-            ok = MODE == GROUPED_GRAD ? mbar_wait_cluster(&full[stage], phase, a.status, SITEG_MMA_FULL)
-                                      : mbar_wait(&full[stage], phase, a.status, SITEG_MMA_FULL);
-            if (!ok) break;
-            tc_fence_after_sync();
-            const uint32_t s = smem_u32(smem + stage * STAGE_BYTES);
-            const uint64_t ld = dl.base + (s >> 4), cd = dc.base + ((s + L_BYTES) >> 4);
-#pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)
-              tc_mma_ss2<KIND_F16>(d_tmem, ld + k * dl.kstep, cd + k * dc.kstep, idesc, (kb > seg || k > 0) ? 1u : 0u);
-            tc_commit2(empty_local + stage * 8);
-            tc_commit2(empty_peer + stage * 8);
             if (++stage == STAGES) { stage = 0; phase ^= 1; }
           }
-          if (ok) {
-            const uint32_t f_local = smem_u32(&acc_full[buf]);
-            tc_commit2(f_local);
-            tc_commit2(mapa_shared(f_local, 1));
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer (leader CTA only)
+      if (lane == 0 && rank == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        int lt = 0;
+        bool ok = true;
+        const OperandDesc dl = make_operand_desc<BK, UMMA_K>(L_MN), dc = make_operand_desc<BK, UMMA_K>(C_MN);
+        const uint32_t empty_local = smem_u32(&empty[0]), empty_peer = mapa_shared(empty_local, 1);
+        while (ok && ring.take(tile)) {
+          ring.leave();
+          const int kbs = tile.k_blocks;
+          const uint32_t idesc = a.idesc | ((uint32_t)(tile.width >> 3) << 17);
+          for (int seg = 0; seg < kbs && ok; seg += PROMOTE ? kPromoteBlocks : kbs, ++lt) {
+            const int buf = lt & 1, end = PROMOTE ? min(seg + kPromoteBlocks, kbs) : kbs;
+            const uint32_t aphase = (lt >> 1) & 1;
+            ok = mbar_wait(&acc_empty[buf], aphase ^ 1, a.status, SITEG_MMA_ACC);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t d_tmem = tmem_base + buf * BT;
+            for (int kb = seg; kb < end; ++kb) {
+              // a cleared block was written by threads of both CTAs
+              ok = MODE == GROUPED_GRAD ? mbar_wait_cluster(&full[stage], phase, a.status, SITEG_MMA_FULL)
+                                        : mbar_wait(&full[stage], phase, a.status, SITEG_MMA_FULL);
+              if (!ok) break;
+              tc_fence_after_sync();
+              const uint32_t s = smem_u32(smem + stage * STAGE_BYTES);
+              const uint64_t ld = dl.base + (s >> 4), cd = dc.base + ((s + L_BYTES) >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / UMMA_K; ++k)
+                tc_mma_ss2<KIND_F16>(d_tmem, ld + k * dl.kstep, cd + k * dc.kstep, idesc, (kb > seg || k > 0) ? 1u : 0u);
+              tc_commit2(empty_local + stage * 8);
+              tc_commit2(empty_peer + stage * 8);
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (ok) {
+              const uint32_t f_local = smem_u32(&acc_full[buf]);
+              tc_commit2(f_local);
+              tc_commit2(mapa_shared(f_local, 1));
+            }
           }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // ------------------------------------------------------------ rows behind a group's end (gradient, both CTAs)
-    // The last block of a group reaches into the next group's rows, or past the last one, where anything may lie: those K
-    // rows are zeroed in both operands.  A K row is 128 bytes in every chunk, swizzled within itself.
-    if constexpr (MODE == GROUPED_GRAD) {
-      int pos = 0;            // stages used before this tile
-      uint32_t phases = 0;    // one bit per stage
-      while (__all_sync(~0u, ring.take(tile))) {
-        __syncwarp();
-        if (lane == 0) ring.leave();
-        else ++ring.n;
-        const int kbs = tile.k_blocks, valid = tile.nrows - (kbs - 1) * BK;
-        if (kbs > 0 && valid < BK) {
-          const int stage = (pos + kbs - 1) % STAGES;
-          bool ok = true;
-          if (lane == 0) ok = mbar_wait(&tail[stage], (phases >> stage) & 1, a.status, SITEG_FIX_TAIL);
-          ok = __shfl_sync(~0u, ok, 0);
-          if (!ok) break;
-          phases ^= 1u << stage;
-          uint8_t* sl = smem + stage * STAGE_BYTES;
-          for (int c = 0; c < 2 + (tile.width / 2 + 63) / 64; ++c)
-            for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
-              *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
+      __syncwarp();
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ rows behind a group's end (gradient, both CTAs)
+      // The last block of a group reaches into the next group's rows, or past the last one, where anything may lie: those K
+      // rows are zeroed in both operands.  A K row is 128 bytes in every chunk, swizzled within itself.
+      if constexpr (MODE == GROUPED_GRAD) {
+        int pos = 0;            // stages used before this tile
+        uint32_t phases = 0;    // one bit per stage
+        while (__all_sync(~0u, ring.take(tile))) {
           __syncwarp();
-          if (lane == 0) mbar_arrive_remote_release(mapa_shared(smem_u32(&full[stage]), 0));
+          if (lane == 0) ring.leave();
+          else ++ring.n;
+          const int kbs = tile.k_blocks, valid = tile.nrows - (kbs - 1) * BK;
+          if (kbs > 0 && valid < BK) {
+            const int stage = (pos + kbs - 1) % STAGES;
+            bool ok = true;
+            if (lane == 0) ok = mbar_wait(&tail[stage], (phases >> stage) & 1, a.status, SITEG_FIX_TAIL);
+            ok = __shfl_sync(~0u, ok, 0);
+            if (!ok) break;
+            phases ^= 1u << stage;
+            uint8_t* sl = smem + stage * STAGE_BYTES;
+            for (int c = 0; c < 2 + (tile.width / 2 + 63) / 64; ++c)
+              for (int off = valid * 128 + lane * 16; off < BK * 128; off += 512)
+                *reinterpret_cast<uint4*>(sl + c * (BK * 128) + off) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote_release(mapa_shared(smem_u32(&full[stage]), 0));
+          }
+          pos = (pos + kbs) % STAGES;
         }
-        pos = (pos + kbs) % STAGES;
       }
+    } else if (warp == 3) {
+      // ------------------------------------------------------------ tile scheduler (each CTA for itself, the same tiles)
+      deal_tiles<MODE>(a, ring, first_tile, tile_step, lane);
     }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------ tile scheduler (each CTA for itself, the same tiles)
-    deal_tiles<MODE, BT>(a, ring, first_tile, tile_step, lane);
-  }
   } else {
     if (SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ------------------------------------------------------------ epilogue (warps 4..11, both CTAs)
@@ -642,15 +644,22 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-template <int MODE, typename OutT, int BT>
-static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td, const GroupedArgs& a,
-                               long long tiles, cudaStream_t stream) {
+template <int MODE, typename OutT>
+static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
+                               const GroupedArgs& a, long long tiles, cudaStream_t stream) {
   constexpr int EXTRA = 1024 + 1024 + 8 * 32 * 128;
   constexpr int STAGE = 128 * 128 + BT / 2 * 128;
-  constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE < 12 ? (227 * 1024 - EXTRA) / STAGE : 12;
+  constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE;
   constexpr int SMEM = STAGES * STAGE + EXTRA;
-  auto kern = gemm_grouped_kernel<MODE, OutT, BT, STAGES>;
+  auto kern = gemm_grouped_kernel<MODE, OutT, STAGES>;
   if (int rc = configure_once(h, kern, SMEM)) return rc;
+  if (sizeof(OutT) == 4) {  // what the epilogue takes over has to be there, or it would wait for it
+    static const int regs = [&] {
+      cudaFuncAttributes attr = {};
+      return cudaFuncGetAttributes(&attr, kern) == cudaSuccess ? attr.numRegs : 0;
+    }();
+    if (regs < 168) MOYE_FAIL(MOYE_ERR_CUDA, "the Float32 kernel was built with %d registers a thread, 168 are needed", regs);
+  }
   const long long pairs = tiles < h->num_sms / 2 ? tiles : h->num_sms / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -670,23 +679,12 @@ static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CU
   return MOYE_OK;
 }
 
-template <int MODE, typename OutT>
-static int launch_grouped_bt(int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
-                             const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  if constexpr (MODE != GROUPED_GRAD) {
-    if (bt == 32) return launch_grouped_inst<MODE, OutT, 32>(h, tl, tc, tn, td, a, tiles, stream);
-    if (bt == 64) return launch_grouped_inst<MODE, OutT, 64>(h, tl, tc, tn, td, a, tiles, stream);
-  }
-  if (bt == 256) return launch_grouped_inst<MODE, OutT, 256>(h, tl, tc, tn, td, a, tiles, stream);
-  return launch_grouped_inst<MODE, OutT, 128>(h, tl, tc, tn, td, a, tiles, stream);
-}
-
 template <int MODE>
-static int launch_grouped_out(int out, int bt, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
-                              const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  if (out == MOYE_F32) return launch_grouped_bt<MODE, float>(bt, h, tl, tc, tn, td, a, tiles, stream);
-  if (out == MOYE_F16) return launch_grouped_bt<MODE, __half>(bt, h, tl, tc, tn, td, a, tiles, stream);
-  return launch_grouped_bt<MODE, __nv_bfloat16>(bt, h, tl, tc, tn, td, a, tiles, stream);
+static int launch_grouped(int out, moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
+                          const GroupedArgs& a, long long tiles, cudaStream_t stream) {
+  if (out == MOYE_F32) return launch_grouped_inst<MODE, float>(h, tl, tc, tn, td, a, tiles, stream);
+  if (out == MOYE_F16) return launch_grouped_inst<MODE, __half>(h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped_inst<MODE, __nv_bfloat16>(h, tl, tc, tn, td, a, tiles, stream);
 }
 
 static int check_grouped_types(const char* who, const moye_tensor_t* x, const moye_tensor_t* y, const moye_tensor_t* out) {
@@ -737,9 +735,6 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows or groups of B overlap", who);
   if ((reinterpret_cast<uintptr_t>(B->ptr) & 15) != 0 || (outer > 1 && pitch % 8 != 0) || (G > 1 && B->stride[0] % 8 != 0))
     MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: B needs a base, a row pitch and a group pitch that are multiples of 16 bytes", who);
-  // Columns of a tile: what holds an average group, so that its weight is streamed once.
-  const int64_t mean = (R + G - 1) / G;
-  const int bt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
   const int ob = dtype_bytes(D->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
@@ -756,22 +751,22 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   a.D = D->ptr;
   a.ld = D->stride[0];
   a.status = h->d_status;
-  const long long live = G < R ? G : R, tiles = (live + (R - live) / bt) * a.lane_tiles;  // at most
+  const long long live = G < R ? G : R, tiles = (live + (R - live) / BT) * a.lane_tiles;  // at most
   if (tiles > INT32_MAX / 2) MOYE_FAIL(MOYE_ERR_TOO_LARGE, "%s: too many tiles", who);
   CUtensorMap tl, tc, tn, td;
   std::memset(&td, 0, sizeof(td));
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
                               (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
-  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, bt / 2, true)) return rc;
-  if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, grouped_box_rows(bt), true)) return rc;
+  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, BT / 2, true)) return rc;
+  if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, kColBox, true)) return rc;
   a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f);
   if (a.tma_out)
     if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
-  log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G, (long long)N,
-           (long long)K, A->dtype, bt);
-  if (mn) return launch_grouped_out<GROUPED_MN_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
-  return launch_grouped_out<GROUPED_K_MAJOR>(D->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d", (long long)R, (long long)G, (long long)N,
+           (long long)K, A->dtype);
+  if (mn) return launch_grouped<GROUPED_MN_MAJOR>(D->dtype, h, tl, tc, tn, td, a, tiles, stream);
+  return launch_grouped<GROUPED_K_MAJOR>(D->dtype, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
@@ -791,7 +786,6 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   if (int rc = check_row_operand(who, "dD", dD)) return rc;
   if ((K > 1 && dB->stride[2] != 1) || (N > 1 && dB->stride[1] < K) || (G > 1 && dB->stride[0] < (N - 1) * dB->stride[1] + K))
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: dB needs contiguous rows, and rows and groups that do not overlap", who);
-  const int bt = N <= 128 ? 128 : 256;
   const int ob = dtype_bytes(dB->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
@@ -799,7 +793,7 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   a.lanes = (int)K;
   a.cols = (int)N;
   a.lane_tiles = (int)((K + 255) / 256);
-  a.col_tiles = (int)((N + bt - 1) / bt);
+  a.col_tiles = (int)((N + BT - 1) / BT);
   a.vec_out = (beta == 0.f || ob == 4) && (reinterpret_cast<uintptr_t>(dB->ptr) & 15) == 0 && (N == 1 || (dB->stride[1] * ob) % 16 == 0) &&
               (G == 1 || (dB->stride[0] * ob) % 16 == 0);
   a.offsets = offsets;
@@ -828,9 +822,9 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
     const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;
     if (int rc = encode_tmap_3d(&td, dB->ptr, dB->dtype, K, N, G, row, group, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
   }
-  log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d  -> tiles of 256 x %d", (long long)R, (long long)G,
-           (long long)N, (long long)K, A->dtype, bt);
-  return launch_grouped_out<GROUPED_GRAD>(dB->dtype, bt, h, tl, tc, tn, td, a, tiles, stream);
+  log_line("gemm_grouped_grad %lld rows, %lld groups, %lld x %lld  in %d", (long long)R, (long long)G,
+           (long long)N, (long long)K, A->dtype);
+  return launch_grouped<GROUPED_GRAD>(dB->dtype, h, tl, tc, tn, td, a, tiles, stream);
 }
 
 }  // namespace moye
