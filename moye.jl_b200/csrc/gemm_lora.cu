@@ -15,6 +15,7 @@ namespace moye {
 
 constexpr int kLoraCtas = 8;         // cluster size of the row kernel
 constexpr int kLoraThreads = 256;
+constexpr int kLoraRowChunk = 512;   // columns of a CTA's slice that meet in shared memory before they are stored
 constexpr int kMaxLoraRank = 128;
 
 struct LoraArgs {
@@ -58,9 +59,9 @@ __device__ __forceinline__ float ld_remote_f32(uint32_t cluster_addr) {
 }
 
 template <typename T, typename OutT>
-__global__ void __launch_bounds__(kLoraThreads)
+__global__ void __launch_bounds__(kLoraThreads, 5)
 lora_row_kernel(const LoraArgs g) {
-  __shared__ float part[kMaxLoraRank], v[kMaxLoraRank];
+  __shared__ float part[kMaxLoraRank], v[kMaxLoraRank], out[kLoraRowChunk];
   __shared__ int found;
   griddep_launch();
   griddep_wait();
@@ -87,43 +88,111 @@ lora_row_kernel(const LoraArgs g) {
       for (int n = n0 + tid; n < n1; n += kLoraThreads) d_row[n] = c_row[n];
     return;
   }
+  const T* b_rows = static_cast<const T*>(g.B) + a * g.b_stride;
   {
+    // a warp takes 2 rows of A[a] at a time, two words of 16 bytes of each per lane
     const int kv = g.k / 8, v0 = (int)((long long)kv * rank / kLoraCtas), v1 = (int)((long long)kv * (rank + 1) / kLoraCtas);
     const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(g.X) + row * g.x_pitch);
-    for (int r = warp; r < g.rank; r += kLoraThreads / 32) {
-      const uint4* ar = reinterpret_cast<const uint4*>(static_cast<const T*>(g.A) + a * g.a_stride + r * g.a_pitch);
-      float s = 0.f;
-      for (int i = v0 + lane; i < v1; i += 32) {
-        float xf[8], af[8];
-        lora_unpack<T>(x[i], xf);
-        lora_unpack<T>(ar[i], af);
+    for (int r0 = warp * 2; r0 < g.rank; r0 += kLoraThreads / 16) {  // R is a multiple of 8: both rows exist
+      const T* ar = static_cast<const T*>(g.A) + a * g.a_stride + r0 * g.a_pitch;
+      float s[2] = {0.f, 0.f};
+      for (int i0 = v0; i0 < v1; i0 += 64) {
+        uint4 xw[2], aw[2][2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += xf[e] * af[e];
+        for (int h = 0; h < 2; ++h) {
+          const int i = min(i0 + h * 32 + lane, v1 - 1);
+          xw[h] = x[i];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) aw[r][h] = reinterpret_cast<const uint4*>(ar + r * g.a_pitch)[i];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (i0 + h * 32 + lane >= v1) continue;
+          float xf[8];
+          lora_unpack<T>(xw[h], xf);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float af[8];
+            lora_unpack<T>(aw[r][h], af);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[r] += xf[e] * af[e];
+          }
+        }
       }
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-      if (lane == 0) part[r] = s;
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s[r] += __shfl_xor_sync(~0u, s[r], d);
+        if (lane == 0) part[r0 + r] = s[r];
+      }
     }
   }
   cluster_arrive();
   cluster_wait();  // every CTA's partial vector is in place
-  if (tid < g.rank) {
+  if (tid < kMaxLoraRank) {
     float s = 0.f;
-    for (int c = 0; c < kLoraCtas; ++c) s += ld_remote_f32(mapa_shared(smem_u32(part + tid), c));
-    v[tid] = s * (g.scales ? g.scales[a] : 1.f);
+    if (tid < g.rank) {
+      for (int c = 0; c < kLoraCtas; ++c) s += ld_remote_f32(mapa_shared(smem_u32(part + tid), c));
+      s *= g.scales ? g.scales[a] : 1.f;
+    }
+    v[tid] = s;
   }
   cluster_arrive();  // this CTA has read the others' parts; it leaves only after they have read its own (below)
   __syncthreads();
-  for (int n = n0 + tid; n < n1; n += kLoraThreads) {
-    const uint4* b = reinterpret_cast<const uint4*>(static_cast<const T*>(g.B) + a * g.b_stride + n * g.b_pitch);
-    float s = 0.f;
-    for (int i = 0; i < g.rank / 8; ++i) {
-      float bf[8];
-      lora_unpack<T>(b[i], bf);
+  const int words = g.rank / 8;
+  if (words <= 4) {  // short rows: one per thread (128 requests, R = 16: 8 us against 11 with the rows shared)
+    for (int n = n0 + tid; n < n1; n += kLoraThreads) {
+      const uint4* b = reinterpret_cast<const uint4*>(b_rows + n * g.b_pitch);
+      const float c = lora_load(c_row + n);
+      uint4 w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += bf[e] * v[i * 8 + e];
+      for (int i = 0; i < 4; ++i) w[i] = b[min(i, words - 1)];
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= words) break;
+        float bf[8];
+        lora_unpack<T>(w[i], bf);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += bf[e] * v[i * 8 + e];
+      }
+      lora_store(d_row + n, c + s);
     }
-    lora_store(d_row + n, lora_load(c_row + n) + s);
+    cluster_wait();
+    return;
+  }
+  // long rows: `lanes` neighbouring lanes share one, 16 bytes each, so that a warp reads whole rows, 4 batches of them
+  // under way (128 requests, R = 64: 28 us against 34 with a row per thread)
+  int lanes = 1;
+  while (lanes < words) lanes *= 2;
+  const int sub = lane & (lanes - 1), per_warp = 32 / lanes, mine = lane / lanes;
+  float vf[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) vf[e] = v[sub * 8 + e];
+  for (int c0 = n0; c0 < n1; c0 += kLoraRowChunk) {
+    const int c1 = min(c0 + kLoraRowChunk, n1);
+    // the loop is the warp's, not the lane's: all 32 lanes meet in its shuffles
+    for (int nw = c0 + warp * per_warp; nw < c1; nw += 4 * (kLoraThreads / 32) * per_warp) {
+      const int n = nw + mine;
+      uint4 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        w[u] = reinterpret_cast<const uint4*>(b_rows + min(n + u * (kLoraThreads / 32) * per_warp, c1 - 1) * g.b_pitch)[min(sub, words - 1)];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float bf[8], s = 0.f;
+        lora_unpack<T>(w[u], bf);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += bf[e] * vf[e];
+        if (sub >= words) s = 0.f;
+        for (int d = lanes / 2; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+        const int at = n + u * (kLoraThreads / 32) * per_warp;
+        if (sub == 0 && at < c1) out[at - c0] = s;
+      }
+    }
+    __syncthreads();
+    for (int n = c0 + tid; n < c1; n += kLoraThreads) lora_store(d_row + n, lora_load(c_row + n) + out[n - c0]);
+    __syncthreads();
   }
   cluster_wait();
 }
@@ -835,9 +904,9 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
   g.offsets = offsets;
   g.scales = scales;
   // Requests of several rows share their adapter's factors on the tensor cores.  A row by itself costs its factors' bytes
-  // from L2, about 4.3e-7 us x R (K + N) (2048 rows, R = 16, K = N = 4096: 117 us; R = 64: 416); the tile kernel starts 10 us
-  // later and takes about 3.6e-5 us x (K + N) per tile (256 tiles, R = 16: 93 us; R = 64: 109).  64 requests of 4 / 8 / 16
-  // rows, R = 16: rows 22 / 37 / 64 us, tiles 33 / 35 / 35.
+  // from L2, 3e-7 to 4e-7 us x R (K + N) (512 rows, K = N = 4096: R = 16 28 us, R = 64 86 us); the tile kernel starts
+  // 10 us later and takes about 3.6e-5 us x (K + N) per tile (256 tiles, R = 16: 93 us; R = 64: 109).  64 requests of
+  // 4 / 8 / 16 rows, R = 16: rows 22 / 37 / 64 us, tiles 33 / 35 / 35.
   const double tiles = (double)T / 128 + (requests < T ? requests : T);
   if (offsets && (double)T * R > 84 * tiles + 2.3e7 / (double)(K + N)) {
     auto on16 = [](const moye_tensor_t* t) {
