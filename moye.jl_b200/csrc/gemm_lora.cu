@@ -203,6 +203,7 @@ lora_row_kernel(const LoraArgs g) {
 // the rows in CTA order and handing the result to all; every CTA then multiplies it with its 128-column chunks of B[a] and
 // adds C.  The product of rank R enters the second multiplication as a sum of 16-bit parts: two parts carry 16 (bf16)
 // or 22 (f16) bits, a sixteenth of an output step or less; bf16 operands with a Float32 output take three (24 bits).
+// A Float32 output also has its sums over K taken out of tensor memory every 512 products, as in gemm_grouped.cu.
 // f16 has not the range of the fp32 sums (65504, and steps of 2^-24 near zero): a row is brought to magnitude 1 by a power
 // of two first, which the epilogue takes back.
 //
@@ -333,13 +334,15 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   float* parts = reinterpret_cast<float*>(cboxes);           // before that (C > 1): [128][R] fp32
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bar_off);
   uint64_t *k_full = bars, *k_empty = bars + 12, *b_full = bars + 24, *b_empty = bars + 28, *acc_full = bars + 32, *acc_empty = bars + 34,
-           *v_acc = bars + 36, *p_ready = bars + 37, *v_ready = bars + 38, *c_full = bars + 40;  // c_full[8 warps][c_bufs <= 6]
+           *v_acc = bars + 36, *p_ready = bars + 37, *v_ready = bars + 38, *c_full = bars + 40,  // c_full[8 warps][c_bufs <= 6]
+           *v_full = bars + 88, *v_empty = bars + 90;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 39);
-  int* scratch = reinterpret_cast<int*>(bars + 88);          // 12 warp sums, then the tile
+  int* scratch = reinterpret_cast<int*>(bars + 92);          // 12 warp sums, then the tile
   float* row_max = reinterpret_cast<float*>(bars + 128);     // [2 sets][128 rows]
   float* row_up = row_max + 256;                             // [128 rows]
   constexpr uint32_t TMEM_COLS = 256;
-  constexpr bool RANGE = std::is_same<T, __half>::value;
+  constexpr bool RANGE = std::is_same<T, __half>::value, PROMOTE = sizeof(OutT) == 4;
+  constexpr int RUN = 8;  // K blocks summed in tensor memory
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
@@ -394,6 +397,8 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], turned ? 4 : 8);
+      mbar_init(&v_full[b], 1);
+      mbar_init(&v_empty[b], 8);
     }
     mbar_init(v_acc, 1);
     mbar_init(p_ready, C);
@@ -454,16 +459,23 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(&k_full[stage], phase, p.status, SITEL_MMA_FULL);
-        if (!ok) break;
+      for (int kb = kb0, run = 0; kb < kb1 && ok; ++run) {
+        const int end = PROMOTE ? min(kb + RUN, kb1) : kb1;
+        const uint32_t v_tmem = tmem_base + (run & 1) * 128;
+        ok = mbar_wait(&v_empty[run & 1], ((run >> 1) & 1) ^ 1, p.status, SITEL_MMA_ACC);
         tc_fence_after_sync();
-        const uint32_t s = smem_u32(smem + stage * p.k_bytes);
-        const uint64_t xd = umma_desc_k_sw128(s), ad = umma_desc_k_sw128(s + 128 * 128);
+        for (const int first = kb; kb < end && ok; ++kb) {
+          ok = mbar_wait(&k_full[stage], phase, p.status, SITEL_MMA_FULL);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t s = smem_u32(smem + stage * p.k_bytes);
+          const uint64_t xd = umma_desc_k_sw128(s), ad = umma_desc_k_sw128(s + 128 * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_ss<KIND_F16>(tmem_base, xd + 2 * k, ad + 2 * k, p.idesc1, (kb > kb0 || k > 0) ? 1u : 0u);
-        tc_commit(&k_empty[stage]);
-        if (++stage == p.k_stages) { stage = 0; phase ^= 1; }
+          for (int k = 0; k < 4; ++k) tc_mma_ss<KIND_F16>(v_tmem, xd + 2 * k, ad + 2 * k, p.idesc1, (kb > first || k > 0) ? 1u : 0u);
+          tc_commit(&k_empty[stage]);
+          if (++stage == p.k_stages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) tc_commit(&v_full[run & 1]);
       }
       if (ok) tc_commit(v_acc);
       stage = 0;
@@ -520,25 +532,48 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         store((part * rblocks + (col >> 6)) * (128 * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 4) * 2, w0, w1);
       }
     };
-    bool ok = lora_epi_all(mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
-    if (ok) {
+    // this set's columns of the rank-R product, 16 at a time from 16 set on; those behind R are products with zero rows
+    float sums[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sums[i][j] = 0.f;
+    bool ok = true;
+    for (int kb = kb0, run = 0; kb < kb1 && ok; kb += PROMOTE ? RUN : kb1 - kb0, ++run) {
+      ok = lora_epi_all(mbar_wait(&v_full[run & 1], (run >> 1) & 1, p.status, SITEL_EPI_V));
+      if (!ok) break;
       tc_fence_after_sync();
-      if (C == 1 && lane == 0)
-        for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
-      auto each_16 = [&](auto&& f) {  // this set's columns; those behind R are products with zero rows: zero
-        for (int c = set * 16; c < rsteps * 16; c += 32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (set + 2 * i < rsteps) {
           uint32_t v[16];
-          tmem_ld_x16(t_lane + c, v);
+          tmem_ld_x16(t_lane + (run & 1) * 128 + (set + 2 * i) * 16, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            f(c + j, make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
+          for (int j = 0; j < 16; ++j) sums[i][j] += __uint_as_float(v[j]);
         }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_empty[run & 1]);
+    }
+    // the boxes of C lie where the K blocks did
+    ok = ok && lora_epi_all(mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
+    if (ok) {
+      if (C == 1 && lane == 0)
+        for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
+      auto each_4 = [&](auto&& f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (set + 2 * i < rsteps)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              f((set + 2 * i) * 16 + j, make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]));
       };
       float down = scale, most = 0.f;
       auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))); };
       if (RANGE && C == 1) {
-        each_16([&](int, const float4& x) { largest(x); });
+        each_4([&](int, const float4& x) { largest(x); });
         row_max[set * 128 + my_row] = most;
         lora_epi_all(true);
         float up;
@@ -546,7 +581,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         down *= scale;
         if (set == 0) row_up[my_row] = up;
       }
-      each_16([&](int c, const float4& x) {
+      each_4([&](int c, const float4& x) {
         if (C == 1) {
           write_parts(my_row, c, make_float4(x.x * down, x.y * down, x.z * down, x.w * down),
                       [&](int at, uint32_t w0, uint32_t w1) { *reinterpret_cast<uint2*>(vparts + at) = make_uint2(w0, w1); });
@@ -558,7 +593,6 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         }
       });
       if (RANGE && C > 1) row_max[set * 128 + my_row] = most;
-      tc_fence_before_sync();
       if (C == 1) {
         fence_proxy_async_smem();
         lora_epi_all(true);
