@@ -47,7 +47,7 @@ struct GroupedArgs {
   int k_blocks;         // forward: blocks of 64 along K
   int lane_tiles, col_tiles;
   int vec_out;          // D has a 16-byte base and pitches (and, for 16-bit outputs, beta is 0: one rounding)
-  int tma_out;          // ... and TMA too: beta is 0 (or, for Float32 outputs, 1)
+  int tma_out;          // ... and TMA too: beta is 0 (or, for Float32 outputs, 1), rows are whole 16-byte units
   const int* offsets;
   uint32_t idesc;       // without N
   float alpha, beta;
@@ -760,7 +760,7 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     return rc;
   if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, BT / 2, true)) return rc;
   if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, kColBox, true)) return rc;
-  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f);
+  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f) && (a.lanes * ob) % 16 == 0;  // TMA writes whole 16-byte units, past an odd extent too
   if (a.tma_out)
     if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d", (long long)R, (long long)G, (long long)N,
@@ -816,7 +816,7 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
     if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
     if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
   }
-  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f);
+  a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f) && (a.lanes * ob) % 16 == 0;  // TMA writes whole 16-byte units, past an odd extent too
   if (a.tma_out) {
     const uint64_t row = N > 1 ? (uint64_t)dB->stride[1] * ob : ((uint64_t)K * ob + 15) / 16 * 16;
     const uint64_t group = G > 1 ? (uint64_t)dB->stride[0] * ob : (uint64_t)N * row;

@@ -103,6 +103,12 @@ def _differ():
     raise RuntimeError("operands live on different devices")
 
 
+def _fits(plan, x, what):
+    """The kernels index the plan by the tokens of `x`: an array of another length would reach outside it."""
+    if x.shape[0] != plan.tokens:
+        raise _lib.MoyeError(-4, f"the plan is for {plan.tokens} tokens, {what} has {x.shape[0]} rows")
+
+
 def _call(fn, dev, stream, *args):
     """fn(handle, *args, stream) with device number `dev`, the operands', current."""
     if stream is None:
@@ -150,6 +156,7 @@ def gather_rows_(dst, src, plan, stream=None):
     `combine_rows_(dsrc, ddst, plan)`."""
     td, dev = _arg(dst, 2, "dst")
     ts, d1 = _arg(src, 2, "src")
+    _fits(plan, src, "src")
     if not dev == d1 == plan._at:
         _differ()
     _call(_lib.load().moye_b200_gather_rows, dev, stream, td, ts, plan._pointers()[1], plan.choices)
@@ -162,6 +169,7 @@ def combine_rows_(dst, src, plan, weights=None, stream=None):
     td, dev = _arg(dst, 2, "dst")
     ts, d1 = _arg(src, 2, "src")
     tw, d2 = (None, dev) if weights is None else _arg(weights, 2, "weights")
+    _fits(plan, dst, "dst")
     if not dev == d1 == d2 == plan._at:
         _differ()
     _call(_lib.load().moye_b200_combine_rows, dev, stream, td, ts, tw, plan._pointers()[1], plan.choices)
@@ -177,6 +185,7 @@ def combine_rows_grad_(dsrc, dweights, ddst, src, plan, weights, stream=None):
     t2, d2 = _arg(ddst, 2, "ddst")
     t3, d3 = _arg(src, 2, "src")
     t4, d4 = _arg(weights, 2, "weights")
+    _fits(plan, ddst, "ddst")
     if not dev == d1 == d2 == d3 == d4 == plan._at:
         _differ()
     _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, t0, t1, t2, t3, t4, plan._pointers()[1], plan.choices)

@@ -117,6 +117,73 @@ def test_alpha_beta_and_pitched_views(mb, dev):
     mb.synchronize_status(dev)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("alpha,beta", [(1.0, 1.0), (0.5, 1.0), (1.5, -0.75)])
+def test_adding_to_aligned_outputs(mb, dev, kind, alpha, beta):
+    """beta on rows that vectors and TMA may write: the memory adds, or the old values are read, also at group ends."""
+    offsets, rows, n, k = [0, 40, 40, 300, 333], 340, 264, 200
+    a, b, d = operands(rows, 4, n, k, torch.bfloat16, dev, seed=6)
+    edge = torch.tensor(offsets, dtype=torch.int32, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(7)
+    old, old_b = (torch.randn(*s, generator=gen, device=dev).to(DT[kind]) for s in ((rows, n), (4, n, k)))
+    got = mb.gemm_grouped_(old.clone(), a, b, edge, alpha=alpha, beta=beta)
+    got_b = mb.gemm_grouped_grad_(old_b.clone(), d, a, edge, alpha=alpha, beta=beta)
+    mb.synchronize_status(dev)
+    assert torch.equal(got[333:], old[333:])
+    for g in range(4):
+        s = slice(offsets[g], offsets[g + 1])
+        want = alpha * (a[s].double() @ b[g].double().T) + beta * old[s].double()
+        mag = abs(alpha) * (a[s].double().abs() @ b[g].double().abs().T) + abs(beta) * old[s].double().abs()
+        assert within(got[s], want, mag, k, DT[kind])
+        want = alpha * (d[s].double().T @ a[s].double()) + beta * old_b[g].double()
+        mag = abs(alpha) * (d[s].double().abs().T @ a[s].double().abs()) + abs(beta) * old_b[g].double().abs()
+        assert within(got_b[g], want, mag, offsets[g + 1] - offsets[g], DT[kind])
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_odd_extents_between_padded_pitches(mb, dev, out):
+    """Extents that are no multiple of anything; what lies in the padding (not numbers) is neither read nor written."""
+    offsets, rows, n, k = [0, 5, 70, 333], 333, 131, 203
+    edge = torch.tensor(offsets, dtype=torch.int32, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(8)
+
+    def padded(*shape):
+        x = torch.full((*shape[:-1], (shape[-1] + 15) // 8 * 8), float("nan"), dtype=torch.bfloat16, device=dev)
+        x[..., :shape[-1]] = torch.randn(*shape, generator=gen, device=dev)
+        return x[..., :shape[-1]]
+
+    a, b, d, bt = padded(rows, k), padded(3, n, k), padded(rows, n), padded(3, k, n)
+    for x, w, width in ((a, b, n), (a, bt.transpose(1, 2), n), (d, b.transpose(1, 2), k)):
+        big = torch.full((rows, (width + 15) // 8 * 8), 9.0, dtype=DT[out], device=dev)
+        got = mb.gemm_grouped_(big[:, :width], x, w, edge)
+        for g in range(3):
+            s = slice(offsets[g], offsets[g + 1])
+            assert within(got[s], x[s].double() @ w[g].double().T, x[s].double().abs() @ w[g].double().abs().T, x.shape[1], DT[out])
+        assert bool((big[:, width:] == 9).all())
+    big = torch.full((3, n, (k + 15) // 8 * 8), 9.0, dtype=DT[out], device=dev)
+    got = mb.gemm_grouped_grad_(big[:, :, :k], d, a, edge)
+    for g in range(3):
+        s = slice(offsets[g], offsets[g + 1])
+        assert within(got[g], d[s].double().T @ a[s].double(), d[s].double().abs().T @ a[s].double().abs(), offsets[g + 1] - offsets[g], DT[out])
+    assert bool((big[:, :, k:] == 9).all())
+    mb.synchronize_status(dev)
+
+
+def test_a_group_longer_than_many_tiles(mb, dev):
+    """9 row tiles (a full band of 8 and one more) and a sum over 2100 rows."""
+    offsets, rows, n, k = [0, 2100, 2110], 2110, 520, 136
+    a, b, d = operands(rows, 2, n, k, torch.bfloat16, dev, seed=9)
+    edge = torch.tensor(offsets, dtype=torch.int32, device=dev)
+    for ot in (torch.bfloat16, torch.float32):
+        got = mb.gemm_grouped_(torch.empty(rows, n, dtype=ot, device=dev), a, b, edge)
+        grad = mb.gemm_grouped_grad_(torch.empty(2, n, k, dtype=ot, device=dev), d, a, edge)
+        for g in range(2):
+            s = slice(offsets[g], offsets[g + 1])
+            assert within(got[s], a[s].double() @ b[g].double().T, a[s].double().abs() @ b[g].double().abs().T, k, ot)
+            assert within(grad[g], d[s].double().T @ a[s].double(), d[s].double().abs().T @ a[s].double().abs(), offsets[g + 1] - offsets[g], ot)
+    mb.synchronize_status(dev)
+
+
 def test_neighbours_do_not_leak(mb, dev):
     """A group of infinities beside an ordinary one: neither the rows' products nor the weights' gradients mix."""
     edge = torch.tensor([0, 5, 9, 100], dtype=torch.int32, device=dev)

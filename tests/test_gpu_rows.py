@@ -239,6 +239,11 @@ def test_refusals(mb, dev):
     refused(-4, mb.gather_rows_, f(8, 16), f(4, 8), plan)
     refused(-2, mb.gather_rows_, f(8, 16), f(4, 16, dtype=torch.float32), plan)
     refused(-3, mb.gather_rows_, f(16, 8).t(), f(4, 16), plan)        # rows of dst are not contiguous
+    for n in (3, 5):                                                   # not the plan's tokens
+        refused(-4, mb.gather_rows_, f(2 * n, 16), f(n, 16), plan)
+        refused(-4, mb.combine_rows_, f(n, 16), f(2 * n, 16), plan)
+        wn = torch.zeros(n, 2, device=dev)
+        refused(-4, mb.combine_rows_grad_, f(2 * n, 16), wn, f(n, 16), f(2 * n, 16), plan, wn)
     both = f(8, 16)
     refused(-1, mb.gather_rows_, both, both[4:], plan)                # overlap
     refused(-1, mb.combine_rows_, both[:4], both, plan)
