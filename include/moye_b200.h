@@ -284,9 +284,10 @@ int moye_b200_axpby(moye_handle_t h, const moye_tensor_t* Y, const moye_tensor_t
 /* ---- rows that choose their own weights: rows sorted by group, products of row groups, low-rank adapters --------
  * None of these has a counterpart in the reference.  Whole numbers are int32 device arrays, contiguous.  Numbers read
  * on the device (choices, borders, adapter numbers) may hold anything: what is out of range is skipped as described,
- * never followed. */
+ * never followed.  Outputs must not overlap inputs.  None of the calls keeps scratch: they run side by side on several
+ * streams, and a captured call follows new values in the same arrays. */
 
-/* Sorts the choices of `tokens` rows by group, on the device, stably and without atomics between runs' results.
+/* Sorts the choices of `tokens` rows by group, on the device and stably: the same ids give the same order every time.
  * ids (tokens) or (tokens, choices), 32- or 64-bit integers (MOYE_S32 / MOYE_U64 read as signed), any strides; the
  * choice j of token t is entry t * choices + j.  An id outside 0..groups-1 is dropped.  groups <= 1024.
  *   order[p]    the entry at sorted position p; -1 from offsets[groups] on           (tokens * choices)
@@ -315,8 +316,8 @@ int moye_b200_combine_rows_grad(moye_handle_t h, const moye_tensor_t* dsrc, cons
 
 /* D[i] = alpha * A[i] . B[g]^T + beta * D[i] for the rows offsets[g] <= i < offsets[g+1]; other rows of D are left as
  * they were, and D is not read when beta == 0.  A (rows, K), B (groups, N, K), D (rows, N); offsets: groups + 1 borders
- * on the device, not decreasing (clamped to the rows; a border that runs backwards makes an empty group); groups <= 1024.
- * f16 or bf16 operands, fp32 accumulation, D f32 or the operands' type.  A: contiguous rows; B: unit stride along K, or
+ * on the device, not decreasing (clamped to the rows; a border that runs backwards makes an empty group); groups <= 1024,
+ * extents up to 2^27.  f16 or bf16 operands, fp32 accumulation, D f32 or the operands' type.  A: contiguous rows; B: unit stride along K, or
  * along N (the swapped view of a (groups, K, N) array: dA = dD . B, the gradient of A); base and pitches of A and B
  * multiples of 16 bytes.  D: contiguous rows, any pitch. */
 int moye_b200_gemm_grouped(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* A, const moye_tensor_t* B,
@@ -333,7 +334,8 @@ int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const 
  * is the request with offsets[q] <= i < offsets[q+1] (borders not decreasing), or q = i when offsets is NULL (then
  * requests = rows).  X (rows, K), A (count, R, K), B (count, N, R), C and D (rows, N).  An adapter number outside
  * 0..count-1 means none: D[i] = C[i].  Rows outside every request are left as they were.  C NULL or C = D: in place.
- * scales: one float per adapter, or NULL for 1.  The product of rank R stays in fp32 or an equivalent split.  X, A, B
+ * scales: one float per adapter, or NULL for 1.  The product of rank R is kept in fp32, or as a sum of 16-bit parts that
+ * carries 16 bits or more of it (24 for bf16 with f32 outputs; f16 relative to the row's largest).  X, A, B
  * all f16 or all bf16; C and D both f32 or both the operands' type; R a multiple of 8 from 8 to 128 (pad with zeros),
  * K a multiple of 8; base and pitches of X, A, B multiples of 16 bytes. */
 int moye_b200_gemm_lora(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* X, const moye_tensor_t* A,

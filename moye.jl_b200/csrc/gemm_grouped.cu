@@ -95,7 +95,10 @@ __device__ __forceinline__ void deal_tiles(const GroupedArgs& a, TileRing& ring,
   auto deal = [&](const GroupedTile& t) {
     if (lane == 0) {
       const int slot = ring.n % kTileRing;
-      ok = mbar_wait(&ring.empty[slot], ((ring.n / kTileRing) & 1) ^ 1, a.status, SITEG_RING);
+      // debug build: a tile inside the arrays, columns inside the accumulator
+      ok = MOYE_DBG_OK(t.k_blocks < 0 || (t.row0 >= 0 && t.nrows >= 0 && t.row0 + t.nrows <= a.rows && t.lane0 >= 0 && t.lane0 < a.lanes &&
+                                          t.ncols > 0 && t.width <= BT && t.g < a.groups), a.status, 983) &&
+           mbar_wait(&ring.empty[slot], ((ring.n / kTileRing) & 1) ^ 1, a.status, SITEG_RING);
       if (ok) {
         ring.slots[slot] = t;
         mbar_arrive(&ring.full[slot]);

@@ -350,6 +350,8 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   lora_find_tile(g, blockIdx.x / C, scratch, scratch + 12);
   const int q = scratch[12], row0 = scratch[13], nrows = scratch[14];
   if (q < 0) return;  // fewer tiles than clusters; the same in the whole cluster
+  // debug build: a tile inside the arrays
+  if (!MOYE_DBG_OK(q < g.requests && row0 >= 0 && nrows > 0 && nrows <= 128 && row0 + nrows <= g.rows, p.status, 984)) return;
   const int a = g.which[q];
   const int chunks = (g.n + 127) / 128, kbs = (g.k + 63) / 64;
   const int ch0 = chunks * rank / C, ch1 = chunks * (rank + 1) / C;
@@ -532,7 +534,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         store((part * rblocks + (col >> 6)) * (128 * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 4) * 2, w0, w1);
       }
     };
-    // this set's columns of the rank-R product, 16 at a time from 16 set on; those behind R are products with zero rows
+    // this set's columns of the rank-R product, 16 at a time from 16 set on
     float sums[4][16];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -557,6 +559,12 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_empty[run & 1]);
     }
+    // A rank that ends inside 16 columns: the products with rows of zeros behind it, undefined where X is infinite, are zero
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((set + 2 * i) * 16 + 8 == g.rank)
+#pragma unroll
+        for (int j = 8; j < 16; ++j) sums[i][j] = 0.f;
     // the boxes of C lie where the K blocks did
     ok = ok && lora_epi_all(mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
     if (ok) {

@@ -197,7 +197,30 @@ int launch_group_rows(moye_b200_ctx* h, const moye_tensor_t* ids, int groups, in
   const int smem = (kGroupWarps + 2) * groups * 4;
   if (int rc = configure_once(h, group_rows_kernel, (kGroupWarps + 2) * kMaxGroups * 4)) return rc;
   cudaLaunchConfig_t cfg = {};
-  const unsigned ctas = n > 4096 ? 8 : 1;
+  // One CTA while its warps have at most 4 batches of 32 choices each, then 8; beyond 32768 choices 16, if the device holds
+  // a cluster of 16 (131072 choices, 128 groups: 8 CTAs are bound by their own instructions)
+  unsigned ctas = n > 4096 ? 8 : 1;
+  if (n > 32768) {
+    static const bool holds_16 = [] {
+      int clusters = 0;
+      cudaLaunchConfig_t probe = {};
+      probe.gridDim = dim3(16);
+      probe.blockDim = dim3(kGroupThreads);
+      probe.dynamicSmemBytes = (kGroupWarps + 2) * kMaxGroups * 4;
+      cudaLaunchAttribute size[1];
+      size[0].id = cudaLaunchAttributeClusterDimension;
+      size[0].val.clusterDim.x = 16;
+      size[0].val.clusterDim.y = 1;
+      size[0].val.clusterDim.z = 1;
+      probe.attrs = size;
+      probe.numAttrs = 1;
+      const bool ok = cudaFuncSetAttribute(group_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                      cudaOccupancyMaxActiveClusters(&clusters, group_rows_kernel, &probe) == cudaSuccess && clusters > 0;
+      if (!ok) (void)cudaGetLastError();
+      return ok;
+    }();
+    if (holds_16) ctas = 16;
+  }
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kGroupThreads);
   cfg.dynamicSmemBytes = smem;

@@ -131,6 +131,78 @@ function MoYe.axpby!(a::Number, X::MoYeArray{T, N, ViewEngine{T, CuPtr{T}}}, b::
     return Y
 end
 
+# ---- rows that choose their own weights.  Rows are columns in Julia's storage order: an array of the C ABI that is
+# (rows, width) with contiguous rows is a CuMatrix (width, rows) here, and rank-3 weights (groups, N, K) a CuArray (K, N, groups).
+function row_tensor(x::CuArray{T}) where {T}
+    d = ndims(x)
+    sh, st = reverse(size(x)), reverse(strides(x))
+    MoyeTensor(Ptr{Cvoid}(UInt(pointer(x))), moye_dtype(T), Int32(d),
+               ntuple(i -> i <= d ? Int64(sh[i]) : Int64(0), 4), ntuple(i -> i <= d ? Int64(st[i]) : Int64(0), 4))
+end
+moye_dtype(::Type{Int64}) = Int32(9)
+dptr(x) = x === nothing ? C_NULL : Ptr{Cvoid}(UInt(pointer(x)))
+"Sorted order of (choices, tokens) group numbers, counted from 0; numbers outside 0:groups-1 are dropped."
+struct RowGroups
+    order::CuVector{Int32}; offsets::CuVector{Int32}; inverse::CuMatrix{Int32}; groups::Int
+end
+function group_rows(ids::CuMatrix{<:Union{Int32, Int64}}, groups::Integer; stream = CUDA.stream())
+    p = RowGroups(CuVector{Int32}(undef, length(ids)), CuVector{Int32}(undef, groups + 1), CuMatrix{Int32}(undef, size(ids)), groups)
+    check(ccall((:moye_b200_group_rows, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(ids)), Int32(groups), dptr(p.order), dptr(p.offsets), dptr(p.inverse), stream.handle))
+    return p
+end
+function gather_rows!(dst::CuMatrix, src::CuMatrix, p::RowGroups; stream = CUDA.stream())
+    size(src, 2) == size(p.inverse, 2) || error("the plan is for another number of tokens")
+    check(ccall((:moye_b200_gather_rows, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Int32, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(dst)), Ref(row_tensor(src)), dptr(p.inverse), Int32(size(p.inverse, 1)), stream.handle))
+    return dst
+end
+function combine_rows!(dst::CuMatrix, src::CuMatrix, p::RowGroups, weights::Union{CuMatrix, Nothing} = nothing; stream = CUDA.stream())
+    size(dst, 2) == size(p.inverse, 2) || error("the plan is for another number of tokens")
+    tW = weights === nothing ? C_NULL : Ref(row_tensor(weights))
+    check(ccall((:moye_b200_combine_rows, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(dst)), Ref(row_tensor(src)), tW, dptr(p.inverse), Int32(size(p.inverse, 1)), stream.handle))
+    return dst
+end
+function combine_rows_grad!(dsrc::CuMatrix, dweights::CuMatrix, ddst::CuMatrix, src::CuMatrix, p::RowGroups, weights::CuMatrix;
+                            stream = CUDA.stream())
+    size(ddst, 2) == size(p.inverse, 2) || error("the plan is for another number of tokens")
+    check(ccall((:moye_b200_combine_rows_grad, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Int32, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(dsrc)), Ref(row_tensor(dweights)), Ref(row_tensor(ddst)), Ref(row_tensor(src)),
+                Ref(row_tensor(weights)), dptr(p.inverse), Int32(size(p.inverse, 1)), stream.handle))
+    return dsrc, dweights
+end
+function gemm_grouped!(D::CuMatrix, A::CuMatrix, B::CuArray{T, 3} where {T}, offsets::CuVector{Int32}; alpha = 1, beta = 0, stream = CUDA.stream())
+    length(offsets) == size(B, 3) + 1 || error("one border more than groups")
+    check(ccall((:moye_b200_gemm_grouped, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Cfloat, Cfloat, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(D)), Ref(row_tensor(A)), Ref(row_tensor(B)), dptr(offsets), Float32(alpha), Float32(beta), stream.handle))
+    return D
+end
+function gemm_grouped_grad!(dB::CuArray{T, 3} where {T}, dD::CuMatrix, A::CuMatrix, offsets::CuVector{Int32}; alpha = 1, beta = 0, stream = CUDA.stream())
+    length(offsets) == size(dB, 3) + 1 || error("one border more than groups")
+    check(ccall((:moye_b200_gemm_grouped_grad, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Cfloat, Cfloat, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(dB)), Ref(row_tensor(dD)), Ref(row_tensor(A)), dptr(offsets), Float32(alpha), Float32(beta), stream.handle))
+    return dB
+end
+"D += scales[a] * (X A[a]') B[a]' for the rows of every request, in place behind the shared projection."
+function gemm_lora!(D::CuMatrix, X::CuMatrix, A::CuArray{T, 3}, B::CuArray{T, 3}, adapters::CuVector{Int32},
+                    offsets::Union{CuVector{Int32}, Nothing} = nothing; scales::Union{CuVector{Float32}, Nothing} = nothing,
+                    stream = CUDA.stream()) where {T}
+    (offsets === nothing || length(offsets) == length(adapters) + 1) || error("one border more than requests")
+    (scales === nothing || length(scales) == size(A, 3)) || error("one scale per adapter")
+    check(ccall((:moye_b200_gemm_lora, libmoye_b200[]), Cint,
+                (Ptr{Cvoid}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ref{MoyeTensor}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Ptr{Cvoid}),
+                handle(), Ref(row_tensor(D)), Ref(row_tensor(X)), Ref(row_tensor(A)), Ref(row_tensor(B)), C_NULL, dptr(adapters),
+                dptr(offsets), Int32(length(adapters)), dptr(scales), stream.handle))
+    return D
+end
+
 # ---- Swizzle{B,M,S}: the XOR functor MoYe's README lists as missing (README.md:14-17); composes with a layout
 struct Swizzle{B, M, S} end
 Swizzle(b::Int, m::Int, s::Int) = Swizzle{b, m, s}()

@@ -335,3 +335,51 @@ def test_a_layer_of_experts(mb, dev):
         err = (got.double() - want).abs()
         assert float(err.square().mean().sqrt() / rms) < 6 * 2.0 ** -9
         assert float(err.max() / rms) < 36 * 2.0 ** -9 + float(want.abs().max() / rms) * 2.0 ** -8
+
+
+def test_two_streams_at_once(mb, dev):
+    """The operators of two streams share no scratch: run beside one another they give what they give alone."""
+    def make(seed):
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        r = lambda *s, scale=1.0: (torch.randn(*s, generator=gen, device=dev) * scale).to(torch.bfloat16)
+        ids = torch.randint(0, 6, (700, 2), generator=gen, device=dev)
+        return {"ids": ids, "x": r(700, 256), "w": r(6, 512, 256, scale=1 / 16), "a": r(3, 16, 512, scale=1 / 16), "b": r(3, 256, 16),
+                "which": torch.arange(7, dtype=torch.int32, device=dev) % 4, "edge": (torch.arange(8, device=dev) * 200).int(), "weights": torch.rand(700, 2, generator=gen, device=dev)}
+
+    def step(s):
+        plan = mb.group_rows(s["ids"], 6)
+        xs = mb.gather_rows_(torch.zeros(1400, 256, dtype=torch.bfloat16, device=dev), s["x"], plan)
+        h = mb.gemm_grouped_(torch.zeros(1400, 512, dtype=torch.bfloat16, device=dev), xs, s["w"], plan)
+        g = mb.gemm_grouped_grad_(torch.zeros(6, 512, 256, device=dev), h, xs, plan)
+        y = mb.gemm_lora_(torch.zeros(1400, 256, dtype=torch.bfloat16, device=dev), h, s["a"], s["b"], s["which"], s["edge"])
+        return plan.order, h, g, y, mb.combine_rows_(torch.zeros(700, 256, dtype=torch.bfloat16, device=dev), y, plan, s["weights"])
+
+    states = [make(31), make(32)]
+    alone = [step(s) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(states[i]))
+    torch.cuda.synchronize()
+    mb.synchronize_status(dev)
+    for i in (0, 1):
+        for out in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(out, alone[i]))
+
+
+def test_under_the_debug_build(dev):
+    """The debug library checks every tile against the arrays on the device: the small tests pass under it unchanged."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    res = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-k",
+                          "(test_grouped_product and 5-bf16) or (test_weight_gradient and 5-f16) or (test_lora_tiles and 0-bf16) or clamped or no_rows",
+                          os.path.join(here, "test_gpu_grouped.py"), os.path.join(here, "test_gpu_lora.py")], capture_output=True, text=True,
+                         env=dict(os.environ, MOYE_B200_DEBUG="1"), timeout=600)
+    assert res.returncode == 0 and " passed" in res.stdout, res.stdout[-3000:] + res.stderr[-1000:]

@@ -69,6 +69,43 @@ def test_lora(mb, dev, case, kind, out):
     mb.synchronize_status(dev)
 
 
+# sizes at which requests share their factors on the tensor cores: tiles of 1 to 128 rows in one launch, turned (up to 32
+# rows) and not, a cluster of CTAs per tile and one CTA per tile, outputs that TMA can and cannot write, every part of R
+TILES = [
+    ([0, 1, 3, 20, 52, 85, 213, 341, 800], 805, [3, 0, 1, -1, 2, 3, 9, 0], 1001, 520, 64, 4),
+    ([2, 3, 20, 52, 85, 213, 341, 800], 800, [0, 1, 2, 2, 3, -1, 1], 1000, 520, 72, 4),
+    ([0, 3000], 3000, [0], 520, 136, 128, 1),
+    ([0, 4000, 4000, 4001], 4001, [1, 0, 0], 264, 4096, 8, 2),
+    (list(range(0, 8001, 40)), 8000, [i % 4 for i in range(200)], 264, 200, 24, 3),
+    (list(range(0, 1537, 32)), 1536, [i % 5 for i in range(48)], 131, 1032, 48, 5),
+]
+
+
+@pytest.mark.parametrize("out", ["same", "f32"])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(TILES)))
+def test_lora_tiles(mb, dev, case, kind, out):
+    offsets, rows, which, n, k, rank, count = TILES[case]
+    ot = DT[kind] if out == "same" else torch.float32
+    x, a, b, scales, w, edge = make(TILES[case], kind, dev)
+    x[:offsets[0]], x[offsets[-1]:] = float("nan"), float("inf")
+    c = torch.randn(rows, n + 9, device=dev).to(ot)[:, :n]
+    if n % 8 == 0:
+        c = c.contiguous()
+    d0 = torch.full((rows, n), -3.0, device=dev).to(ot)
+    d = d0.clone()
+    mb.gemm_lora_(d, x, a, b, w, edge, scales=scales, C=c)
+    mb.synchronize_status(dev)
+    check(d, c, x, a, b, scales, which, offsets, ot, d0)
+    wide = torch.full((rows, n + 24), 5.0, device=dev).to(ot)
+    inplace = wide[:, 8:8 + n]
+    inplace.copy_(c)
+    mb.gemm_lora_(inplace, x, a, b, w, edge)
+    check(inplace, c, x, a, b, None, which, offsets, ot, c)
+    assert bool((wide[:, :8] == 5).all()) and bool((wide[:, 8 + n:] == 5).all())
+    mb.synchronize_status(dev)
+
+
 def test_pitched_views_and_moye_arrays(mb, dev):
     offsets, which, n, k, rank = [0, 5, 200], [1, 0], 100, 64, 16
     gen = torch.Generator(device=dev).manual_seed(3)
@@ -93,7 +130,7 @@ def test_infinities_stay_in_their_rows(mb, dev):
 
 
 @pytest.mark.parametrize("size", [1e-6, 3e5])
-@pytest.mark.parametrize("offsets", [[0, 300], [0, 20], [0, 1, 2], list(range(0, 40 * 200, 40))])
+@pytest.mark.parametrize("offsets", [[0, 3000], [0, 20], [0, 1, 2], list(range(0, 40 * 200, 40)), list(range(0, 30 * 160, 30))])
 def test_the_range_of_f16(mb, dev, offsets, size):
     """The product of rank R may leave the range of f16 (65504; steps of 2^-24 near zero) where the operands and the result
     do not: its 16-bit parts are taken relative to the row's largest."""
@@ -114,13 +151,13 @@ def test_the_range_of_f16(mb, dev, offsets, size):
 def test_an_infinity_stays_one(mb, dev):
     """One infinite product of rank R: the outputs it reaches are infinite, not undefined."""
     for kind in ("f16", "bf16"):
-        for rows in (1, 20, 300):
-            x, a, b = torch.ones(rows, 64, device=dev).to(DT[kind]), torch.zeros(1, 8, 64, device=dev).to(DT[kind]), torch.ones(1, 40, 8, device=dev).to(DT[kind])
+        for rows, k, n in ((1, 64, 40), (20, 64, 40), (300, 64, 40), (6000, 512, 264)):
+            x, a, b = torch.ones(rows, k, device=dev).to(DT[kind]), torch.zeros(1, 8, k, device=dev).to(DT[kind]), torch.ones(1, n, 8, device=dev).to(DT[kind])
             x[rows // 2, 0] = float("inf")
             a[0, 3, 0] = 1.0
             a[0, 3, 1] = 1.0
             x[:, 2:] = 0
-            d = mb.gemm_lora_(torch.zeros(rows, 40, device=dev), x, a[:, 3:4].expand(1, 8, 64).contiguous(), b, torch.zeros(1, dtype=torch.int32, device=dev),
+            d = mb.gemm_lora_(torch.zeros(rows, n, device=dev), x, a[:, 3:4].expand(1, 8, k).contiguous(), b, torch.zeros(1, dtype=torch.int32, device=dev),
                               torch.tensor([0, rows], dtype=torch.int32, device=dev))
             assert bool((d[rows // 2] == float("inf")).all()) and int((~d.isfinite()).any(1).sum()) == 1
 
@@ -157,9 +194,9 @@ def test_beside_a_projection_captured(mb, dev):
 
 
 def test_same_bits_every_time(mb, dev):
-    for case in (1, 3, 7):
-        x, a, b, scales, w, edge = make(CASES[case], "bf16", dev)
-        rows, n = CASES[case][1], CASES[case][3]
+    for case in (CASES[1], CASES[3], TILES[0], TILES[2], TILES[5]):
+        x, a, b, scales, w, edge = make(case, "bf16", dev)
+        rows, n = case[1], case[3]
         outs = [mb.gemm_lora_(torch.zeros(rows, n, device=dev), x, a, b, w, edge, scales) for _ in range(3)]
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
