@@ -14,6 +14,9 @@ the operands' device or on `stream`, a violation raises `MoyeError`, nothing fal
 borders, choices and adapter numbers stay on the device: no call waits for the GPU, and a captured call follows new
 values in the same arrays.  The reference has no counterpart.
 """
+import struct
+import threading
+
 import torch
 
 from . import _lib
@@ -26,6 +29,8 @@ __all__ = ["RowGroups", "group_rows", "group_rows_", "gather_rows_", "combine_ro
 
 # the stream's handle alone: a torch Stream object costs 2 us a call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_thread = threading.get_ident
 _PACK = _lib.TENSOR_PACKERS
 _INT32, _FLOAT32 = torch.int32, torch.float32
 
@@ -67,10 +72,13 @@ class RowGroups:
 def _arg(x, rank, what):
     """(descriptor bytes, device index) of a rank-`rank` device array."""
     if isinstance(x, torch.Tensor):
-        dev, dtype = x.get_device(), TORCH_TO_MOYE.get(x.dtype)
-        if dev >= 0 and dtype is not None and x.dim() == rank:
-            return _PACK[rank].pack(x.data_ptr(), dtype, rank, *x.shape, *x.stride()), dev
-        shape, where = tuple(x.shape), x.device
+        dev = x.get_device()
+        if dev >= 0:
+            try:
+                return _PACK[rank].pack(x.data_ptr(), TORCH_TO_MOYE[x.dtype], rank, *x.shape, *x.stride()), dev
+            except (KeyError, struct.error):  # a type that has no counterpart, another rank: said below
+                pass
+        shape, where, dtype = tuple(x.shape), x.device, TORCH_TO_MOYE.get(x.dtype)
     elif isinstance(x, MoYeArray):
         l = x.layout
         modes = [coalesce(l[i]) for i in range(len(l))] if len(l) > 1 else [coalesce(l)]
@@ -113,11 +121,12 @@ def _call(fn, dev, stream, *args):
     """fn(handle, *args, stream) with device number `dev`, the operands', current."""
     if stream is None:
         stream = _raw_stream(dev)
-    if torch.cuda.current_device() == dev:
-        rc = fn(_lib.handle(dev), *args, stream)
+    handle = _lib._handles.get((_thread(), dev)) or _lib.handle(dev)
+    if _current_device() == dev:
+        rc = fn(handle, *args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(_lib.handle(dev), *args, stream)
+            rc = fn(handle, *args, stream)
     if rc:
         _lib.check(rc)
 
@@ -214,7 +223,7 @@ def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
     tb, d2 = _arg(B, 3, "B")
     if not dev == d1 == d2:
         _differ()
-    _call(_lib.load().moye_b200_gemm_grouped, dev, stream, td, ta, tb, _borders(offsets, int(B.shape[0]), dev), alpha, beta)
+    _call(_lib.load().moye_b200_gemm_grouped, dev, stream, td, ta, tb, _borders(offsets, int(B.shape[0]), dev), float(alpha), float(beta))
     return D
 
 
@@ -226,7 +235,7 @@ def gemm_grouped_grad_(dB, dD, A, offsets, alpha=1.0, beta=0.0, stream=None):
     ta, d2 = _arg(A, 2, "A")
     if not dev == d1 == d2:
         _differ()
-    _call(_lib.load().moye_b200_gemm_grouped_grad, dev, stream, tb, td, ta, _borders(offsets, int(dB.shape[0]), dev), alpha, beta)
+    _call(_lib.load().moye_b200_gemm_grouped_grad, dev, stream, tb, td, ta, _borders(offsets, int(dB.shape[0]), dev), float(alpha), float(beta))
     return dB
 
 

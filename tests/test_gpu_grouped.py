@@ -95,7 +95,7 @@ def test_alpha_beta_and_pitched_views(mb, dev):
     for alpha, beta in ((0.5, 1.0), (-2.0, 0.25)):
         big = base.clone()
         got = big[:, 3:3 + n]                                        # rows of D on no 16-byte boundary
-        mb.gemm_grouped_(mb.MoYeArray(got), mb.MoYeArray(a), b, edge, alpha=alpha, beta=beta)
+        mb.gemm_grouped_(mb.MoYeArray(got), mb.MoYeArray(a), mb.MoYeArray(b), edge, alpha=alpha, beta=beta)
         old = base[:, 3:3 + n].double()
         for g in range(3):
             s = slice(offsets[g], offsets[g + 1])

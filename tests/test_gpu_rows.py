@@ -49,7 +49,7 @@ def data(tokens, choices, width, dtype, dev, seed=3):
 
 
 @pytest.mark.parametrize("id_type", [torch.int32, torch.int64])
-@pytest.mark.parametrize("tokens,choices,groups", [(0, 2, 5), (1, 1, 1), (31, 3, 4), (4096, 1, 64), (4097, 1, 64), (700, 9, 1024), (20000, 8, 128)])
+@pytest.mark.parametrize("tokens,choices,groups", [(0, 2, 5), (1, 1, 1), (31, 3, 4), (4096, 1, 64), (4097, 1, 64), (700, 9, 1024), (20000, 8, 128), (33000, 1, 1024)])
 def test_group_rows(mb, dev, tokens, choices, groups, id_type):
     ids = ids_for(tokens, choices, groups, 5, id_type)
     plan = mb.group_rows(ids.to(dev), groups)
