@@ -214,7 +214,7 @@ lora_row_kernel(const LoraArgs g) {
 // row of the box, which goes out by TMA again.  (C through registers and D by vector stores, on two CTAs per SM: 16384 rows
 // of 24 requests, rank 64, 4096 x 4096: 115 us.)
 //
-// Measured: those 16384 rows 83 us (X streams at 6.3 TB/s, C and D at 5.6; 4 us of start-up, 1.5 of exchange between them),
+// Measured: those 16384 rows 80 us (X streams at 6.3 TB/s, C and D at 5.6; 4 us of start-up, 1.5 of exchange between them),
 // 64 requests of 16 rows, R = 64: 43 us against 215 row by row.
 //
 // Tiles of at most 32 rows turn the second product round: the lanes are the columns of D and the rows its columns, so
@@ -519,8 +519,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     uint64_t* my_full = c_full + (warp - 4) * p.c_bufs;
     const int nboxes = VEC && !turned && qd * 32 < nrows ? (ch1 - ch0) * BPC : 0;
     auto box_col = [&](int k) { return (ch0 + k / BPC) * 128 + set * 64 + (k % BPC) * BW; };
-    auto request = [&](int k) {  // one lane
-      const int slot = k % p.c_bufs;
+    auto request = [&](int k, int slot) {  // one lane
       mbar_arrive_expect_tx(&my_full[slot], 4096);
       tma_load_2d(my_boxes + slot * 4096, &tmC, &my_full[slot], box_col(k), row0 + qd * 32);
     };
@@ -572,7 +571,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     ok = ok && lora_epi_all(mbar_wait(v_acc, 0, p.status, SITEL_EPI_V));
     if (ok) {
       if (C == 1 && lane == 0)
-        for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
+        for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k, k);
       auto each_4 = [&](auto&& f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -581,6 +580,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             for (int j = 0; j < 16; j += 4)
               f((set + 2 * i) * 16 + j, make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]));
       };
+      const int turn = my_row % (rsteps * 4);  // of this row's units in `parts`
       float down = scale, most = 0.f;
       auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))); };
       if (RANGE && C == 1) {
@@ -598,8 +598,8 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
                       [&](int at, uint32_t w0, uint32_t w1) { *reinterpret_cast<uint2*>(vparts + at) = make_uint2(w0, w1); });
         } else {
           // 16-byte units of a row rotated by the row: neighbouring rows fall on different banks
-          const int units = rsteps * 4, u = (c >> 2) + my_row;
-          *reinterpret_cast<float4*>(parts + my_row * units * 4 + (u % units) * 4) = x;
+          const int units = rsteps * 4, u = (c >> 2) + turn;
+          *reinterpret_cast<float4*>(parts + my_row * units * 4 + (u < units ? u : u - units) * 4) = x;
           if (RANGE) largest(x);
         }
       });
@@ -651,7 +651,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           ok = lora_epi_all(mbar_wait_cluster(v_ready, 0, p.status, SITEL_EPI_PARTS));
           fence_proxy_async_smem();
           if (ok && lane == 0)
-            for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k);
+            for (int k = 0; k < p.c_bufs - 1 && k < nboxes; ++k) request(k, k);
         }
       }
     }
@@ -692,6 +692,8 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       }
     } else {
       const bool live = qd * 32 < nrows, whole = qd * 32 + 32 <= nrows;  // this warp's 32 rows
+      int slot = 0;  // of the next box, and the parity of its barrier
+      uint32_t box_phase = 0;
       const float up = RANGE && my_row < nrows ? row_up[my_row] : 1.f;
       for (int i = 0; i < ch1 - ch0 && ok; ++i) {
         const int buf = i & 1;
@@ -710,11 +712,11 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         }
         if constexpr (VEC) {
           for (int b = 0; b < BPC; ++b) {
-            const int k = i * BPC + b, slot = k % p.c_bufs, col = box_col(k);
+            const int k = i * BPC + b, col = box_col(k);
             uint32_t v[BW];
 #pragma unroll
             for (int c = 0; c < BW; c += 32) tmem_ld_x32(t_half + b * BW + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
-            ok = mbar_wait(&my_full[slot], (k / p.c_bufs) & 1, p.status, SITEL_EPI_C);
+            ok = mbar_wait(&my_full[slot], box_phase, p.status, SITEL_EPI_C);
             tmem_ld_wait();
             if (b == BPC - 1) release();
             if (!ok) break;
@@ -743,7 +745,9 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
                       *reinterpret_cast<const uint4*>(my_boxes + slot * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
               }
             }
-            if (lane == 0 && k + p.c_bufs - 1 < nboxes) request(k + p.c_bufs - 1);
+            // box k + c_bufs - 1 goes where box k - 1 was
+            if (lane == 0 && k + p.c_bufs - 1 < nboxes) request(k + p.c_bufs - 1, slot == 0 ? p.c_bufs - 1 : slot - 1);
+            if (++slot == p.c_bufs) { slot = 0; box_phase ^= 1; }
           }
         } else {
           float* st = reinterpret_cast<float*>(my_boxes);  // 32 rows of 32 columns, 16-byte units swizzled by the row
