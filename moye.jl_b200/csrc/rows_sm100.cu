@@ -16,6 +16,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstdlib>
+
 #include "common.h"
 #include "ptx.cuh"
 
@@ -619,6 +621,10 @@ int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const mo
   if (int rc = check_rows("combine_rows_grad", ddst, dsrc, dsrc, choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", weights, ddst->shape[0], choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", dweights, ddst->shape[0], choices)) return rc;
+  // any order of the modes, but an element of its own for every choice (no broadcast output)
+  const long long T = dweights->shape[0], st = std::llabs(dweights->stride[0]), sc = std::llabs(dweights->stride[1]);
+  if (st > sc ? choices > 1 && (sc == 0 || (T > 1 && st < choices * sc)) : (T > 1 && st == 0) || (choices > 1 && T > 1 && sc < T * st))
+    MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "combine_rows_grad: elements of dweights overlap");
   if (weights->dtype != dweights->dtype) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "combine_rows_grad: weights and dweights differ in type");
   if (ddst->shape[0] == 0) return MOYE_OK;
   if (ddst->shape[1] == 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "combine_rows_grad: rows of width 0");

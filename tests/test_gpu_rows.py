@@ -256,3 +256,25 @@ def test_refusals(mb, dev):
     with pytest.raises(RuntimeError):
         mb.gather_rows_(torch.zeros(8, 16), torch.zeros(4, 16), plan)
     torch.cuda.synchronize()
+
+
+def test_an_element_of_its_own_for_every_weight_gradient(mb, dev):
+    ids = torch.zeros(4, 2, dtype=torch.int64, device=dev)
+    plan = mb.group_rows(ids, 3)
+    ones, w = torch.ones(8, 16, device=dev), torch.ones(4, 2, device=dev)
+    z = lambda *s: torch.zeros(*s, device=dev)
+    for bad in (z(4, 1).expand(4, 2), z(1, 2).expand(4, 2), z(1, 1).expand(4, 2), z(9).as_strided((4, 2), (1, 1)), z(9).as_strided((4, 2), (1, 2)),
+                z(9).as_strided((4, 2), (2, 2))):
+        with pytest.raises(mb.MoyeError) as e:
+            mb.combine_rows_grad_(z(8, 16), bad, ones[:4], ones, plan, w)
+        assert e.value.code == -3, str(e.value)
+    for good in (z(4, 2), z(2, 4).t(), z(8, 6)[::2, 1::4], z(3, 9).t()[:8:2, :2]):
+        mb.combine_rows_grad_(z(8, 16), good, ones[:4], ones, plan, w)
+        assert bool((good == 16).all())
+    one = mb.group_rows(ids[:1], 3)   # a single token, a single choice: their strides say nothing
+    for shape, stride, p in (((1, 2), (0, 1), one), ((4, 1), (2, 0), mb.group_rows(ids[:, 0], 3))):
+        good = z(8).as_strided(shape, stride)
+        n = shape[0] * shape[1]
+        mb.combine_rows_grad_(z(n, 16), good, ones[:shape[0]], ones[:n], p, w[:shape[0], :shape[1]])
+        assert bool((good == 16).all())
+    mb.synchronize_status(dev)
