@@ -712,6 +712,12 @@ static int check_row_operand(const char* who, const char* what, const moye_tenso
   return MOYE_OK;
 }
 
+// Bytes from row to row, of any tensor map's liking where there is but one row, whose pitch says nothing.
+static uint64_t row_pitch(const moye_tensor_t* t) {
+  const uint64_t eb = dtype_bytes(t->dtype);
+  return t->shape[0] > 1 ? t->stride[0] * eb : (t->shape[1] * eb + 15) / 16 * 16;
+}
+
 static int check_borders(const char* who, const int* offsets, int groups) {
   if (groups < 1 || groups > kMaxGemmGroups)
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d groups (got %d)", who, kMaxGemmGroups, groups);
@@ -766,11 +772,11 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
   if (int rc = encode_tmap_3d(&tl, B->ptr, B->dtype, inner, outer, G, (outer > 1 ? pitch : (inner + 7) / 8 * 8) * 2,
                               (G > 1 ? B->stride[0] : (inner + 7) / 8 * 8) * 2, 64, mn ? 64 : 128, true))
     return rc;
-  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, BT / 2, true)) return rc;
-  if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, kColBox, true)) return rc;
+  if (int rc = encode_tmap_2d_uncached(&tc, A->ptr, A->dtype, K, R, row_pitch(A), 64, BT / 2, true)) return rc;
+  if (int rc = encode_tmap_2d_uncached(&tn, A->ptr, A->dtype, K, R, row_pitch(A), 64, kColBox, true)) return rc;
   a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f) && (a.lanes * ob) % 16 == 0;  // TMA writes whole 16-byte units, past an odd extent too
   if (a.tma_out)
-    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, (uint64_t)D->stride[0] * ob, ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&td, D->ptr, D->dtype, N, R, row_pitch(D), ob == 2 ? 64 : 32, 32, ob == 2)) return rc;
   log_line("gemm_grouped %lld rows, %lld groups, %lld x %lld  in %d", (long long)R, (long long)G, (long long)N,
            (long long)K, A->dtype);
   if (mn) return launch_grouped<GROUPED_MN_MAJOR>(D->dtype, h, tl, tc, tn, td, a, tiles, stream);
@@ -821,8 +827,8 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   std::memset(&tl, 0, sizeof(tl));
   std::memset(&tc, 0, sizeof(tc));
   if (R > 0) {  // without rows the kernel loads nothing, every group's sum is empty
-    if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, (uint64_t)A->stride[0] * 2, 64, 64, true)) return rc;
-    if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, (uint64_t)dD->stride[0] * 2, 64, 64, true)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&tl, A->ptr, A->dtype, K, R, row_pitch(A), 64, 64, true)) return rc;
+    if (int rc = encode_tmap_2d_uncached(&tc, dD->ptr, dD->dtype, N, R, row_pitch(dD), 64, 64, true)) return rc;
   }
   a.tma_out = a.vec_out && (beta == 0.f || beta == 1.f) && (a.lanes * ob) % 16 == 0;  // TMA writes whole 16-byte units, past an odd extent too
   if (a.tma_out) {

@@ -945,10 +945,11 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
   g.n = (int)N;
   g.k = (int)K;
   g.X = X->ptr; g.A = A->ptr; g.B = B->ptr; g.C = C->ptr; g.D = D->ptr;
-  g.x_pitch = X->stride[0];
+  g.x_pitch = T > 1 ? X->stride[0] : K;  // the pitch of a single row says nothing
   g.a_pitch = A->stride[1]; g.a_stride = A->stride[0];
   g.b_pitch = B->stride[1]; g.b_stride = B->stride[0];
-  g.c_pitch = C->stride[0]; g.d_pitch = D->stride[0];
+  g.c_pitch = T > 1 ? C->stride[0] : N;
+  g.d_pitch = T > 1 ? D->stride[0] : N;
   g.which = which;
   g.offsets = offsets;
   g.scales = scales;

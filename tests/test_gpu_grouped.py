@@ -169,6 +169,23 @@ def test_odd_extents_between_padded_pitches(mb, dev, out):
     mb.synchronize_status(dev)
 
 
+@pytest.mark.parametrize("k", [1001, 1008])
+def test_the_pitch_of_a_single_row_says_nothing(mb, dev, k):
+    gen = torch.Generator(device=dev).manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen, device=dev).to(torch.bfloat16)
+    one = lambda t: t.as_strided(t.shape, (t.shape[1] + 3, 1))
+    a, b, d = one(r(1, k)), r(2, 72, 1008)[:, :, :k], one(r(1, 72))
+    edge = torch.tensor([0, 0, 1], dtype=torch.int32, device=dev)
+    got = mb.gemm_grouped_(one(torch.zeros(1, 72, device=dev, dtype=torch.bfloat16)), a, b, edge)
+    want, mag = a.double() @ b[1].double().T, a.double().abs() @ b[1].double().abs().T
+    assert within(got, want, mag, k, torch.bfloat16)
+    grad = mb.gemm_grouped_grad_(torch.ones(2, 72, k, device=dev, dtype=torch.bfloat16), d, a, edge)
+    mb.synchronize_status(dev)
+    assert bool((grad[0] == 0).all())
+    want = d.double().T @ a.double()
+    assert within(grad[1], want, want.abs(), 1, torch.bfloat16)
+
+
 def test_a_group_longer_than_many_tiles(mb, dev):
     """9 row tiles (a full band of 8 and one more) and a sum over 2100 rows."""
     offsets, rows, n, k = [0, 2100, 2110], 2110, 520, 136

@@ -120,6 +120,16 @@ def test_pitched_views_and_moye_arrays(mb, dev):
     assert torch.equal(big[:, :3], base[:, :3]) and torch.equal(big[:, 3 + n:], base[:, 3 + n:])
 
 
+def test_the_pitch_of_a_single_row_says_nothing(mb, dev):
+    case = ([0, 1], 1, [0], 272000, 272000, 128, 1)  # long enough for the tiles of the tensor cores
+    x, a, b, scales, w, edge = make(case, "bf16", dev)
+    one = lambda t: t.as_strided(t.shape, (t.shape[1] + 3, 1))
+    c = torch.randn(1, 272000, device=dev).to(torch.bfloat16)
+    got = mb.gemm_lora_(one(torch.zeros_like(c)), one(x), a, b, w, edge, scales, C=one(c))
+    mb.synchronize_status(dev)
+    check(got, c, x, a, b, scales, [0], [0, 1], torch.bfloat16, c)
+
+
 def test_infinities_stay_in_their_rows(mb, dev):
     x, a, b, scales, w, edge = make(CASES[3], "bf16", dev)
     x[:2], x[300:], x[129] = float("nan"), float("inf"), float("inf")
