@@ -5,6 +5,8 @@ The shared library is built in-tree (``moye.jl_b200/lib/libmoye_b200.so``) by
 visible when a handle is requested, the call raises.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 import threading
@@ -110,12 +112,14 @@ EXPORTS = {
 }
 
 _lib = None
+_handles = {}  # (thread, device) -> handle
+calls = None  # the compiled module of the row-group calls, bound to the loaded library
 _lock = threading.Lock()
 
 
 def load():
     """dlopen the in-tree library and type its exports.  Raises if it has not been built."""
-    global _lib
+    global _lib, calls
     if _lib is not None:
         return _lib
     with _lock:
@@ -129,16 +133,30 @@ def load():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args
+            calls = _load_calls(lib)
             _lib = lib
     return _lib
+
+
+def _load_calls(lib):
+    """csrc/calls.cpp, bound to the entry points of `lib`.  None where it was not built, or for another torch than the one
+    that runs: the calls then take the way through ctypes into the same entry points, at more of the host's time."""
+    path = os.path.join(os.path.dirname(LIB_PATH), "moye_calls.so")
+    try:
+        import torch  # noqa: F401  the module's own libraries
+        loader = importlib.machinery.ExtensionFileLoader("moye_calls", path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("moye_calls", path, loader=loader))
+        loader.exec_module(mod)
+    except (ImportError, OSError):
+        return None
+    names = ("group_rows", "gather_rows", "combine_rows", "combine_rows_grad", "gemm_grouped", "gemm_grouped_grad", "gemm_lora")
+    mod.bind(tuple(ctypes.cast(getattr(lib, "moye_b200_" + n), ctypes.c_void_p).value for n in names), _handles)
+    return mod
 
 
 def check(rc):
     if rc != 0:
         raise MoyeError(rc, load().moye_b200_last_error().decode())
-
-
-_handles = {}
 
 
 def handle(device=None):

@@ -1,22 +1,26 @@
 """Builds libmoye_b200.so in-tree (moye.jl_b200/lib/) with nvcc for sm_100a.
 
 Usage: python moye.jl_b200/build.py [--force] [--verbose] [--debug]
+Also builds lib/moye_calls.so, the row-group calls' way from Python into the library (host code only, against torch's headers).
 nvcc cross-compiles, so this works on a machine without a GPU.  Every source is compiled to its
 own object (kept under lib/obj/, rebuilt only when it or a header changed), the objects side by
 side, then linked.  `--debug` builds lib/libmoye_b200_debug.so with -DMOYE_DEBUG: the kernels
 then check every TMA coordinate, tensor-memory column and stage index on the device and report
 a violation through the status word instead of touching memory.
 """
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 OUT = os.path.join(LIBDIR, "libmoye_b200.so")
+OUT_CALLS = os.path.join(LIBDIR, "moye_calls.so")
 OUT_DEBUG = os.path.join(LIBDIR, "libmoye_b200_debug.so")
 SOURCES = ["api.cu", "gemm_sm100.cu", "gemm_single.cu", "gemm_pair.cu", "gemm_wide.cu", "gemm_splitk.cu",
            "gemm_skinny.cu", "copy_sm100.cu", "transpose_sm100.cu", "layout_sm100.cu", "axpby_sm100.cu", "ldsm_sm100.cu",
@@ -30,6 +34,27 @@ def _newer(path, deps):
         return True
     t = os.path.getmtime(path)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_calls(force=False):
+    """Compile csrc/calls.cpp, a Python extension module; returns its path."""
+    src = os.path.join(CSRC, "calls.cpp")
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    if not force and not _newer(OUT_CALLS, [src, os.path.join(CSRC, HEADERS[-1]), os.path.join(torch_dir, "version.py"), os.path.abspath(__file__)]):
+        return OUT_CALLS
+    os.makedirs(LIBDIR, exist_ok=True)
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")]
+    import torch
+    res = subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
+                         [x for i in include for x in ("-isystem", i)] +
+                         [src, "-o", OUT_CALLS, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
+                         capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("building moye_calls failed")
+    return OUT_CALLS
 
 
 def build(force=False, verbose=False, debug=False):
@@ -72,3 +97,4 @@ def build(force=False, verbose=False, debug=False):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, debug="--debug" in sys.argv))
+    print(build_calls(force="--force" in sys.argv))

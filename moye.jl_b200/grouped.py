@@ -13,6 +13,9 @@ argument (and return it), operands are torch CUDA tensors or MoYeArrays, calls a
 the operands' device or on `stream`, a violation raises `MoyeError`, nothing falls back to another implementation.  Group
 borders, choices and adapter numbers stay on the device: no call waits for the GPU, and a captured call follows new
 values in the same arrays.  The reference has no counterpart.
+
+Every call is offered to the compiled module of csrc/calls.cpp first (`_lib.calls`), which takes plain tensors on the
+current device into the same entry points; what it does not take is checked, explained and launched here.
 """
 import struct
 import threading
@@ -45,9 +48,10 @@ class RowGroups:
 
     __slots__ = ("tokens", "choices", "groups", "_buf", "_at")
 
-    def __init__(self, tokens, choices, groups, device):
+    def __init__(self, tokens, choices, groups, device, buf=None):
         self.tokens, self.choices, self.groups = tokens, choices, groups
-        self._buf = torch.empty(2 * tokens * choices + groups + 1, dtype=_INT32, device=device)  # order, inverse, offsets
+        # order, inverse, offsets
+        self._buf = torch.empty(2 * tokens * choices + groups + 1, dtype=_INT32, device=device) if buf is None else buf
         self._at = self._buf.get_device()
 
     @property
@@ -131,10 +135,24 @@ def _call(fn, dev, stream, *args):
         _lib.check(rc)
 
 
+def _taken(rc):
+    """What the compiled call said: True if it launched, False if it leaves the call to this module; raises its errors."""
+    if rc < 0:
+        _lib.check(rc)
+    return rc == 0
+
+
 def group_rows(ids, groups):
     """Sort the group numbers `ids` ((tokens,) or (tokens, choices), int32 or int64) by group: a new `RowGroups`.
     Equal numbers keep their order; numbers outside 0..groups-1 are dropped (a capacity that ran out, a masked token).
     At most 1024 groups.  Runs on the current stream, which also owns the new tensors."""
+    if _lib.calls is not None:
+        buf = _lib.calls.new_plan(ids, groups)
+        if type(buf) is torch.Tensor:
+            shape = ids.shape
+            return RowGroups(shape[0], shape[1] if len(shape) == 2 else 1, groups, None, buf)
+        if buf < 0:
+            _lib.check(buf)
     if not torch.is_tensor(ids):
         raise TypeError("ids must be a torch.Tensor")
     if ids.dim() not in (1, 2):
@@ -148,6 +166,10 @@ def group_rows(ids, groups):
 
 def group_rows_(plan, ids, stream=None):
     """`group_rows` into the tensors of an existing plan of the same tokens, choices and groups."""
+    if _lib.calls is not None:
+        rc = _lib.calls.group_rows(ids, plan._buf, plan.tokens, plan.choices, plan.groups, stream)
+        if _taken(rc):
+            return plan
     rank = len(ids.shape)
     t, dev = _arg(ids, 1 if rank == 1 else 2, "ids")
     if ids.shape[0] != plan.tokens or (ids.shape[1] if rank == 2 else 1) != plan.choices:
@@ -163,6 +185,8 @@ def gather_rows_(dst, src, plan, stream=None):
     """dst[p] = src[plan.order[p] // choices] for the kept positions; rows of dst behind them are left as they were.
     src (tokens, width), dst (tokens * choices, width); any element type, contiguous rows.  Its gradient is
     `combine_rows_(dsrc, ddst, plan)`."""
+    if _lib.calls is not None and _taken(_lib.calls.gather_rows(dst, src, plan._buf, plan.tokens, plan.choices, stream)):
+        return dst
     td, dev = _arg(dst, 2, "dst")
     ts, d1 = _arg(src, 2, "src")
     _fits(plan, src, "src")
@@ -175,6 +199,8 @@ def gather_rows_(dst, src, plan, stream=None):
 def combine_rows_(dst, src, plan, weights=None, stream=None):
     """dst[t] = sum_j weights[t, j] * src[plan.inverse[t, j]] over the choices that were kept (none: zeros), in fp32 in
     the order of j with one rounding.  `weights` (tokens, choices) in f32, f16 or bf16; None counts every choice once."""
+    if _lib.calls is not None and _taken(_lib.calls.combine_rows(dst, src, plan._buf, plan.tokens, plan.choices, weights, stream)):
+        return dst
     td, dev = _arg(dst, 2, "dst")
     ts, d1 = _arg(src, 2, "src")
     tw, d2 = (None, dev) if weights is None else _arg(weights, 2, "weights")
@@ -189,6 +215,9 @@ def combine_rows_grad_(dsrc, dweights, ddst, src, plan, weights, stream=None):
     """The gradient of `combine_rows_(dst, src, plan, weights)`: dsrc[inverse[t, j]] = weights[t, j] * ddst[t] (rows
     behind the kept positions are left as they were), dweights[t, j] = <ddst[t], src[inverse[t, j]]>, 0 where the choice
     was dropped.  Returns (dsrc, dweights)."""
+    if _lib.calls is not None and _taken(_lib.calls.combine_rows_grad(dsrc, dweights, ddst, src, plan._buf, plan.tokens, plan.choices,
+                                                                      weights, stream)):
+        return dsrc, dweights
     t0, dev = _arg(dsrc, 2, "dsrc")
     t1, d1 = _arg(dweights, 2, "dweights")
     t2, d2 = _arg(ddst, 2, "ddst")
@@ -199,6 +228,13 @@ def combine_rows_grad_(dsrc, dweights, ddst, src, plan, weights, stream=None):
         _differ()
     _call(_lib.load().moye_b200_combine_rows_grad, dev, stream, t0, t1, t2, t3, t4, plan._pointers()[1], plan.choices)
     return dsrc, dweights
+
+
+def _borders_plain(offsets):
+    """The tensor that holds the borders and the index of the first."""
+    if isinstance(offsets, RowGroups):
+        return offsets._buf, 2 * offsets.tokens * offsets.choices
+    return offsets, 0
 
 
 def _borders(offsets, groups, dev):
@@ -218,6 +254,8 @@ def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
     groups + 1 borders or the RowGroups they come from.  B may be the swapped view of a (groups, K, N) array:
     `gemm_grouped_(dA, dD, B.transpose(1, 2), offsets)` is the gradient of A.  Rows outside the groups are left as they
     were; D is not read when beta == 0."""
+    if _lib.calls is not None and _taken(_lib.calls.gemm_grouped(D, A, B, *_borders_plain(offsets), alpha, beta, stream)):
+        return D
     td, dev = _arg(D, 2, "D")
     ta, d1 = _arg(A, 2, "A")
     tb, d2 = _arg(B, 3, "B")
@@ -230,6 +268,8 @@ def gemm_grouped_(D, A, B, offsets, alpha=1.0, beta=0.0, stream=None):
 def gemm_grouped_grad_(dB, dD, A, offsets, alpha=1.0, beta=0.0, stream=None):
     """dB[g] = alpha * sum of dD[i]^T A[i] over the rows of group g + beta * dB[g]: the gradient of `gemm_grouped_` with
     respect to B.  Every group is written (an empty one becomes beta * dB[g]); beta = 1 accumulates over micro-batches."""
+    if _lib.calls is not None and _taken(_lib.calls.gemm_grouped_grad(dB, dD, A, *_borders_plain(offsets), alpha, beta, stream)):
+        return dB
     tb, dev = _arg(dB, 3, "dB")
     td, d1 = _arg(dD, 2, "dD")
     ta, d2 = _arg(A, 2, "A")
@@ -247,6 +287,8 @@ def gemm_lora_(D, X, A, B, adapters, offsets=None, scales=None, C=None, stream=N
     one int32 per request, a number outside 0..count-1 means none.  `offsets` (requests + 1 borders, int32) says which
     rows are a request's; without it every row is one.  Rows outside every request are left as they were.  R is a
     multiple of 8 up to 128: pad adapters of smaller rank with zeros."""
+    if _lib.calls is not None and _taken(_lib.calls.gemm_lora(D, X, A, B, adapters, offsets, scales, C, stream)):
+        return D
     td, dev = _arg(D, 2, "D")
     tx, d1 = _arg(X, 2, "X")
     ta, d2 = _arg(A, 3, "A")

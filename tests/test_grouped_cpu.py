@@ -51,3 +51,21 @@ def test_entry_points_check_their_handle(mb):
     assert lib.moye_b200_gemm_grouped_grad(z, z, z, z, z, f, f, z) == -1
     assert lib.moye_b200_gemm_lora(z, z, z, z, z, z, z, z, 0, z, z) == -1
     assert b"null handle" in lib.moye_b200_last_error()
+
+
+def test_the_compiled_calls_leave_what_is_not_plain(mb):
+    """Arrays that are not on a device, wrong types, wrong argument counts: not taken (1), never an exception or a launch."""
+    mb._lib.load()
+    calls = mb._lib.calls
+    assert calls is not None, "lib/moye_calls.so was not built"
+    x, v = torch.zeros(4, 8), torch.zeros(20, dtype=torch.int32)
+    for odd in (x, None, 3, "x", torch.zeros(4, 8).to_sparse(), torch.zeros(4, 8, dtype=torch.complex64)):
+        assert calls.gather_rows(odd, x, v, 4, 2, None) == 1
+        assert calls.combine_rows(x, odd, v, 4, 2, None, None) == 1
+        assert calls.combine_rows_grad(x, x, odd, x, v, 4, 2, x, None) == 1
+        assert calls.gemm_grouped(odd, x, x, v, 0, 1.0, 0.0, None) == 1
+        assert calls.gemm_grouped_grad(x, odd, x, v, 0, 1.0, 0.0, None) == 1
+        assert calls.gemm_lora(odd, x, x, x, v, None, None, None, None) == 1
+        assert calls.group_rows(odd, v, 4, 2, 3, None) == 1
+        assert calls.new_plan(odd, 3) == 1
+    assert calls.new_plan(x) == 1 and calls.gather_rows() == 1 and calls.group_rows(v, v, 10 ** 30, 2, 3, None) == 1
