@@ -196,11 +196,25 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
+// Two values rounded by one instruction, the first in the low half.
 template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-  const T lo = cvt_out<T>(a), hi = cvt_out<T>(b);
-  return (uint32_t)(*reinterpret_cast<const uint16_t*>(&lo)) | ((uint32_t)(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+  const __half2 x = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Float32 tiles leave through two staging tiles a warp in turn (those gradients in Float32: 193 -> 184 us), 16-bit ones
+// through one a warp, two for the pair.  What is left of shared memory holds 5 stages of operands, or 6 (16-bit with 5: 1 to
+// 2 % slower on long sums).
+template <typename OutT>
+__host__ __device__ constexpr int grouped_epi_bufs() { return sizeof(OutT) == 4 ? 2 : 1; }
 
 template <int MODE, typename OutT, int STAGES>
 __global__ void __launch_bounds__(384, 1)
@@ -216,7 +230,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
   constexpr bool L_MN = MODE != GROUPED_K_MAJOR, C_MN = MODE == GROUPED_GRAD;
   constexpr bool PROMOTE = sizeof(OutT) == 4;
   constexpr int EPI_BUF = 32 * 128;            // a staging tile: 32 columns of 128 bytes
-  constexpr int EPI_BYTES = 8 * EPI_BUF;       // one per epilogue warp (Float32 outputs) or two per pair of them
+  constexpr int EPI_BUFS = grouped_epi_bufs<OutT>();  // staging tiles of each epilogue warp
+  constexpr int EPI_BYTES = 8 * EPI_BUFS * EPI_BUF;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -414,7 +429,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     // Four warps read the tensor memory's four quarters of 32 lanes; two such sets share the blocks of 32 columns.
     const int q = warp & 3;
     const int set = (warp - 4) >> 2;
-    uint8_t* my_epi = epi + (PROMOTE ? warp - 4 : (warp - 4) >> 1 << 1) * EPI_BUF;
+    uint8_t* my_epi = epi + (PROMOTE ? warp - 4 : (warp - 4) >> 1 << 1) * (EPI_BUFS * EPI_BUF);
     int buf = 0, lt = 0;
     bool ok = true;
     while (ok && all_of_128(1 + set, ring.take(tile))) {
@@ -487,11 +502,12 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[i * 32 + j]);
             if (a.vec_out) {
               // [32 columns][32 lanes] per warp, stored as rows of 128 bytes
-              float* sb = reinterpret_cast<float*>(my_epi);
+              float* sb = reinterpret_cast<float*>(my_epi + buf * EPI_BUF);
+              buf ^= 1;
               const bool add = a.beta == 1.f;  // the memory adds: nothing is read
               const bool whole = a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols);
-              if (lane == 0) tma_store_wait_read<0>();
-              __syncwarp();  // the last block has left
+              if (lane == 0) tma_store_wait_read<1>();
+              __syncwarp();  // the block that was here has left
 #pragma unroll
               for (int j = 0; j < 32; ++j) sb[j * 32 + lane] = __uint_as_float(v[j]) * a.alpha;
               if (whole) {
@@ -506,10 +522,11 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
                     if (add) tma_reduce_add_2d(&tmD, sb, x, tile.col0 + c);
                     else tma_store_2d(&tmD, sb, x, tile.col0 + c);
                   }
-                  tma_store_commit();
                 }
+                if (lane == 0) tma_store_commit();
                 continue;
               }
+              if (lane == 0) tma_store_commit();  // an empty group: every block counts as one
               __syncwarp();
               const int x = l0 + q * 32 + (lane & 7) * 4, j0 = lane >> 3;
               float4 w[8];
@@ -551,83 +568,101 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
         const int t_buf = (lt & 1) * BT;
         const int blocks = tile.width / 32, last = (blocks - 1 - set) / 2 * 2 + set;  // this set's last block (below 0: none)
         if (kbs > 0 && blocks <= set) release();
+        // Two blocks at a time: short sums are bound by a block's latencies (tensor-memory load, conversion, proxy fence,
+        // barriers; 0.8 us of them), which two have in common (64 weight gradients of 2048 x 2048, one row each: 163 -> 128 us).
 #pragma unroll 1
-        for (int blk = set; blk < blocks; blk += 2) {
-          const int c = blk * 32;
-          const uint32_t at = t_lane + t_buf + c;
+        for (int blk = set; blk < blocks; blk += 4) {
+          const int both = blk + 2 < blocks ? 2 : 1;
           if (a.vec_out) {
-            // Two warps share a staging tile [32 columns][128 bytes of 64 lanes] in the 128-byte swizzle; of two tiles one is
-            // free again when its readers have come to the next barrier.  Whole 8 x 8 fragments are staged transposed: single
-            // 16-bit elements would take twice the shared-memory cycles, which the tensor cores need for their operands.
-            const uint32_t sb = smem_u32(my_epi + buf * EPI_BUF);
+            // Two warps share two staging tiles [32 columns][128 bytes of 64 lanes] in the 128-byte swizzle.  Whole 8 x 8
+            // fragments are staged transposed: single 16-bit elements would take twice the shared-memory cycles, which the tensor
+            // cores need for their operands.
+            uint32_t f[2][4][4];
             {
-              uint32_t v[2][16];
+              uint32_t v[4][16];
               if (kbs > 0) {
-                tmem_ld_16x32(at, v[0]);
-                tmem_ld_16x32(at + (16u << 16), v[1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (h < both) {
+                    tmem_ld_16x32(t_lane + t_buf + (blk + 2 * h) * 32, v[2 * h]);
+                    tmem_ld_16x32(t_lane + t_buf + (blk + 2 * h) * 32 + (16u << 16), v[2 * h + 1]);
+                  }
                 tmem_ld_wait();
-                if (blk == last) release();
+                if (blk + 2 * both - 2 == last) release();
               } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[0][j] = v[1][j] = 0u;
+                for (int j = 0; j < 64; ++j) v[j >> 4][j & 15] = 0u;
               }
-              const int row = lane & 7, unit = (q & 1) * 4 + (lane >> 3);  // this thread's row and fragment of every group of four
 #pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                uint32_t f[4];
+              for (int j = 0; j < 32; ++j) {
+                const int h = j >> 4, b = (j >> 2) & 3, i = j & 3;
+                f[h][b][i] = pack_pair<OutT>(__uint_as_float(v[2 * h + (i >> 1)][4 * b + 2 * (i & 1)]) * a.alpha,
+                                             __uint_as_float(v[2 * h + (i >> 1)][4 * b + 2 * (i & 1) + 1]) * a.alpha);
+              }
+            }
+            // the tiles are free when the stores of the last step have read them, and both warps are done with it
+            const bool storer = (q & 1) == 0 && lane == 0;
+            auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(3 + ((warp - 4) >> 1)) : "memory"); };  // barriers 3..6
+            if (storer) tma_store_wait_read<0>();
+            meet();
+            const int row = lane & 7, unit = (q & 1) * 4 + (lane >> 3);  // this thread's row and fragment of every group of four
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (h < both) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                  stmatrix_x4_trans(smem_u32(my_epi + h * EPI_BUF) + (b * 8 + row) * 128 + ((unit ^ row) << 4), f[h][b][0], f[h][b][1],
+                                    f[h][b][2], f[h][b][3]);
+              }
+            fence_proxy_async_smem();
+            meet();
+            // A block that belongs to this tile as a whole goes out by TMA, the last rows of a group by vector stores.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h >= both) break;
+              const int c = (blk + 2 * h) * 32;
+              const uint8_t* from = my_epi + h * EPI_BUF;
+              if (a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols)) {
+                const int x = l0 + (q >> 1) * 64;
+                if (storer && x < a.lanes) {
+                  if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, from, x, tile.col0 + c, tile.g);
+                  else tma_store_2d(&tmD, from, x, tile.col0 + c);
+                  tma_store_commit();
+                }
+                continue;
+              }
+              const int x = l0 + (q >> 1) * 64 + (lane & 7) * 8, j0 = (q & 1) * 16 + (lane >> 3);
+              uint4 w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = *reinterpret_cast<const uint4*>(from + (j0 + i * 4) * 128 + (((lane & 7) ^ ((j0 + i * 4) & 7)) << 4));
+              OutT* p = row0 + (c + j0) * a.ld + x;
+              const int live = x < a.lanes ? tile.ncols - c - j0 : 0;  // rows i * 4 < live are stored
+              if (x + 8 <= a.lanes) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  f[i] = pack_pair<OutT>(__uint_as_float(v[i >> 1][4 * b + 2 * (i & 1)]) * a.alpha,
-                                         __uint_as_float(v[i >> 1][4 * b + 2 * (i & 1) + 1]) * a.alpha);
-                stmatrix_x4_trans(sb + (b * 8 + row) * 128 + ((unit ^ row) << 4), f[0], f[1], f[2], f[3]);
+                  if (i * 4 < live) *reinterpret_cast<uint4*>(p + i * 4 * a.ld) = w[i];
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (i * 4 < live)
+                    for (int k = 0; x + k < a.lanes; ++k) p[i * 4 * a.ld + k] = reinterpret_cast<const OutT*>(&w[i])[k];
               }
             }
-            // A block that belongs to this tile as a whole goes out by TMA, the last rows of a group by vector stores.  The
-            // thread that issues a pair's TMA stores lets the one before drain first: it read the tile that comes next.
-            const bool whole = a.tma_out && (MODE == GROUPED_GRAD || c + 32 <= tile.ncols);
-            const bool storer = (q & 1) == 0 && lane == 0;
-            fence_proxy_async_smem();
-            if (storer) tma_store_wait_read<0>();
-            asm volatile("bar.sync %0, 64;" ::"r"(3 + ((warp - 4) >> 1)) : "memory");  // barriers 3..6
-            if (whole) {
-              const int x = l0 + (q >> 1) * 64;
-              if (storer && x < a.lanes) {
-                if constexpr (MODE == GROUPED_GRAD) tma_store_3d(&tmD, my_epi + buf * EPI_BUF, x, tile.col0 + c, tile.g);
-                else tma_store_2d(&tmD, my_epi + buf * EPI_BUF, x, tile.col0 + c);
-                tma_store_commit();
-              }
-              buf ^= 1;
-              continue;
-            }
-            const int x = l0 + (q >> 1) * 64 + (lane & 7) * 8, j0 = (q & 1) * 16 + (lane >> 3);
-            uint4 w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = *reinterpret_cast<const uint4*>(my_epi + buf * EPI_BUF + (j0 + i * 4) * 128 + (((lane & 7) ^ ((j0 + i * 4) & 7)) << 4));
-            OutT* p = row0 + (c + j0) * a.ld + x;
-            const int live = x < a.lanes ? tile.ncols - c - j0 : 0;  // rows i * 4 < live are stored
-            if (x + 8 <= a.lanes) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (i * 4 < live) *reinterpret_cast<uint4*>(p + i * 4 * a.ld) = w[i];
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (i * 4 < live)
-                  for (int k = 0; x + k < a.lanes; ++k) p[i * 4 * a.ld + k] = reinterpret_cast<const OutT*>(&w[i])[k];
-            }
-            buf ^= 1;
           } else {
-            uint32_t v[32];
-            if (kbs > 0) {
-              tmem_ld_x32(at, v);
-              tmem_ld_wait();
-            } else {
+            for (int h = 0; h < both; ++h) {
+              const int c = (blk + 2 * h) * 32;
+              uint32_t v[32];
+              if (kbs > 0) {
+                tmem_ld_x32(t_lane + t_buf + c, v);
+                tmem_ld_wait();
+              } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0u;
+                for (int j = 0; j < 32; ++j) v[j] = 0u;
+              }
+              if (kbs > 0 && blk + 2 * h == last) release();
+              store_elements(c, v);
             }
-            if (kbs > 0 && blk == last) release();
-            store_elements(c, v);
           }
         }
       }
@@ -655,7 +690,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
 template <int MODE, typename OutT>
 static int launch_grouped_inst(moye_b200_ctx* h, const CUtensorMap& tl, const CUtensorMap& tc, const CUtensorMap& tn, const CUtensorMap& td,
                                const GroupedArgs& a, long long tiles, cudaStream_t stream) {
-  constexpr int EXTRA = 1024 + 1024 + 8 * 32 * 128;
+  constexpr int EXTRA = 1024 + 1024 + 8 * grouped_epi_bufs<OutT>() * 32 * 128;
   constexpr int STAGE = 128 * 128 + BT / 2 * 128;
   constexpr int STAGES = (227 * 1024 - EXTRA) / STAGE;
   constexpr int SMEM = STAGES * STAGE + EXTRA;
