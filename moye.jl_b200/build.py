@@ -97,4 +97,5 @@ def build(force=False, verbose=False, debug=False):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, debug="--debug" in sys.argv))
-    print(build_calls(force="--force" in sys.argv))
+    if importlib.util.find_spec("torch"):  # the library itself needs none
+        print(build_calls(force="--force" in sys.argv))

@@ -69,3 +69,11 @@ def test_the_compiled_calls_leave_what_is_not_plain(mb):
         assert calls.group_rows(odd, v, 4, 2, 3, None) == 1
         assert calls.new_plan(odd, 3) == 1
     assert calls.new_plan(x) == 1 and calls.gather_rows() == 1 and calls.group_rows(v, v, 10 ** 30, 2, 3, None) == 1
+
+
+def test_without_the_compiled_calls_there_is_the_way_through_ctypes(mb, tmp_path, monkeypatch):
+    lib = mb._lib.load()
+    monkeypatch.setattr(mb._lib, "LIB_PATH", str(tmp_path / "libmoye_b200.so"))
+    assert mb._lib._load_calls(lib) is None                    # not built
+    (tmp_path / "moye_calls.so").write_bytes(b"no library")
+    assert mb._lib._load_calls(lib) is None                    # cannot be loaded
