@@ -523,6 +523,11 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       mbar_arrive_expect_tx(&my_full[slot], 4096);
       tma_load_2d(my_boxes + slot * 4096, &tmC, &my_full[slot], box_col(k), row0 + qd * 32);
     };
+    // Scale first, then the power of two: their product leaves fp32 where a row is zero or tiny (2^126 * 4), and would make
+    // the row's zeros undefined.
+    auto scaled = [&](const float4& x, float down) {
+      return make_float4(x.x * scale * down, x.y * scale * down, x.z * scale * down, x.w * scale * down);
+    };
     // the value of `x` as PARTS 16-bit numbers, the largest first
     auto write_parts = [&](int row, int col, float4 x, auto&& store) {  // 4 columns at once
       float r[4] = {x.x, x.y, x.z, x.w};
@@ -581,7 +586,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
               f((set + 2 * i) * 16 + j, make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]));
       };
       const int turn = my_row % (rsteps * 4);  // of this row's units in `parts`
-      float down = scale, most = 0.f;
+      float down = 1.f, most = 0.f;
       auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))); };
       if (RANGE && C == 1) {
         each_4([&](int, const float4& x) { largest(x); });
@@ -589,12 +594,11 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         lora_epi_all(true);
         float up;
         lora_range(fmaxf(row_max[my_row], row_max[128 + my_row]) * fabsf(scale), down, up);
-        down *= scale;
         if (set == 0) row_up[my_row] = up;
       }
       each_4([&](int c, const float4& x) {
         if (C == 1) {
-          write_parts(my_row, c, make_float4(x.x * down, x.y * down, x.z * down, x.w * down),
+          write_parts(my_row, c, scaled(x, down),
                       [&](int at, uint32_t w0, uint32_t w1) { *reinterpret_cast<uint2*>(vparts + at) = make_uint2(w0, w1); });
         } else {
           // 16-byte units of a row rotated by the row: neighbouring rows fall on different banks
@@ -637,8 +641,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             }
             float down = 1.f, up;
             if (RANGE) range_of(row, down, up);
-            down *= scale;
-            write_parts(row, u * 4, make_float4(s.x * down, s.y * down, s.z * down, s.w * down), [&](int off, uint32_t w0, uint32_t w1) {
+            write_parts(row, u * 4, scaled(s, down), [&](int off, uint32_t w0, uint32_t w1) {
               const uint32_t to = smem_u32(vparts + off);
               for (int c = 0; c < C; ++c) st_remote_u32x2(mapa_shared(to, c), w0, w1);
             });

@@ -254,3 +254,39 @@ def test_refusals(mb, dev):
     refused(-2, *ok, C=z(4, 32, dtype=torch.float32))
     refused(-4, *ok, C=z(4, 40))
     torch.cuda.synchronize()
+
+
+# requests, K, N, R: a row each, turned tiles on several CTAs and on one, longer tiles on several CTAs and on one
+SCALED = [(list(range(0, 9)), 512, 264, 24), (list(range(0, 601, 30)), 4096, 1000, 24), (list(range(0, 4801, 30)), 512, 264, 24),
+          ([0, 150, 300], 2048, 4096, 64), (list(range(0, 8001, 40)), 512, 264, 24)]
+
+
+@pytest.mark.parametrize("out", ["same", "f32"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(SCALED)))
+def test_scales_of_any_size_and_rows_of_zeros(mb, dev, case, kind, out):
+    """Scales far from 1, negative and zero; rows of X and an adapter that are zero leave C as it is, whatever the scale."""
+    offsets, k, n, rank = SCALED[case]
+    rows, requests, size = offsets[-1], len(offsets) - 1, [4.0, 64.0, -8.0, 0.0, 1e30, -2.0 ** -40]
+    ot = DT[kind] if out == "same" else torch.float32
+    which = [i % len(size) for i in range(requests)]
+    x, a, b, _, w, edge = make((offsets, rows, which, n, k, rank, len(size)), kind, dev)
+    x[::3] = 0
+    x[1] = torch.finfo(DT[kind]).tiny  # a row whose product is far below 1
+    a[4] = 0
+    scales = torch.tensor(size, device=dev)
+    c = torch.randn(rows, n, device=dev).to(ot)
+    got = mb.gemm_lora_(torch.full_like(c, float("nan")), x, a, b, w, edge, scales, C=c)
+    mb.synchronize_status(dev)
+    assert torch.equal(got[::3], c[::3])
+    for q, i in enumerate(which):
+        s = slice(offsets[q], offsets[q + 1])
+        if size[i] == 0 or i == 4:
+            assert torch.equal(got[s], c[s])
+        add = size[i] * ((x[s].double() @ a[i].double().T) @ b[i].double().T)
+        mag = abs(size[i]) * ((x[s].double().abs() @ a[i].double().abs().T) @ b[i].double().abs().T)
+        want = c[s].double() + add
+        tol = (k + rank + 4) * 2.0 ** -23 * (mag + c[s].double().abs())
+        if ot != torch.float32:
+            tol = tol + 2.0 ** -16 * mag + torch.finfo(ot).eps / 2 * want.abs() + torch.finfo(ot).tiny * torch.finfo(ot).eps
+        assert bool(((got[s].double() - want).abs() <= tol).all())
