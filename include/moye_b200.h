@@ -316,7 +316,7 @@ int moye_b200_combine_rows_grad(moye_handle_t h, const moye_tensor_t* dsrc, cons
 
 /* D[i] = alpha * A[i] . B[g]^T + beta * D[i] for the rows offsets[g] <= i < offsets[g+1]; other rows of D are left as
  * they were, and D is not read when beta == 0.  A (rows, K), B (groups, N, K), D (rows, N); offsets: groups + 1 borders
- * on the device, not decreasing (clamped to the rows; a border that runs backwards makes an empty group); groups <= 1024,
+ * on the device, not decreasing (clamped to the rows; one below an earlier one counts as that one, its group is empty); groups <= 1024,
  * extents up to 2^27.  f16 or bf16 operands, fp32 accumulation, D f32 or the operands' type.  A: contiguous rows; B: unit stride along K, or
  * along N (the swapped view of a (groups, K, N) array: dA = dD . B, the gradient of A); base and pitches of A and B
  * multiples of 16 bytes.  D: contiguous rows, any pitch. */
@@ -331,8 +331,8 @@ int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const 
                                 const int32_t* offsets, float alpha, float beta, void* stream);
 
 /* Low-rank adapters of many requests: D[i] = C[i] + scales[a] * (X[i] . A[a]^T) . B[a]^T, where a = adapters[q] and q
- * is the request with offsets[q] <= i < offsets[q+1] (borders not decreasing), or q = i when offsets is NULL (then
- * requests = rows).  X (rows, K), A (count, R, K), B (count, N, R), C and D (rows, N).  An adapter number outside
+ * is the request with offsets[q] <= i < offsets[q+1] (borders not decreasing: one below an earlier one counts as that
+ * one), or q = i when offsets is NULL (then requests = rows).  X (rows, K), A (count, R, K), B (count, N, R), C and D (rows, N).  An adapter number outside
  * 0..count-1 means none: D[i] = C[i].  Rows outside every request are left as they were.  C NULL or C = D: in place.
  * scales: one float per adapter, or NULL for 1.  The product of rank R is kept in fp32, or as a sum of 16-bit parts that
  * carries 16 bits or more of it (24 for bf16 with f32 outputs; f16 relative to the row's largest).  X, A, B

@@ -4,7 +4,8 @@
 //
 // where a = adapters[q] is the adapter of the request q that row i belongs to: offsets[q] <= i < offsets[q+1], or
 // q = i when no offsets are given (a decoding step).  An adapter number outside 0..adapters-1 means none: D[i] = C[i].
-// Rows outside every request are left as they were.  No counterpart in the reference.
+// Rows outside every request are left as they were.  A border below an earlier one counts as that one, so that requests
+// never share a row: both kernels then take a row once, by the same request.  No counterpart in the reference.
 //
 // The product of rank R between the two factors never leaves the chip: a thread-block cluster takes a row, CTA c of it
 // a slice of K for the first factor; the partial R-vectors meet through distributed shared memory (fp32, summed in CTA
@@ -68,17 +69,19 @@ lora_row_kernel(const LoraArgs g) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / kLoraCtas, rank = (int)cluster_ctarank();
   if (g.offsets) {
-    if (tid == 0) found = -1;
+    // the first request that ends behind the row, unless the row lies before all of them
+    if (tid == 0) found = g.requests;
     __syncthreads();
-    for (int q = tid; q < g.requests; q += kLoraThreads)
-      if (g.offsets[q] <= row && row < g.offsets[q + 1]) atomicMax(&found, q);
+    if (g.offsets[0] <= row)
+      for (int q = tid; q < g.requests; q += kLoraThreads)
+        if (row < g.offsets[q + 1]) atomicMin(&found, q);
     __syncthreads();
   } else if (tid == 0) {
     found = row;
   }
   __syncthreads();
   const int q = found;
-  if (q < 0) return;  // the same in every CTA of the cluster
+  if (q >= g.requests) return;  // the same in every CTA of the cluster
   const int a = g.which[q];
   const int n0 = (int)((long long)g.n * rank / kLoraCtas), n1 = (int)((long long)g.n * (rank + 1) / kLoraCtas);
   const OutT* c_row = static_cast<const OutT*>(g.C) + row * g.c_pitch;
@@ -289,23 +292,48 @@ __device__ __forceinline__ void lora_range(float m, float& down, float& up) {
 __device__ __forceinline__ void lora_find_tile(const LoraArgs& g, int want, int* sums, int* result) {
   const int tid = threadIdx.x, per = (g.requests + kLoraTileThreads - 1) / kLoraTileThreads;
   const int q0 = min(tid * per, g.requests), q1 = min(q0 + per, g.requests);
-  auto tiles_of = [&](int q, int& lo, int& hi) {
-    lo = min(max(__ldg(g.offsets + q), 0), g.rows);
-    hi = min(max(__ldg(g.offsets + q + 1), 0), g.rows);
-    return hi > lo ? (hi - lo + 127) >> 7 : 0;
+  auto border = [&](int q) { return min(max(__ldg(g.offsets + q), 0), g.rows); };
+  int high = 0;  // the largest border before q0, where that is not border(q0) itself
+  auto tiles_of = [&](int q, int& lo, int& hi) {  // in the order of q, from q0 on
+    if (q == q0) lo = max(border(q), high);
+    else lo = hi;
+    hi = max(border(q + 1), lo);
+    return (hi - lo + 127) >> 7;
   };
-  int mine = 0, lo, hi;
-  for (int q = q0; q < q1; ++q) mine += tiles_of(q, lo, hi);
-  if (tid == 0) result[0] = -1;
-  int incl = mine;
+  int before = 0, mine = 0, lo = 0, hi = 0;
+  bool back = false;
+  auto count = [&]() {  // tiles of this thread's requests, and of its warp's threads before it
+    mine = 0;
+    for (int q = q0; q < q1; ++q) {
+      mine += tiles_of(q, lo, hi);
+      back |= hi != border(q + 1);
+    }
+    int incl = mine;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(~0u, incl, d);
-    if ((tid & 31) >= d) incl += up;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, incl, d);
+      if ((tid & 31) >= d) incl += up;
+    }
+    if ((tid & 31) == 31) sums[tid >> 5] = incl;
+    before = incl - mine;
+  };
+  if (tid == 0) result[0] = -1;
+  count();
+  if (__syncthreads_or(back)) {
+    // a border runs backwards: the largest before each thread's requests, then again
+    int top = 0;
+    for (int q = q0; q < q1; ++q) top = max(top, border(q));
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_up_sync(~0u, top, d));
+    if ((tid & 31) == 31) sums[tid >> 5] = top;
+    high = __shfl_up_sync(~0u, top, 1);
+    if ((tid & 31) == 0) high = 0;
+    __syncthreads();
+    for (int w = 0; w < (tid >> 5); ++w) high = max(high, sums[w]);
+    __syncthreads();
+    count();
+    __syncthreads();
   }
-  if ((tid & 31) == 31) sums[tid >> 5] = incl;
-  __syncthreads();
-  int before = incl - mine;
   for (int w = 0; w < (tid >> 5); ++w) before += sums[w];
   if (before <= want && want < before + mine) {
     for (int q = q0; q < q1; ++q) {

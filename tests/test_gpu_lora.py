@@ -290,3 +290,38 @@ def test_scales_of_any_size_and_rows_of_zeros(mb, dev, case, kind, out):
         if ot != torch.float32:
             tol = tol + 2.0 ** -16 * mag + torch.finfo(ot).eps / 2 * want.abs() + torch.finfo(ot).tiny * torch.finfo(ot).eps
         assert bool(((got[s].double() - want).abs() <= tol).all())
+
+
+def running(offsets, rows):
+    """Borders inside the array, none below an earlier one."""
+    out, high = [], 0
+    for o in offsets:
+        high = max(high, min(max(o, 0), rows))
+        out.append(high)
+    return out
+
+
+# the last three reach the tiles of the tensor cores: two requests that ask for the same rows, borders that fall by one
+# in the middle of 400 requests (more than the CTA has threads), and a first border behind the rest
+BACKWARDS = [([0, 4, 1, 3, 9], 12, 64, 136, 16), ([-3, 5, 2, 7, 99], 9, 64, 136, 16), ([6, 2, 4, 8], 9, 64, 136, 16),
+             ([0, 3000, 0, 3000], 3000, 1024, 1000, 64),
+             ([40 * i - 41 * (i % 50 == 49) for i in range(401)], 16000, 512, 264, 24),
+             ([700, 0, 300, 1200, 1100, 2000, 5000], 3000, 1024, 131, 64)]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("case", range(len(BACKWARDS)))
+def test_borders_that_run_backwards(mb, dev, case, in_place):
+    """Every row belongs to one request at most, the same in both kernels, and is added to once."""
+    offsets, rows, k, n, rank = BACKWARDS[case]
+    which = [i % 5 - 1 for i in range(1, len(offsets))]
+    x, a, b, scales, w, edge = make((offsets, rows, which, n, k, rank, 4), "bf16", dev)
+    c = torch.randn(rows, n, device=dev)
+    d0 = c.clone() if in_place else torch.full_like(c, -3.0)
+    got = mb.gemm_lora_(d0.clone(), x, a, b, w, edge, scales, C=None if in_place else c)
+    if in_place:
+        got2 = c.clone()
+        mb.gemm_lora_(got2, x, a, b, w, edge, scales, C=got2)
+        assert torch.equal(got, got2)
+    mb.synchronize_status(dev)
+    check(got, c, x, a, b, scales, which, running(offsets, rows), torch.float32, d0)
