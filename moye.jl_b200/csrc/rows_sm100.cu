@@ -627,9 +627,9 @@ int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const mo
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "combine_rows_grad: elements of dweights overlap");
   if (weights->dtype != dweights->dtype) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "combine_rows_grad: weights and dweights differ in type");
   if (ddst->shape[0] == 0) return MOYE_OK;
-  if (ddst->shape[1] == 0) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "combine_rows_grad: rows of width 0");
-  if (!dsrc->ptr || !ddst->ptr || !src->ptr || !inverse) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: null pointer");
-  if (overlap(dsrc, src) || overlap(dsrc, ddst)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: dsrc overlaps an input");
+  const bool empty = ddst->shape[1] == 0;  // no rows to read or write: the weights' gradients are empty sums
+  if (!inverse || (!empty && (!dsrc->ptr || !ddst->ptr || !src->ptr))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: null pointer");
+  if (!empty && (overlap(dsrc, src) || overlap(dsrc, ddst))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: dsrc overlaps an input");
   RowArgs g = {};
   g.tokens = (int)ddst->shape[0];
   g.choices = choices;

@@ -278,3 +278,19 @@ def test_an_element_of_its_own_for_every_weight_gradient(mb, dev):
         mb.combine_rows_grad_(z(n, 16), good, ones[:shape[0]], ones[:n], p, w[:shape[0], :shape[1]])
         assert bool((good == 16).all())
     mb.synchronize_status(dev)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("choices", [2, 5])
+def test_rows_of_width_zero(mb, dev, choices, kind):
+    """Nothing to move; the gradients of the weights are empty sums."""
+    ids = ids_for(7, choices, 3, 31).to(dev)
+    plan = mb.group_rows(ids, 3)
+    x, ys = torch.empty(7, 0, dtype=DT[kind], device=dev), torch.empty(7 * choices, 0, dtype=DT[kind], device=dev)
+    w, dw = torch.ones(7, choices, device=dev), torch.full((7, choices), float("nan"), device=dev)
+    mb.gather_rows_(ys, x, plan)
+    mb.combine_rows_(x, ys, plan, w)
+    mb.combine_rows_grad_(ys, dw, x, ys, plan, w)
+    mb.combine_rows_grad_(ys.clone(), dw, x, ys, plan, w)
+    mb.synchronize_status(dev)
+    assert bool((dw == 0).all())
