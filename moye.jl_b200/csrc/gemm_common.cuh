@@ -26,7 +26,7 @@ struct GemmArgs {
   const float* bias;  // fused epilogue: D = act(alpha*acc + beta*C + bias)
   int bias_mode;      // 0 none, 1 one value per column n (length N), 2 one value per row m (length M)
   int act;            // 0 none, 1 relu, 2 gelu (erf form), 3 silu
-  void* D;            // output pointer and element strides, for the kernels that store D with plain stores
+  void* D;            // output pointer and element strides, for plain stores
   long long d_sm, d_sn;
   // stream-K tail of the 256 x 512 pair kernel (all zero / null when it is off)
   int sk_tiles;          // the last `sk_tiles` tiles of the schedule are cut in two along K (see gemm_wide.cu)
@@ -160,6 +160,39 @@ struct FixUp {
   bool release;            // hand the accumulator back after the last tensor-memory read
   int chunk0;              // the warp's slab holds 8 chunks of 32 columns; this call starts at chunk `chunk0`
 };
+
+// A TMA store writes whole 16-byte units: where the contiguous mode of D ends inside one, a box that reaches over the end
+// would also write the rest of the unit, which is not D's.  The threads store (or, EPI_RED, add) such a box themselves,
+// from the staging tile the warp has just filled.
+template <typename OutT, bool OUT_M_MAJOR>
+__device__ __forceinline__ bool box_over_ragged_end(const GemmArgs& g, int m0, int n0) {
+  constexpr int W = OUT_M_MAJOR ? 32 : 128 / (int)sizeof(OutT);
+  const int at = OUT_M_MAJOR ? m0 : n0, end = OUT_M_MAJOR ? g.M : g.N;
+  return at + W > end && (end * (int)sizeof(OutT) & 15) != 0;
+}
+template <typename OutT, bool OUT_M_MAJOR, bool ADD>
+__device__ __forceinline__ void store_box_by_threads(const GemmArgs& g, const uint8_t* sb, int m0, int n0, int lane) {
+  constexpr int W = OUT_M_MAJOR ? 32 : 128 / (int)sizeof(OutT);
+  OutT* d = static_cast<OutT*>(g.D);
+  auto put = [&](long long at, OutT v) {
+    if constexpr (ADD) v = __ldcg(d + at) + v;  // written by another CTA a moment ago: from L2
+    d[at] = v;
+  };
+  if constexpr (OUT_M_MAJOR) {  // [32 columns][32 rows]
+    const int end = min(32, g.N - n0);
+    if (m0 + lane < g.M)
+#pragma unroll 1
+      for (int j = 0; j < end; ++j) put(m0 + lane + (n0 + j) * g.d_sn, reinterpret_cast<const OutT*>(sb)[j * 32 + lane]);
+  } else {  // [32 rows][128 bytes], 16-byte units swizzled by the row
+    const int end = min(32, g.M - m0);
+#pragma unroll 1
+    for (int r = 0; r < end; ++r)
+      for (int e = lane; e < W && n0 + e < g.N; e += 32) {
+        const int byte = e * (int)sizeof(OutT);
+        put((m0 + r) * g.d_sm + n0 + e, *reinterpret_cast<const OutT*>(sb + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15)));
+      }
+  }
+}
 
 // Epilogue of one accumulator tile for one warp: its 32 TMEM lanes x BN columns go
 // TMEM -> registers -> (alpha, beta, convert) -> staging tile in shared memory -> TMA store.
@@ -346,7 +379,10 @@ __device__ __forceinline__ void epilogue_tile_impl(const GemmArgs& g, const CUte
       ++nstore;
       continue;
     }
-    if (lane == 0) {
+    if (box_over_ragged_end<OutT, OUT_M_MAJOR>(g, m0, n0 + c * SC)) {
+      store_box_by_threads<OutT, OUT_M_MAJOR, RED>(g, sb, m0, n0 + c * SC, lane);
+      if (lane == 0) tma_store_commit();  // an empty group: every box counts as one
+    } else if (lane == 0) {
       if constexpr (RED) {
         if constexpr (OUT_M_MAJOR) tma_reduce_add_2d(tmD, sb, m0, n0 + c * SC);
         else tma_reduce_add_2d(tmD, sb, n0 + c * SC, m0);

@@ -888,3 +888,77 @@ def test_random_decode_shapes_around_the_schedule_boundaries(mb, dev, seed):
         mb.synchronize_status(dev)
         err = ((C.double() - ref).abs().max() / ref.abs().max().clamp_min(1e-6)).item()
         assert err <= (5e-3 if C.dtype == torch.float32 else 2e-2), (case, M, N, K, path, C.dtype, err)
+
+
+RAGGED = [dict(path=1, tile_n=64), dict(path=1, tile_n=256), dict(path=3, tile_n=128), dict(path=3, tile_n=256), dict(path=4, tail=False),
+          dict(path=4, tail=True), dict(path=5, split_k=2), dict(path=2), dict(path=0)]
+
+
+@pytest.mark.parametrize("m_major", [False, True])
+@pytest.mark.parametrize("kind", ["f16-f16", "bf16-f32", "s8-s32", "e4m3-bf16", "f32-f32"])
+@pytest.mark.parametrize("how", range(len(RAGGED)))
+def test_what_lies_behind_rows_that_end_inside_16_bytes(mb, dev, how, kind, m_major):
+    """D is a view into a wider array, its contiguous extent no multiple of 16 bytes: nothing beside it is written, and its
+    values are those of the product with rows of whole 16-byte units, where the same kernel runs.  Off by at most one cut of
+    2^-23 per product and the output's rounding from the exact value (integers: equal)."""
+    kw = dict(RAGGED[how])
+    small = kw["path"] == 2
+    M, N, K = (75 if small else 301), 1003, 1008
+    types = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32, "s32": torch.int32, "e4m3": torch.float8_e4m3fn}
+    kin, kout = kind.split("-")
+    ot = types[kout]
+    if small and kin not in ("f16", "bf16"):
+        pytest.skip("the decode kernel takes 16-bit operands")
+    gen = torch.Generator(device=dev).manual_seed(3)
+
+    def operand(rows):
+        if kin == "s8":
+            return torch.randint(-128, 128, (rows, K), generator=gen, device=dev, dtype=torch.int8)
+        return (torch.rand(rows, K, generator=gen, device=dev) * 2 - 1).to(types[kin])
+
+    up = lambda x: (x + 15) // 16 * 16
+    A, B = operand(up(M)), operand(up(N))  # as many rows as a D of whole 16-byte units needs
+    filler = 77
+
+    def product(m, n, alpha, beta):
+        inner, outer = (m, n) if m_major else (n, m)
+        wide = torch.full((outer + 1, up(inner) + 32), filler, device=dev, dtype=ot)
+        view = wide[:outer, 16:16 + inner]
+        d = view.t() if m_major else view
+        if beta:
+            d.copy_((torch.arange(m, device=dev)[:, None] * 3 + torch.arange(n, device=dev)[None, :]) % 17)
+        c = d.clone()
+        D = mb.MoYeArray(d)
+        mb.gemm_(D, mb.MoYeArray(A[:m]), mb.MoYeArray(B[:n]), D if beta else None, alpha=alpha, beta=beta, **kw)
+        mb.synchronize_status(dev)
+        beside = wide.clone()
+        beside[:outer, 16:16 + inner] = filler
+        assert bool((beside == filler).all()), "the product wrote outside D"
+        want = alpha * (A[:m].double() @ B[:n].double().T) + beta * c.double()
+        if kin == "s8":
+            assert torch.equal(d.double(), want)
+        else:
+            mag = abs(alpha) * (A[:m].double().abs() @ B[:n].double().abs().T) + abs(beta) * c.double().abs()
+            tol = (K + 8) * 2.0 ** -23 * mag + (torch.finfo(ot).eps / 2 * want.abs() if ot != torch.float32 else 0)
+            assert bool(((d.double() - want).abs() <= tol).all())
+        return d.clone()
+
+    for alpha, beta in ((1.0, 0.0),) if small else ((1.0, 0.0), (1.0, 1.0)) if kin == "s8" else ((1.0, 0.0), (0.5, 1.0)):
+        got = product(M, N, alpha, beta)
+        if kw["path"] not in (0, 2):
+            whole = product(up(M) if m_major else M, N if m_major else up(N), alpha, beta)
+            assert torch.equal(got, whole[:M, :N])
+
+
+def test_the_last_row_of_an_array_that_ends_inside_16_bytes(mb, dev):
+    """One row, and several, whose last element is the last of its memory's view: what comes behind stays."""
+    A, B = torch.ones(200, 64, device=dev).half(), torch.ones(131, 64, device=dev).half()
+    for rows, path in ((1, 1), (200, 1), (200, 3)):
+        flat = torch.full((rows * 136 + 16,), 7.0, device=dev, dtype=torch.float16)
+        d = flat[:rows * 136].view(rows, 136)[:, :131]
+        mb.matmul(A[:rows], B, d, path=path)
+        mb.synchronize_status(dev)
+        assert bool((d == 64).all())
+        rest = flat.clone()
+        rest[:rows * 136].view(rows, 136)[:, :131] = 7
+        assert bool((rest == 7).all())
