@@ -168,7 +168,7 @@ template <typename OutT, bool OUT_M_MAJOR>
 __device__ __forceinline__ bool box_over_ragged_end(const GemmArgs& g, int m0, int n0) {
   constexpr int W = OUT_M_MAJOR ? 32 : 128 / (int)sizeof(OutT);
   const int at = OUT_M_MAJOR ? m0 : n0, end = OUT_M_MAJOR ? g.M : g.N;
-  return at + W > end && (end * (int)sizeof(OutT) & 15) != 0;
+  return at + W > end && end % (16 / (int)sizeof(OutT)) != 0;
 }
 template <typename OutT, bool OUT_M_MAJOR, bool ADD>
 __device__ __forceinline__ void store_box_by_threads(const GemmArgs& g, const uint8_t* sb, int m0, int n0, int lane) {
