@@ -9,8 +9,11 @@
 // (V 128-bit reads along the source rows, V 128-bit writes along the destination rows) into a second swizzled
 // tile, and TMA stores it.  The thread -> block map walks diagonals, which makes every 8-lane phase of both the
 // reads and the writes touch 8 distinct 16-byte bank groups: no padding, no bank conflicts.  Loads run one
-// stage ahead of the stores, four CTAs per SM.  Ragged edges need no code: TMA zero-fills loads and clips stores.
+// stage ahead of the stores, four CTAs per SM.  Ragged edges: TMA zero-fills loads and clips stores, but at whole 16-byte
+// units; where a destination row ends inside one, the box over its end is stored by threads.
 // HBM-bound: algorithmic traffic is one read plus one write of the tensor.
+#include <type_traits>
+
 #include "common.h"
 #include "ptx.cuh"
 
@@ -23,6 +26,9 @@ struct TransposeArgs {
   int tiles_m;  // stages along m
   long long tiles;
   int* status;
+  void* dst;    // for the box over the end of rows that end inside 16 bytes
+  long long dst_pitch;  // elements
+  int n;
 };
 
 // Tile order: m fastest.  A banded two-dimensional order (contiguous spans in both the source and the destination
@@ -123,6 +129,7 @@ __global__ void __launch_bounds__(64 * RM_) transpose_tma_kernel(const __grid_co
   const int t8 = lane & 7;
   const int bi = t8 + (RM_ == 2 ? 8 * (warp & 1) : 0);
   const int bj = (t8 + (lane >> 3) + 4 * (RM_ == 2 ? (warp >> 1) : warp)) & 7;
+  const bool ragged = a.m % V != 0;
   bool failed = false;
   for (long long i = 0; i < mine; ++i) {
     const int slot = (int)(i % SLOTS);
@@ -154,14 +161,27 @@ __global__ void __launch_bounds__(64 * RM_) transpose_tma_kernel(const __grid_co
     }
     fence_proxy_async_smem();
     __syncthreads();
-    if (tid == 0) {
+    if (ragged || tid == 0) {
       int tm, tn;
       transpose_tile_coord(first + i * stride, a, tm, tn);
       const int m0 = tm * Cfg::ROWS, n0 = tn * Cfg::COLS;
       uint8_t* o = out + (int)(i & 1) * STAGE;
-      tma_store_2d(&tmD, o, m0, n0);
-      if (RM_ == 2 && m0 + 8 * V < a.m) tma_store_2d(&tmD, o + Cfg::OUT_HALF, m0 + 8 * V, n0);
-      tma_store_commit();
+      if (ragged && m0 + Cfg::ROWS > a.m) {
+        using Raw = typename std::conditional<E == 8, uint2, typename std::conditional<E == 4, uint32_t,
+                    typename std::conditional<E == 2, uint16_t, uint8_t>::type>::type>::type;
+        Raw* d = static_cast<Raw*>(a.dst);
+        const int rows = min(Cfg::COLS, a.n - n0), here = a.m - m0;
+        for (int at = tid; at < rows * Cfg::ROWS; at += 64 * RM_) {
+          const int r = at / Cfg::ROWS, e = at % Cfg::ROWS, byte = e % (8 * V) * E;
+          if (e < here)
+            d[(long long)(n0 + r) * a.dst_pitch + m0 + e] =
+                *reinterpret_cast<const Raw*>(o + e / (8 * V) * Cfg::OUT_HALF + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+        }
+      } else if (tid == 0) {
+        tma_store_2d(&tmD, o, m0, n0);
+        if (RM_ == 2 && m0 + 8 * V < a.m) tma_store_2d(&tmD, o + Cfg::OUT_HALF, m0 + 8 * V, n0);
+      }
+      if (tid == 0) tma_store_commit();  // possibly empty: every stage counts as one
     }
   }
   if (tid == 0) {
@@ -174,14 +194,17 @@ __global__ void __launch_bounds__(64 * RM_) transpose_tma_kernel(const __grid_co
 }
 
 template <int E, int SLOTS_ = 2, int NB_ = 0, int RM_ = 1>
-static int launch_transpose_inst(moye_b200_ctx* h, const CUtensorMap& ts, const CUtensorMap& td, int64_t m, int64_t n,
-                                 cudaStream_t stream) {
+static int launch_transpose_inst(moye_b200_ctx* h, const CUtensorMap& ts, const CUtensorMap& td, void* dst, int64_t dst_pitch, int64_t m,
+                                 int64_t n, cudaStream_t stream) {
   using Cfg = TransposeCfg<E, SLOTS_, NB_, RM_>;
   TransposeArgs a;
   a.m = (int)m;
   a.tiles_m = (int)((m + Cfg::ROWS - 1) / Cfg::ROWS);
   a.tiles = (long long)a.tiles_m * ((n + Cfg::COLS - 1) / Cfg::COLS);
   a.status = h->d_status;
+  a.dst = dst;
+  a.dst_pitch = dst_pitch;
+  a.n = (int)n;
   auto kern = transpose_tma_kernel<E, SLOTS_, NB_, RM_>;
   if (int rc = configure_once(h, kern, Cfg::SMEM)) return rc;
   // Measured on 8192^2 (fp16 / fp32): 2 slots of 8 KB with 4 CTAs per SM reach 5.7 / 6.0 TB/s; deeper rings, larger
@@ -213,10 +236,10 @@ int launch_transpose(moye_b200_ctx* h, void* dst, int64_t dst_pitch, const void*
   if (int rc = make_tmap_2d(h, &ts, src, dtype, n, m, (uint64_t)src_pitch * eb, 8 * V, 8 * V * rm, TMAP_SWIZZLE_128B)) return rc;
   if (int rc = make_tmap_2d(h, &td, dst, dtype, m, n, (uint64_t)dst_pitch * eb, 8 * V, 8 * V * nb, TMAP_SWIZZLE_128B)) return rc;
   switch (eb) {
-    case 1: return launch_transpose_inst<1>(h, ts, td, m, n, stream);
-    case 2: return launch_transpose_inst<2>(h, ts, td, m, n, stream);
-    case 4: return launch_transpose_inst<4>(h, ts, td, m, n, stream);
-    default: return launch_transpose_inst<8>(h, ts, td, m, n, stream);
+    case 1: return launch_transpose_inst<1>(h, ts, td, dst, dst_pitch, m, n, stream);
+    case 2: return launch_transpose_inst<2>(h, ts, td, dst, dst_pitch, m, n, stream);
+    case 4: return launch_transpose_inst<4>(h, ts, td, dst, dst_pitch, m, n, stream);
+    default: return launch_transpose_inst<8>(h, ts, td, dst, dst_pitch, m, n, stream);
   }
 }
 

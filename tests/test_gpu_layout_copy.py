@@ -275,3 +275,22 @@ def test_ldmatrix_tiled_copy_refuses_what_the_instruction_cannot_do(mb, dev):
     f32 = torch.zeros(1024, device=dev)
     with pytest.raises(mb.MoyeError):    # 32-bit elements
         mb.copyto_(tiled_copy, mb.MoYeArray(f32, mb.make_layout((32, 32))), mb.MoYeArray(f32, mb.make_layout((32, 32))))
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float16, torch.float32, torch.int64])
+@pytest.mark.parametrize("m,n", [(1, 5), (129, 3), (1001, 70), (257, 1003), (3001, 2049)])
+def test_transposing_copy_of_rows_that_end_inside_16_bytes(mb, dev, dtype, m, n):
+    """Destination columns whose length is no multiple of 16 bytes, in a longer array: what lies behind each stays."""
+    up = lambda x: (x + 15) // 16 * 16
+    lds, ldd = up(n) + 16, up(m) + 16
+    src = torch.randint(-100, 100, (m, lds), device=dev).to(dtype)
+    dst = torch.full((n + 1, ldd), 7, device=dev).to(dtype)
+    for mirrored in (False, True):
+        dst.fill_(7)
+        S, D = mb.MoYeArray(src.view(-1), mb.make_layout((m, n), (lds, 1))), mb.MoYeArray(dst.view(-1), mb.make_layout((m, n), (1, ldd)))
+        if mirrored:
+            S, D = mb.MoYeArray(src.view(-1), mb.make_layout((n, m), (1, lds))), mb.MoYeArray(dst.view(-1), mb.make_layout((n, m), (ldd, 1)))
+        mb.copyto_(D, S)
+        mb.synchronize_status(dev)
+        assert torch.equal(dst[:n, :m], src[:, :n].t())
+        assert bool((dst[n:] == 7).all()) and bool((dst[:, m:] == 7).all()), "the copy wrote outside the destination view"
