@@ -298,7 +298,8 @@ int moye_b200_group_rows(moye_handle_t h, const moye_tensor_t* ids, int32_t grou
 
 /* dst[inverse[t*choices + j]] = src[t]: every token's row to the positions of its choices.  src (tokens, width), dst
  * (tokens * choices, width), contiguous rows, any element type of 1, 2, 4 or 8 bytes.  Rows of dst at which nothing
- * arrives are left as they were.  dst and src must not overlap. */
+ * arrives are left as they were.  dst and src must not overlap (they may lie beside one another
+ * in a wider array). */
 int moye_b200_gather_rows(moye_handle_t h, const moye_tensor_t* dst, const moye_tensor_t* src, const int32_t* inverse,
                           int32_t choices, void* stream);
 

@@ -159,6 +159,29 @@ int encode_tmap_2d_uncached(CUtensorMap* out, const void* ptr, int dtype, uint64
 int encode_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, uint64_t dim0, uint64_t dim1, uint64_t dim2,
                    uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, bool swizzle128);
 
+// Whether two matrices of contiguous rows share a byte.  Rows of one pitch may lie beside one another in a wider array;
+// matrices of different pitches are refused for what lies between their ends.
+inline bool rows_overlap(const moye_tensor_t* a, const moye_tensor_t* b) {
+  struct Rows { long long count, width, pitch; };
+  auto rows_of = [](const moye_tensor_t* t) {
+    const long long e = dtype_bytes(t->dtype);
+    const bool one = t->shape[0] == 1 || t->stride[0] == 0;  // the same row again and again is one
+    return Rows{one && t->shape[0] > 0 ? 1 : t->shape[0], t->shape[1] * e, one ? 0 : t->stride[0] * e};
+  };
+  const Rows ra = rows_of(a), rb = rows_of(b);
+  if (ra.count <= 0 || rb.count <= 0 || ra.width <= 0 || rb.width <= 0) return false;
+  const long long apart = static_cast<const char*>(b->ptr) - static_cast<const char*>(a->ptr);
+  if (apart >= (ra.count - 1) * ra.pitch + ra.width || -apart >= (rb.count - 1) * rb.pitch + rb.width) return false;
+  if (ra.count > 1 && rb.count > 1 && ra.pitch != rb.pitch) return true;
+  const long long pitch = ra.count > 1 ? ra.pitch : rb.pitch;
+  if (pitch <= 0) return true;
+  // row j of b starts apart + (j - i) * pitch behind row i of a; the first difference at which it ends behind that row's start
+  const long long behind = -rb.width - apart;
+  long long k = (behind >= 0 ? behind / pitch : -((-behind + pitch - 1) / pitch)) + 1;
+  if (k < 1 - ra.count) k = 1 - ra.count;
+  return k < rb.count && apart + k * pitch < ra.width;
+}
+
 // Raises a kernel's dynamic shared-memory limit the first time this handle launches it.
 template <typename K>
 inline int configure_once(moye_b200_ctx* h, K kernel, int smem_bytes) {

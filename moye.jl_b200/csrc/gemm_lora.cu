@@ -961,13 +961,9 @@ int launch_gemm_lora(moye_b200_ctx* h, const moye_tensor_t* D, const moye_tensor
   for (const moye_tensor_t* t : {D, C})
     if ((N > 1 && t->stride[1] != 1) || (T > 1 && t->stride[0] < N))
       MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "gemm_lora: rows of C and D must be contiguous and must not overlap");
-  auto overlap = [](const moye_tensor_t* a, const moye_tensor_t* b) {
-    auto end = [](const moye_tensor_t* t) { return static_cast<const char*>(t->ptr) + ((t->shape[0] - 1) * t->stride[0] + t->shape[1]) * dtype_bytes(t->dtype); };
-    return a->ptr < static_cast<const void*>(end(b)) && b->ptr < static_cast<const void*>(end(a));
-  };
-  if (overlap(C, D) && !(C->ptr == D->ptr && (T == 1 || C->stride[0] == D->stride[0])))
+  if (rows_overlap(C, D) && !(C->ptr == D->ptr && (T == 1 || C->stride[0] == D->stride[0])))
     MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: C and D overlap without being the same");
-  if (overlap(X, D)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: X and D overlap");
+  if (rows_overlap(X, D)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gemm_lora: X and D overlap");
   LoraArgs g = {};
   g.rows = (int)T;
   g.requests = requests;

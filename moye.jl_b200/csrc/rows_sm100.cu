@@ -504,12 +504,6 @@ static int check_rows(const char* who, const moye_tensor_t* token_side, const mo
   return MOYE_OK;
 }
 
-static bool overlap(const moye_tensor_t* a, const moye_tensor_t* b) {
-  auto span = [](const moye_tensor_t* t) { return ((t->shape[0] - 1) * t->stride[0] + t->shape[1]) * (long long)dtype_bytes(t->dtype); };
-  const char *pa = static_cast<const char*>(a->ptr), *pb = static_cast<const char*>(b->ptr);
-  return pa < pb + span(b) && pb < pa + span(a);
-}
-
 static bool rows_on_16_bytes(const moye_tensor_t* t) {
   const int eb = dtype_bytes(t->dtype);
   return (reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && (t->shape[1] * eb) % 16 == 0 &&
@@ -531,7 +525,7 @@ int launch_gather_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_tens
   if (eb != 1 && eb != 2 && eb != 4 && eb != 8) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "gather_rows: elements of 1, 2, 4 or 8 bytes");
   if (src->shape[0] == 0 || src->shape[1] == 0) return MOYE_OK;
   if (!dst->ptr || !src->ptr || !inverse) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gather_rows: null pointer");
-  if (overlap(dst, src)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gather_rows: dst and src overlap");
+  if (rows_overlap(dst, src)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "gather_rows: dst and src overlap");
   RowArgs g = {};
   g.tokens = (int)src->shape[0];
   g.choices = choices;
@@ -586,7 +580,7 @@ int launch_combine_rows(moye_b200_ctx*, const moye_tensor_t* dst, const moye_ten
     if (int rc = check_weights("combine_rows", weights, dst->shape[0], choices)) return rc;
   if (dst->shape[0] == 0 || dst->shape[1] == 0) return MOYE_OK;
   if (!dst->ptr || !src->ptr || !inverse) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows: null pointer");
-  if (overlap(dst, src)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows: dst and src overlap");
+  if (rows_overlap(dst, src)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows: dst and src overlap");
   RowArgs g = {};
   g.tokens = (int)dst->shape[0];
   g.choices = choices;
@@ -629,7 +623,7 @@ int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const mo
   if (ddst->shape[0] == 0) return MOYE_OK;
   const bool empty = ddst->shape[1] == 0;  // no rows to read or write: the weights' gradients are empty sums
   if (!inverse || (!empty && (!dsrc->ptr || !ddst->ptr || !src->ptr))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: null pointer");
-  if (!empty && (overlap(dsrc, src) || overlap(dsrc, ddst))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: dsrc overlaps an input");
+  if (!empty && (rows_overlap(dsrc, src) || rows_overlap(dsrc, ddst))) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "combine_rows_grad: dsrc overlaps an input");
   RowArgs g = {};
   g.tokens = (int)ddst->shape[0];
   g.choices = choices;

@@ -325,3 +325,22 @@ def test_borders_that_run_backwards(mb, dev, case, in_place):
         assert torch.equal(got, got2)
     mb.synchronize_status(dev)
     check(got, c, x, a, b, scales, which, running(offsets, rows), torch.float32, d0)
+
+
+@pytest.mark.parametrize("case", [([0, 3, 9], 9, [1, 0], 64, 64, 16, 2), ([0, 3000], 3000, [1], 520, 520, 64, 2)])
+def test_columns_of_one_wider_array(mb, dev, case):
+    offsets, rows, which, n, k, rank, count = case
+    x, a, b, scales, w, edge = make(case, "bf16", dev)
+    c = torch.randn(rows, n, device=dev).bfloat16()
+    wide = torch.zeros(rows, k + 2 * n, dtype=torch.bfloat16, device=dev)
+    xs, cs, d = wide[:, :k], wide[:, k:k + n], wide[:, k + n:]
+    xs.copy_(x)
+    cs.copy_(c)
+    got = mb.gemm_lora_(d, xs, a, b, w, edge, scales, C=cs)
+    mb.synchronize_status(dev)
+    check(got, c, x, a, b, scales, which, offsets, torch.bfloat16, d)
+    assert torch.equal(xs, x) and torch.equal(cs, c)
+    for kw in ({"C": wide[:, k + n - 8:k + 2 * n - 8]}, {"C": None}):
+        with pytest.raises(mb.MoyeError) as e:
+            mb.gemm_lora_(d if kw["C"] is not None else wide[:, k - 8:k + n - 8], xs, a, b, w, edge, scales, **kw)
+        assert e.value.code == -1

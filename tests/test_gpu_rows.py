@@ -294,3 +294,32 @@ def test_rows_of_width_zero(mb, dev, choices, kind):
     mb.combine_rows_grad_(ys.clone(), dw, x, ys, plan, w)
     mb.synchronize_status(dev)
     assert bool((dw == 0).all())
+
+
+def test_columns_of_one_wider_array(mb, dev):
+    """Arrays that lie beside one another in one buffer share no element; shifted by a column they do."""
+    tokens, choices, width = 37, 2, 40
+    ids = ids_for(tokens, choices, 5, 37).to(dev)
+    plan = mb.group_rows(ids, 5)
+    x, ys, w, dy = data(tokens, choices, width, torch.bfloat16, dev)
+    n = tokens * choices
+    wide = torch.zeros(n, 4 * width, dtype=torch.bfloat16, device=dev)
+    part = lambda i, rows=n, shift=0: wide[:rows, i * width + shift:(i + 1) * width + shift]
+    refused = lambda fn, *args: pytest.raises(mb.MoyeError, fn, *args).value.code == -1
+    part(0, tokens).copy_(x)
+    mb.gather_rows_(part(1), part(0, tokens), plan)
+    kept = int(plan.offsets[-1])
+    assert torch.equal(part(1)[:kept], x[plan.order[:kept].long() // choices])
+    part(2).copy_(ys)
+    part(0, tokens).copy_(dy)
+    want = mb.combine_rows_grad_(torch.zeros_like(ys), torch.zeros_like(w), dy, ys, plan, w)
+    got = mb.combine_rows_grad_(part(3), torch.zeros_like(w), part(0, tokens), part(2), plan, w)
+    assert torch.equal(got[0][:kept], want[0][:kept]) and torch.equal(got[1], want[1])
+    mb.combine_rows_(part(0, tokens), part(2), plan, w)
+    assert torch.equal(part(0, tokens), mb.combine_rows_(torch.empty_like(x), ys, plan, w))
+    for shift in (-1, 1):
+        assert refused(mb.gather_rows_, part(1), part(1 + shift, tokens, -shift), plan)
+        assert refused(mb.combine_rows_, part(1 + shift, tokens, -shift), part(1), plan, w)
+        assert refused(mb.combine_rows_grad_, part(1), w.clone(), part(3, tokens), part(1 + shift, n, -shift), plan, w)
+    assert refused(mb.gather_rows_, part(1), wide.view(-1)[:tokens * width].view(tokens, width), plan)  # another pitch, the same memory
+    mb.synchronize_status(dev)
