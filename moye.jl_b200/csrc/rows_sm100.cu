@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdlib>
+#include <numeric>
 
 #include "common.h"
 #include "ptx.cuh"
@@ -615,9 +616,9 @@ int launch_combine_rows_grad(moye_b200_ctx*, const moye_tensor_t* dsrc, const mo
   if (int rc = check_rows("combine_rows_grad", ddst, dsrc, dsrc, choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", weights, ddst->shape[0], choices)) return rc;
   if (int rc = check_weights("combine_rows_grad", dweights, ddst->shape[0], choices)) return rc;
-  // any order of the modes, but an element of its own for every choice (no broadcast output)
-  const long long T = dweights->shape[0], st = std::llabs(dweights->stride[0]), sc = std::llabs(dweights->stride[1]);
-  if (st > sc ? choices > 1 && (sc == 0 || (T > 1 && st < choices * sc)) : (T > 1 && st == 0) || (choices > 1 && T > 1 && sc < T * st))
+  // any strides that give every choice an element of its own (no broadcast output): two meet at the least common multiple
+  const long long T = dweights->shape[0], st = std::llabs(dweights->stride[0]), sc = std::llabs(dweights->stride[1]), both = std::gcd(st, sc);
+  if ((T > 1 && st == 0) || (choices > 1 && sc == 0) || (T > 1 && choices > 1 && sc / both < T && st / both < choices))
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "combine_rows_grad: elements of dweights overlap");
   if (weights->dtype != dweights->dtype) MOYE_FAIL(MOYE_ERR_UNSUPPORTED_DTYPE, "combine_rows_grad: weights and dweights differ in type");
   if (ddst->shape[0] == 0) return MOYE_OK;

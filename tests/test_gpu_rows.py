@@ -323,3 +323,37 @@ def test_columns_of_one_wider_array(mb, dev):
         assert refused(mb.combine_rows_grad_, part(1), w.clone(), part(3, tokens), part(1 + shift, n, -shift), plan, w)
     assert refused(mb.gather_rows_, part(1), wide.view(-1)[:tokens * width].view(tokens, width), plan)  # another pitch, the same memory
     mb.synchronize_status(dev)
+
+
+def test_weight_gradients_that_interleave(mb, dev):
+    """Strides whose rows lie in one another without sharing an element."""
+    plan = mb.group_rows(torch.zeros(4, 3, dtype=torch.int64, device=dev), 3)
+    ones, w = torch.ones(12, 16, device=dev), torch.ones(4, 3, device=dev)
+    for stride in ((5, 2), (2, 9), (7, 3), (3, 4), (4, 3)):
+        flat = torch.zeros(64, device=dev)
+        mb.combine_rows_grad_(torch.zeros(12, 16, device=dev), flat.as_strided((4, 3), stride), ones[:4], ones, plan, w)
+        assert bool((flat.as_strided((4, 3), stride) == 16).all()) and int((flat != 0).sum()) == 12
+    for stride in ((4, 2), (2, 3), (3, 3), (2, 6)):
+        with pytest.raises(mb.MoyeError) as e:
+            mb.combine_rows_grad_(torch.zeros(12, 16, device=dev), torch.zeros(64, device=dev).as_strided((4, 3), stride), ones[:4], ones, plan, w)
+        assert e.value.code == -3
+    mb.synchronize_status(dev)
+
+
+@pytest.mark.parametrize("wt", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_gradients_with_16_bit_weights(mb, dev, kind, wt):
+    """Weights and their gradients in 16 bits: the dot product of `width` terms in fp32, then one rounding."""
+    tokens, choices, width = 130, 5, 72
+    plan = mb.group_rows(ids_for(tokens, choices, 9, 41).to(dev), 9)
+    x, ys, w, dy = data(tokens, choices, width, DT[kind], dev)
+    w = w.to(DT[wt])
+    d_ys, d_w = mb.combine_rows_grad_(torch.full_like(ys, float("nan")), torch.full_like(w, float("nan")), dy, ys, plan, w)
+    mb.synchronize_status(dev)
+    inv, kept = plan.inverse.long(), int(plan.offsets[-1])
+    has = inv >= 0
+    at = plan.order[:kept].long()
+    want = dy.double()[at // choices] * w.double().reshape(-1)[at][:, None]
+    assert close(d_ys[:kept], want, want.abs(), 1, DT[kind]) and bool(d_ys[kept:].isnan().all())
+    prod = torch.where(has[:, :, None], ys.double()[inv.clamp(min=0)], 0.0) * dy.double()[:, None, :]
+    assert close(d_w, prod.sum(2), prod.abs().sum(2), width, DT[wt]) and bool((d_w[~has] == 0).all())
