@@ -11,6 +11,8 @@ import os
 import struct
 import threading
 
+from .build import calls_marker
+
 MAX_RANK = 4
 MAX_FLAT_RANK = 12
 
@@ -139,10 +141,14 @@ def load():
 
 
 def _load_calls(lib):
-    """csrc/calls.cpp, bound to the entry points of `lib`.  None where it was not built, or for another torch than the one
-    that runs: the calls then take the way through ctypes into the same entry points, at more of the host's time."""
+    """csrc/calls.cpp, bound to the entry points of `lib`.  None where it was not built, or for another torch, interpreter
+    or version of the library than the ones that run: the calls then take the way through ctypes into the same entry
+    points, at more of the host's time."""
     path = os.path.join(os.path.dirname(LIB_PATH), "moye_calls.so")
     try:
+        with open(path, "rb") as f:
+            if calls_marker(lib.moye_b200_version()) not in f.read():
+                return None
         import torch  # noqa: F401  the module's own libraries
         loader = importlib.machinery.ExtensionFileLoader("moye_calls", path)
         mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("moye_calls", path, loader=loader))

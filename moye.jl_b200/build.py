@@ -10,6 +10,7 @@ a violation through the status word instead of touching memory.
 """
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -36,9 +37,25 @@ def _newer(path, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def calls_built_for():
+    """What the compiled module of the row-group calls depends on: it reads tensors by torch's own layout of them."""
+    import torch
+    return f"torch {torch.__version__} {sys.implementation.cache_tag}"
+
+
+def calls_marker(library_version, built_for=None):
+    """The bytes by which moye_calls.so says what it was built for."""
+    return f"moye_calls for {built_for or calls_built_for()}, library {library_version};".encode()
+
+
 def build_calls(force=False):
     """Compile csrc/calls.cpp, a Python extension module; returns its path."""
     src = os.path.join(CSRC, "calls.cpp")
+    with open(os.path.join(CSRC, HEADERS[-1])) as f:
+        version = re.search(r"#define MOYE_B200_VERSION (\d+)", f.read()).group(1)
+    if os.path.exists(OUT_CALLS):
+        with open(OUT_CALLS, "rb") as f:
+            force = force or calls_marker(version) not in f.read()
     torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
     if not force and not _newer(OUT_CALLS, [src, os.path.join(CSRC, HEADERS[-1]), os.path.join(torch_dir, "version.py"), os.path.abspath(__file__)]):
         return OUT_CALLS
@@ -47,7 +64,7 @@ def build_calls(force=False):
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")]
     import torch
-    res = subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
+    res = subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f'-DMOYE_BUILT_FOR="{calls_built_for()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
                          [x for i in include for x in ("-isystem", i)] +
                          [src, "-o", OUT_CALLS, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
                          capture_output=True, text=True)

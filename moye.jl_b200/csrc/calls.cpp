@@ -14,6 +14,12 @@
 
 #include "../../include/moye_b200.h"
 
+// Read from the file before anything of it runs: another torch or interpreter may lay its objects out differently.
+#define MOYE_TEXT2(x) #x
+#define MOYE_TEXT(x) MOYE_TEXT2(x)
+extern "C" __attribute__((used, visibility("default"))) const char moye_calls_built_for[] =
+    "moye_calls for " MOYE_BUILT_FOR ", library " MOYE_TEXT(MOYE_B200_VERSION) ";";
+
 namespace {
 
 struct Entries {

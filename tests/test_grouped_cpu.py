@@ -77,3 +77,26 @@ def test_without_the_compiled_calls_there_is_the_way_through_ctypes(mb, tmp_path
     assert mb._lib._load_calls(lib) is None                    # not built
     (tmp_path / "moye_calls.so").write_bytes(b"no library")
     assert mb._lib._load_calls(lib) is None                    # cannot be loaded
+
+
+def test_compiled_calls_for_another_torch_are_not_loaded(mb, tmp_path, monkeypatch):
+    """The module reads tensors by torch's layout of them: one that was built for another torch, interpreter or version of
+    the library is left alone, and built again."""
+    import shutil
+    import sys
+
+    lib = mb._lib.load()
+    build = sys.modules[mb._lib.calls_marker.__module__]
+    own = open(build.OUT_CALLS, "rb").read()
+    marker = mb._lib.calls_marker(lib.moye_b200_version())
+    assert marker in own and torch.__version__.encode() in marker and sys.implementation.cache_tag.encode() in marker
+    monkeypatch.setattr(mb._lib, "LIB_PATH", str(tmp_path / "libmoye_b200.so"))
+    other = tmp_path / "moye_calls.so"
+    shutil.copy(build.OUT_CALLS, other)
+    assert mb._lib._load_calls(lib) is not None
+    for a, b in ((torch.__version__, "0" * len(torch.__version__)), (sys.implementation.cache_tag, "x" * len(sys.implementation.cache_tag)),
+                 (f"library {lib.moye_b200_version()}", "library 999")):
+        other.write_bytes(own.replace(marker, marker.replace(a.encode(), b.encode())))
+        assert mb._lib._load_calls(lib) is None
+    monkeypatch.setattr(build, "OUT_CALLS", str(other))
+    assert marker in open(build.build_calls(), "rb").read()
