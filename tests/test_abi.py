@@ -121,3 +121,12 @@ def test_cpp_caller_links_and_reports_no_device(mb, tmp_path):
     mb._lib.load()
     res = subprocess.run([build_c_abi_smoke(tmp_path)], capture_output=True, text=True)
     assert res.returncode == 3 and "no CPU path" in res.stdout, res.stdout + res.stderr
+
+
+def test_every_entry_point_stands_in_the_documented_table():
+    """The table of entry points beside their counterparts: rows that open with a function's name, later ones of a row short."""
+    import glob
+    rows = [line.split("|")[1] for path in glob.glob(os.path.join(ROOT, "*.md")) for line in open(path) if line.startswith("| `moye_b200_")]
+    named = set(re.findall(r"[a-z_0-9]+", " ".join(rows)))
+    missing = [n for n in declared_functions() if n not in named and n[len("moye_b200_"):] not in named]
+    assert not missing, missing
