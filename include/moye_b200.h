@@ -326,7 +326,7 @@ int moye_b200_gemm_grouped(moye_handle_t h, const moye_tensor_t* D, const moye_t
 
 /* The gradient of the weights: dB[g] = alpha * sum over the rows i of group g of dD[i]^T A[i], + beta * dB[g].  Every
  * dB[g] is written: an empty group's becomes beta * dB[g].  Rows behind offsets[groups] are not used, whatever they
- * hold.  A (rows, K) and dD (rows, N) f16 or bf16, contiguous rows, base and pitch multiples of 16 bytes; dB
+ * hold.  Subnormal values are kept, beta = 1 (added by the memory) included.  A (rows, K) and dD (rows, N) f16 or bf16, contiguous rows, base and pitch multiples of 16 bytes; dB
  * (groups, N, K) f32 or the operands' type. */
 int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const moye_tensor_t* dD, const moye_tensor_t* A,
                                 const int32_t* offsets, float alpha, float beta, void* stream);

@@ -400,3 +400,16 @@ def test_under_the_debug_build(dev):
                           os.path.join(here, "test_gpu_grouped.py"), os.path.join(here, "test_gpu_lora.py")], capture_output=True, text=True,
                          env=dict(os.environ, MOYE_B200_DEBUG="1"), timeout=600)
     assert res.returncode == 0 and " passed" in res.stdout, res.stdout[-3000:] + res.stderr[-1000:]
+
+
+@pytest.mark.parametrize("beta", [1.0, 0.5])
+def test_gradients_below_the_normal_range_accumulate(mb, dev, beta):
+    """Float32 outputs: subnormal products and old values are kept as they are (beta = 1 is added by the memory).  The
+    products are 64 and 128 times 2^-140, the old values multiples of 2^-148: every sum is exact."""
+    edge = torch.tensor([0, 64], dtype=torch.int32, device=dev)
+    x, y = torch.full((64, 128), 2.0 ** -70, device=dev).bfloat16(), torch.full((64, 64), 2.0 ** -70, device=dev).bfloat16()
+    for old in (0.0, 6.0 * 2.0 ** -148, -100.0 * 2.0 ** -148, -2.0 ** -126, 2.0 ** -126):
+        db = mb.gemm_grouped_grad_(torch.full((1, 64, 128), old, device=dev), y, x, edge, beta=beta)
+        d = mb.gemm_grouped_(torch.full((64, 64), old, device=dev), x, x.view(1, 64, 128), edge, beta=beta)
+        mb.synchronize_status(dev)
+        assert bool((db.double() == 2.0 ** -134 + beta * old).all()) and bool((d.double() == 2.0 ** -133 + beta * old).all())
