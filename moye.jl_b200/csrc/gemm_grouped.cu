@@ -753,6 +753,19 @@ static uint64_t row_pitch(const moye_tensor_t* t) {
   return t->shape[0] > 1 ? t->stride[0] * eb : (t->shape[1] * eb + 15) / 16 * 16;
 }
 
+// Weights of all groups as one matrix of rows, for `rows_overlap`: exact where the groups follow one another in the rows'
+// own pitch, else a row is all that lies between a group's ends.
+static moye_tensor_t weight_rows(const moye_tensor_t* t, int64_t inner, int64_t outer, int64_t pitch) {
+  moye_tensor_t m = *t;
+  m.rank = 2;
+  const bool even = t->shape[0] == 1 || t->stride[0] == outer * pitch;
+  m.shape[0] = even ? t->shape[0] * outer : t->shape[0];
+  m.shape[1] = even ? inner : (outer - 1) * pitch + inner;
+  m.stride[0] = even ? pitch : t->stride[0];
+  m.stride[1] = 1;
+  return m;
+}
+
 static int check_borders(const char* who, const int* offsets, int groups) {
   if (groups < 1 || groups > kMaxGemmGroups)
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d groups (got %d)", who, kMaxGemmGroups, groups);
@@ -784,6 +797,8 @@ int launch_gemm_grouped(moye_b200_ctx* h, const moye_tensor_t* D, const moye_ten
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: rows or groups of B overlap", who);
   if ((reinterpret_cast<uintptr_t>(B->ptr) & 15) != 0 || (outer > 1 && pitch % 8 != 0) || (G > 1 && B->stride[0] % 8 != 0))
     MOYE_FAIL(MOYE_ERR_MISALIGNED, "%s: B needs a base, a row pitch and a group pitch that are multiples of 16 bytes", who);
+  const moye_tensor_t weights = weight_rows(B, inner, outer, outer > 1 ? pitch : inner);
+  if (rows_overlap(D, A) || rows_overlap(D, &weights)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: D overlaps an operand", who);
   const int ob = dtype_bytes(D->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;
@@ -835,6 +850,8 @@ int launch_gemm_grouped_grad(moye_b200_ctx* h, const moye_tensor_t* dB, const mo
   if (int rc = check_row_operand(who, "dD", dD)) return rc;
   if ((K > 1 && dB->stride[2] != 1) || (N > 1 && dB->stride[1] < K) || (G > 1 && dB->stride[0] < (N - 1) * dB->stride[1] + K))
     MOYE_FAIL(MOYE_ERR_UNSUPPORTED_LAYOUT, "%s: dB needs contiguous rows, and rows and groups that do not overlap", who);
+  const moye_tensor_t weights = weight_rows(dB, K, N, N > 1 ? dB->stride[1] : K);
+  if (rows_overlap(&weights, dD) || rows_overlap(&weights, A)) MOYE_FAIL(MOYE_ERR_INVALID_ARG, "%s: dB overlaps an operand", who);
   const int ob = dtype_bytes(dB->dtype);
   GroupedArgs a = {};
   a.rows = (int)R;

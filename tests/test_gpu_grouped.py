@@ -413,3 +413,34 @@ def test_gradients_below_the_normal_range_accumulate(mb, dev, beta):
         d = mb.gemm_grouped_(torch.full((64, 64), old, device=dev), x, x.view(1, 64, 128), edge, beta=beta)
         mb.synchronize_status(dev)
         assert bool((db.double() == 2.0 ** -134 + beta * old).all()) and bool((d.double() == 2.0 ** -133 + beta * old).all())
+
+
+def test_outputs_over_operands_are_refused(mb, dev):
+    """Tiles are written while others still read: an output that shares memory with an operand would depend on the order."""
+    rows, width, groups = 48, 64, 3
+    edge = torch.tensor([0, 5, 20, 48], dtype=torch.int32, device=dev)
+    flat = torch.zeros(4 * groups * width * width, dtype=torch.bfloat16, device=dev)
+    x, w = flat[:rows * width].view(rows, width), flat[rows * width:][:groups * width * width].view(groups, width, width)
+    free = flat[2 * groups * width * width:]
+    y, g = free[:rows * width].view(rows, width), free[rows * width:][:groups * width * width].view(groups, width, width)
+    mb.gemm_grouped_(y, x, w, edge)
+    mb.gemm_grouped_(y, x, w.transpose(1, 2), edge)
+    mb.gemm_grouped_grad_(g, y, x, edge)
+    shifted = flat[8:8 + rows * width].view(rows, width)
+    for call in (lambda: mb.gemm_grouped_(x, x, w, edge), lambda: mb.gemm_grouped_(shifted, x, w, edge),
+                 lambda: mb.gemm_grouped_(w[2, :48], x, w, edge), lambda: mb.gemm_grouped_(w[2, :48], x, w.transpose(1, 2), edge),
+                 lambda: mb.gemm_grouped_grad_(g, y, g[1, :48], edge), lambda: mb.gemm_grouped_grad_(g, g[2, 16:], x, edge),
+                 lambda: mb.gemm_grouped_grad_(w, y, shifted, edge)):
+        with pytest.raises(mb.MoyeError) as e:
+            call()
+        assert e.value.code == -1, str(e.value)
+    # beside one another in a wider array: rows of A and D, weights and their gradient
+    gen = torch.Generator(device=dev).manual_seed(2)
+    both = torch.randn(rows, 2 * width, generator=gen, device=dev).bfloat16()
+    ws = torch.randn(groups, width, 2 * width, generator=gen, device=dev).bfloat16()
+    want = mb.gemm_grouped_(y, both[:, :width].contiguous(), ws[:, :, :width].contiguous(), edge)
+    mb.gemm_grouped_(both[:, width:], both[:, :width], ws[:, :, :width], edge)
+    assert torch.equal(both[:, width:], want)
+    mb.gemm_grouped_grad_(ws[:, :, width:], want, both[:, :width], edge)
+    assert torch.equal(ws[:, :, width:], mb.gemm_grouped_grad_(g, want, both[:, :width].contiguous(), edge))
+    mb.synchronize_status(dev)
