@@ -403,10 +403,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
           const int kbs = tile.k_blocks, valid = tile.nrows - (kbs - 1) * BK;
           if (kbs > 0 && valid < BK) {
             const int stage = (pos + kbs - 1) % STAGES;
-            bool ok = true;
-            if (lane == 0) ok = mbar_wait(&tail[stage], (phases >> stage) & 1, a.status, SITEG_FIX_TAIL);
-            ok = __shfl_sync(~0u, ok, 0);
-            if (!ok) break;
+            // every lane waits: it is the wait that orders a lane's stores behind the loads that they overwrite
+            if (!__all_sync(~0u, mbar_wait(&tail[stage], (phases >> stage) & 1, a.status, SITEG_FIX_TAIL))) break;
             phases ^= 1u << stage;
             uint8_t* sl = smem + stage * STAGE_BYTES;
             for (int c = 0; c < 2 + (tile.width / 2 + 63) / 64; ++c)
