@@ -643,8 +643,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
               } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  if (i * 4 < live)
-                    for (int k = 0; x + k < a.lanes; ++k) p[i * 4 * a.ld + k] = reinterpret_cast<const OutT*>(&w[i])[k];
+#pragma unroll
+                  for (int k = 0; k < 7; ++k)  // constant indices: `w` stays in registers
+                    if (i * 4 < live && x + k < a.lanes) p[i * 4 * a.ld + k] = reinterpret_cast<const OutT*>(&w[i])[k];
               }
             }
           } else {
