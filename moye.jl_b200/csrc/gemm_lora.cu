@@ -71,10 +71,10 @@ lora_row_kernel(const LoraArgs g) {
   if (g.offsets) {
     // the first request that ends behind the row, unless the row lies before all of them
     if (tid == 0) found = g.requests;
+    const int first = __ldg(g.offsets);
     __syncthreads();
-    if (g.offsets[0] <= row)
-      for (int q = tid; q < g.requests; q += kLoraThreads)
-        if (row < g.offsets[q + 1]) atomicMin(&found, q);
+    for (int q = tid; q < g.requests; q += kLoraThreads)
+      if (row < g.offsets[q + 1]) atomicMin(&found, first <= row ? q : g.requests);
     __syncthreads();
   } else if (tid == 0) {
     found = row;
