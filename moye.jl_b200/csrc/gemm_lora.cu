@@ -615,7 +615,9 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       };
       const int turn = my_row % (rsteps * 4);  // of this row's units in `parts`
       float down = 1.f, most = 0.f;
-      auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))); };
+      // of the finite values: beside an infinity they have to stay finite, or their signs would meet the infinity's
+      auto finite = [](float x) { return isinf(x) ? 0.f : fabsf(x); };
+      auto largest = [&](const float4& x) { most = fmaxf(most, fmaxf(fmaxf(finite(x.x), finite(x.y)), fmaxf(finite(x.z), finite(x.w)))); };
       if (RANGE && C == 1) {
         each_4([&](int, const float4& x) { largest(x); });
         row_max[set * 128 + my_row] = most;

@@ -344,3 +344,24 @@ def test_columns_of_one_wider_array(mb, dev, case):
         with pytest.raises(mb.MoyeError) as e:
             mb.gemm_lora_(d if kw["C"] is not None else wide[:, k - 8:k + n - 8], xs, a, b, w, edge, scales, **kw)
         assert e.value.code == -1
+
+
+@pytest.mark.parametrize("case", range(len(SCALED)))
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_an_infinite_factor_beside_large_values(mb, dev, kind, case):
+    """An adapter with one infinite element: its product of rank R is infinite beside finite ones above the range of f16
+    and of the other sign, and the sum is infinite, not undefined.  Requests of the other adapter have finite sums."""
+    offsets, k, n, rank = SCALED[case]
+    rows, requests = offsets[-1], len(offsets) - 1
+    x, a, b = (torch.zeros(*s, dtype=DT[kind], device=dev) for s in ((rows, k), (2, rank, k), (2, n, rank)))
+    x[:, 0], x[:, 1] = 1.0, 256.0
+    a[0, 0, 0], a[1, 0, 0], a[:, 1:, 1] = float("inf"), 1.0, 32768.0   # the first product infinite or 1, the others 2^23
+    b[:] = -1.0
+    b[:, :, 0] = 1.0
+    which = (torch.arange(requests, device=dev) % 2).to(torch.int32)
+    d = mb.gemm_lora_(torch.zeros(rows, n, device=dev), x, a, b, which, torch.tensor(offsets, dtype=torch.int32, device=dev))
+    mb.synchronize_status(dev)
+    mine = which.repeat_interleave(torch.tensor(offsets, device=dev).diff())
+    assert bool((d[mine == 0] == float("inf")).all())
+    # 1 - (R - 1) 2^23, a sum of R terms in fp32: off by at most (R + 4) * 2^-23 of the magnitudes
+    assert bool(((d[mine == 1].double() - (1 - (rank - 1) * 2.0 ** 23)).abs() <= (rank + 4) * 2.0 ** -23 * rank * 2.0 ** 23).all())
