@@ -196,6 +196,38 @@ inline int configure_once(moye_b200_ctx* h, K kernel, int smem_bytes) {
   return MOYE_OK;
 }
 
+// Clusters of `ctas` CTAs of a kernel with `smem` bytes each that this handle's device holds at once (0: it takes none of
+// that size), found out once per handle: the answer, and the attribute that sizes above 8 need, belong to its device.
+template <typename K>
+inline int clusters_that_fit(moye_b200_ctx* h, K kernel, int ctas, int threads, size_t smem) {
+  const uint64_t key = reinterpret_cast<uint64_t>(kernel) * 16 + (ctas - 1);
+  {
+    std::lock_guard<std::mutex> lk(h->mu);
+    auto it = h->cluster_fit.find(key);
+    if (it != h->cluster_fit.end()) return it->second;
+  }
+  cudaLaunchConfig_t probe = {};
+  probe.gridDim = dim3((unsigned)ctas);
+  probe.blockDim = dim3((unsigned)threads);
+  probe.dynamicSmemBytes = smem;
+  cudaLaunchAttribute size[1];
+  size[0].id = cudaLaunchAttributeClusterDimension;
+  size[0].val.clusterDim.x = ctas;
+  size[0].val.clusterDim.y = 1;
+  size[0].val.clusterDim.z = 1;
+  probe.attrs = size;
+  probe.numAttrs = 1;
+  int fit = 0;
+  if ((ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+      cudaOccupancyMaxActiveClusters(&fit, kernel, &probe) != cudaSuccess) {
+    (void)cudaGetLastError();
+    fit = 0;
+  }
+  std::lock_guard<std::mutex> lk(h->mu);
+  h->cluster_fit[key] = fit;
+  return fit;
+}
+
 // Grows the handle-owned workspace to at least `bytes` (never shrinks).
 int ensure_workspace(moye_b200_ctx* h, size_t bytes);
 // Ticket areas at the front of both stream-K scratch buffers (zero whenever no kernel is running).

@@ -67,15 +67,30 @@ __device__ __forceinline__ void tile_coord(int t, int m_tiles, int n_tiles, int 
   if (grp & 1) ni = n_tiles - 1 - ni;  // serpentine: a new group starts on the B tiles the last one ended on
 }
 
-// Barrier `id` over 128 threads that also ands a flag of each.
-__device__ __forceinline__ bool all_of_128(int id, bool mine) {
+// Barrier `id` over THREADS threads that also ands a flag of each: they go on or give up together.
+template <int THREADS>
+__device__ __forceinline__ bool all_of(int id, bool mine) {
   int r;
   asm volatile(
-      "{\n.reg .pred p, q;\nsetp.ne.s32 q, %2, 0;\nbar.red.and.pred p, %1, 128, q;\nselp.s32 %0, 1, 0, p;\n}\n"
+      "{\n.reg .pred p, q;\nsetp.ne.s32 q, %2, 0;\nbar.red.and.pred p, %1, %3, q;\nselp.s32 %0, 1, 0, p;\n}\n"
       : "=r"(r)
-      : "r"(id), "r"((int)mine)
+      : "r"(id), "r"((int)mine), "n"(THREADS)
       : "memory");
   return r != 0;
+}
+
+// Two values rounded by one instruction, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+  const __half2 x = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 
 template <typename OutT>

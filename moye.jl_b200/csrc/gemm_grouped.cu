@@ -196,20 +196,6 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
-// Two values rounded by one instruction, the first in the low half.
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
-  const __half2 x = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-template <>
-__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-
 // Float32 tiles leave through two staging tiles a warp in turn (those gradients in Float32: 193 -> 184 us), 16-bit ones
 // through one a warp, two for the pair.  What is left of shared memory holds 5 stages of operands, or 6 (16-bit with 5: 1 to
 // 2 % slower on long sums).
@@ -430,7 +416,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
     uint8_t* my_epi = epi + (PROMOTE ? warp - 4 : (warp - 4) >> 1 << 1) * (EPI_BUFS * EPI_BUF);
     int buf = 0, lt = 0;
     bool ok = true;
-    while (ok && all_of_128(1 + set, ring.take(tile))) {
+    while (ok && all_of<128>(1 + set, ring.take(tile))) {
       if (lane == 0) ring.leave();
       else ++ring.n;
       const int kbs = tile.k_blocks;
@@ -456,7 +442,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_consta
       };
       auto arrived = [&]() {  // waits for the accumulator of the next run
         // the four warps of a set go on or give up together: they meet again at the barriers of the stores
-        ok = all_of_128(1 + set, mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC));
+        ok = all_of<128>(1 + set, mbar_wait(&acc_full[lt & 1], (lt >> 1) & 1, a.status, SITEG_EPI_ACC));
         tc_fence_after_sync();
         return ok;
       };

@@ -242,28 +242,8 @@ __device__ __forceinline__ void st_remote_u32x2(uint32_t cluster_addr, uint32_t 
   asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(cluster_addr), "r"(x), "r"(y) : "memory");
 }
 // The epilogue's 256 threads meet, all going on or giving up together.
-__device__ __forceinline__ bool lora_epi_all(bool mine) {
-  int r;
-  asm volatile(
-      "{\n.reg .pred p, q;\nsetp.ne.s32 q, %1, 0;\nbar.red.and.pred p, 1, 256, q;\nselp.s32 %0, 1, 0, p;\n}\n"
-      : "=r"(r)
-      : "r"((int)mine)
-      : "memory");
-  return r != 0;
-}
+__device__ __forceinline__ bool lora_epi_all(bool mine) { return all_of<256>(1, mine); }
 
-template <typename T>
-__device__ __forceinline__ uint32_t lora_pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t lora_pack2<__half>(float a, float b) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t lora_pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 // One 16-byte word of outputs: the input word plus `up` times EPV accumulators.
 __device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, float up, float*) {
   return make_uint4(__float_as_uint(fmaf(__uint_as_float(v[0]), up, __uint_as_float(c.x))), __float_as_uint(fmaf(__uint_as_float(v[1]), up, __uint_as_float(c.y))),
@@ -275,7 +255,7 @@ __device__ __forceinline__ uint4 lora_add(const uint4& c, const uint32_t* v, flo
   lora_unpack<T>(c, f);
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = fmaf(__uint_as_float(v[e]), up, f[e]);
-  return make_uint4(lora_pack2<T>(f[0], f[1]), lora_pack2<T>(f[2], f[3]), lora_pack2<T>(f[4], f[5]), lora_pack2<T>(f[6], f[7]));
+  return make_uint4(pack_pair<T>(f[0], f[1]), pack_pair<T>(f[2], f[3]), pack_pair<T>(f[4], f[5]), pack_pair<T>(f[6], f[7]));
 }
 
 // The powers of two that bring a row whose magnitudes stay below `m` to magnitude 1 (`down`) and back (`up`); 1 where m
@@ -561,7 +541,7 @@ lora_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       float r[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
-        const uint32_t w0 = lora_pack2<T>(r[0], r[1]), w1 = lora_pack2<T>(r[2], r[3]);
+        const uint32_t w0 = pack_pair<T>(r[0], r[1]), w1 = pack_pair<T>(r[2], r[3]);
         const float2 f0 = lora_pair<T>(w0), f1 = lora_pair<T>(w1);
         const float f[4] = {f0.x, f0.y, f1.x, f1.y};
 #pragma unroll
@@ -839,33 +819,7 @@ static int launch_lora_tile(moye_b200_ctx* h, const LoraArgs& g, int dtype, int 
   int ctas = kLoraCtas < kbs ? kLoraCtas : kbs;
   for (; ctas > 1; --ctas) {
     if (tiles * ctas > h->num_sms) continue;
-    const uint64_t key = reinterpret_cast<uint64_t>(kern) * 16 + ctas;
-    int fit = -1;
-    {
-      std::lock_guard<std::mutex> lk(h->mu);
-      auto it = h->cluster_fit.find(key);
-      if (it != h->cluster_fit.end()) fit = it->second;
-    }
-    if (fit < 0) {
-      cudaLaunchConfig_t probe = {};
-      probe.gridDim = dim3((unsigned)ctas);
-      probe.blockDim = dim3(kLoraTileThreads);
-      probe.dynamicSmemBytes = smem;
-      cudaLaunchAttribute size[1];
-      size[0].id = cudaLaunchAttributeClusterDimension;
-      size[0].val.clusterDim.x = ctas;
-      size[0].val.clusterDim.y = 1;
-      size[0].val.clusterDim.z = 1;
-      probe.attrs = size;
-      probe.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&fit, kern, &probe) != cudaSuccess) {
-        (void)cudaGetLastError();
-        fit = 0;
-      }
-      std::lock_guard<std::mutex> lk(h->mu);
-      h->cluster_fit[key] = fit;
-    }
-    if (fit >= tiles) break;
+    if (clusters_that_fit(h, kern, ctas, kLoraTileThreads, smem) >= tiles) break;
   }
   LoraTileArgs p = {};
   p.g = g;

@@ -204,37 +204,7 @@ int launch_group_rows(moye_b200_ctx* h, const moye_tensor_t* ids, int groups, in
   // One CTA while its warps have at most 4 batches of 32 choices each, then 8; beyond 32768 choices 16, if the device holds
   // a cluster of 16 (131072 choices, 128 groups: 8 CTAs are bound by their own instructions)
   unsigned ctas = n > 4096 ? 8 : 1;
-  if (n > 32768) {
-    // found out once per handle: the attribute and the answer belong to its device
-    const uint64_t key = reinterpret_cast<uint64_t>(group_rows_kernel) * 16 + 15;
-    int clusters = -1;
-    {
-      std::lock_guard<std::mutex> lk(h->mu);
-      auto it = h->cluster_fit.find(key);
-      if (it != h->cluster_fit.end()) clusters = it->second;
-    }
-    if (clusters < 0) {
-      cudaLaunchConfig_t probe = {};
-      probe.gridDim = dim3(16);
-      probe.blockDim = dim3(kGroupThreads);
-      probe.dynamicSmemBytes = (kGroupWarps + 2) * kMaxGroups * 4;
-      cudaLaunchAttribute size[1];
-      size[0].id = cudaLaunchAttributeClusterDimension;
-      size[0].val.clusterDim.x = 16;
-      size[0].val.clusterDim.y = 1;
-      size[0].val.clusterDim.z = 1;
-      probe.attrs = size;
-      probe.numAttrs = 1;
-      if (cudaFuncSetAttribute(group_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-          cudaOccupancyMaxActiveClusters(&clusters, group_rows_kernel, &probe) != cudaSuccess) {
-        (void)cudaGetLastError();
-        clusters = 0;
-      }
-      std::lock_guard<std::mutex> lk(h->mu);
-      h->cluster_fit[key] = clusters;
-    }
-    if (clusters > 0) ctas = 16;
-  }
+  if (n > 32768 && clusters_that_fit(h, group_rows_kernel, 16, kGroupThreads, (kGroupWarps + 2) * kMaxGroups * 4) > 0) ctas = 16;
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kGroupThreads);
   cfg.dynamicSmemBytes = smem;

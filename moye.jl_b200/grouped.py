@@ -90,7 +90,7 @@ def _arg(x, rank, what):
             raise _lib.MoyeError(-3, f"{what} must have one stride per mode, got layout {l}")
         shape, dtype, where = tuple(int(m.shape) for m in modes), x.dtype, x.device
         if where.type == "cuda" and len(shape) == rank:
-            return _PACK[rank].pack(x.ptr, dtype, rank, *shape, *(int(m.stride) for m in modes)), where.index
+            return _lib.pack_tensor(x.ptr, dtype, shape, [int(m.stride) for m in modes]), where.index
     else:
         raise TypeError(f"{what} must be a torch.Tensor or a MoYeArray, got {type(x).__name__}")
     if where.type != "cuda":
@@ -183,7 +183,7 @@ def group_rows_(plan, ids, stream=None):
 
 def gather_rows_(dst, src, plan, stream=None):
     """dst[p] = src[plan.order[p] // choices] for the kept positions; rows of dst behind them are left as they were.
-    src (tokens, width), dst (tokens * choices, width); any element type, contiguous rows.  Its gradient is
+    src (tokens, width), dst (tokens * choices, width); any element type a MoYeArray takes, contiguous rows.  Its gradient is
     `combine_rows_(dsrc, ddst, plan)`."""
     if _lib.calls is not None and _taken(_lib.calls.gather_rows(dst, src, plan._buf, plan.tokens, plan.choices, stream)):
         return dst
