@@ -96,6 +96,7 @@ def test_compiled_calls_for_another_torch_are_not_loaded(mb, tmp_path, monkeypat
     assert mb._lib._load_calls(lib) is not None
     for a, b in ((torch.__version__, "0" * len(torch.__version__)), (sys.implementation.cache_tag, "x" * len(sys.implementation.cache_tag)),
                  (f"library {lib.moye_b200_version()}", "library 999")):
+        other.unlink()  # a file of its own: the one before may be mapped
         other.write_bytes(own.replace(marker, marker.replace(a.encode(), b.encode())))
         assert mb._lib._load_calls(lib) is None
     monkeypatch.setattr(build, "OUT_CALLS", str(other))
