@@ -336,7 +336,8 @@ int moye_b200_gemm_grouped_grad(moye_handle_t h, const moye_tensor_t* dB, const 
  * one), or q = i when offsets is NULL (then requests = rows).  X (rows, K), A (count, R, K), B (count, N, R), C and D (rows, N).  An adapter number outside
  * 0..count-1 means none: D[i] = C[i].  Rows outside every request are left as they were.  C NULL or C = D: in place.
  * scales: one float per adapter, or NULL for 1.  The product of rank R is kept in fp32, or as a sum of 16-bit parts that
- * carries 16 bits or more of it (24 for bf16 with f32 outputs; f16 relative to the row's largest).  X, A, B
+ * carries 16 bits or more of it (24 for bf16 with f32 outputs; f16 relative to the row's largest); which of the two depends on
+ * rows, requests, rank and extents, so that a row's last bit may differ from batch to batch.  X, A, B
  * all f16 or all bf16; C and D both f32 or both the operands' type; R a multiple of 8 from 8 to 128 (pad with zeros),
  * K a multiple of 8; base and pitches of X, A, B multiples of 16 bytes. */
 int moye_b200_gemm_lora(moye_handle_t h, const moye_tensor_t* D, const moye_tensor_t* X, const moye_tensor_t* A,

@@ -23,10 +23,12 @@
 // at 1000, plain fp32 sums 6e-7).  Float32 outputs are therefore summed in runs of 512 that the epilogue adds up in
 // registers, rounding to nearest (`PROMOTE`).
 //
-// Bound by memory where groups are short (128 rows in 64 groups, 2048 x 2048 bf16: 67 us, 6.5 TB/s), by the tensor cores
-// where they are long (32768 rows in 32 uneven groups, 4096 x 2048: 422 us, 1300 TFLOP/s, equal groups 1450, the dense pair
-// kernel 1540 on one weight; gradient of the weights 467 us).  What uneven groups lose are last tiles that are too narrow
-// for the operand loads (256 + N cycles a block against 2 N of arithmetic) and a partly filled last wave.
+// Bound by memory where groups are short (128 rows in 64 groups, 2048 x 2048 bf16: 66 us captured, 6.5 TB/s), by the tensor
+// cores where they are long.  32768 rows, 4096 x 2048, in a burst / for seconds at the power cap of 1000 W: one group 386 /
+// 452 us (the dense pair kernel 382 / 446), 32 equal groups 413 / 482, 32 uneven ones 448 / 522 (1227 / 1054 TFLOP/s); the
+// gradient of their rows 466 / 551, of the weights 479 / 569.  Equal groups pay for 32 weights from memory.  What uneven
+// groups lose are last tiles that are too narrow for the operand loads (256 + N cycles a block against 2 N of arithmetic)
+// and a partly filled last wave.
 #include <cstring>
 
 #include "gemm_common.cuh"

@@ -9,7 +9,8 @@
 //
 // The product of rank R between the two factors never leaves the chip: a thread-block cluster takes a row, CTA c of it
 // a slice of K for the first factor; the partial R-vectors meet through distributed shared memory (fp32, summed in CTA
-// order, so the result does not depend on timing); then CTA c takes a slice of N for the second factor.
+// order, so the result does not depend on timing); then CTA c takes a slice of N for the second factor.  82 to 86 clusters
+// are resident at once (5 CTAs per SM by registers): K = N = 4096, R = 16, up to 82 rows 5.5 us, 128 rows two waves, 9.5.
 #include "gemm_common.cuh"
 
 namespace moye {
@@ -205,7 +206,8 @@ lora_row_kernel(const LoraArgs g) {
 // memory) with A[a] (R columns); with C > 1 the fp32 parts meet through distributed shared memory, CTA c summing 1 / C of
 // the rows in CTA order and handing the result to all; every CTA then multiplies it with its 128-column chunks of B[a] and
 // adds C.  The product of rank R enters the second multiplication as a sum of 16-bit parts: two parts carry 16 (bf16)
-// or 22 (f16) bits, a sixteenth of an output step or less; bf16 operands with a Float32 output take three (24 bits).
+// or 22 (f16) bits, off by 2^-17 of a product where the output's rounding takes 2^-9 (a third part moves 0.04 % of bf16
+// outputs by a step, for 9 % of the time); bf16 operands with a Float32 output take three (24 bits).
 // A Float32 output also has its sums over K taken out of tensor memory every 512 products, as in gemm_grouped.cu.
 // f16 has not the range of the fp32 sums (65504, and steps of 2^-24 near zero): a row is brought to magnitude 1 by a power
 // of two first, which the epilogue takes back.
